@@ -15,7 +15,7 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "point_slam_amd", "csrc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-munsafe-fp-atomics",
-         "--cuda-device-only", "-S"]
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "--cuda-device-only", "-S"]
 KEYS = [".vgpr_count", ".agpr_count", ".vgpr_spill_count", ".sgpr_count", ".sgpr_spill_count",
         ".private_segment_fixed_size", ".group_segment_fixed_size", ".max_flat_workgroup_size"]
 
