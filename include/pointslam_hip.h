@@ -352,6 +352,38 @@ int psl_keyframe_overlap_sync(const float* rays_o, const float* rays_d, const fl
                               int32_t n_samples, const float* c2w_host, int32_t n_kf, psl_cam_intr cam, float edge,
                               float* percent_host, void* stream);
 
+/* ---- feature rows held in 8 or 4 bits (no reference counterpart: the reference keeps every feature in fp32) ----------
+ * A row is heads x dim values in groups of `group`; a group stands for code * scale with one fp32 scale = max|x| / Q,
+ * Q = 127 (int8), 7 (int4, two codes to a byte, the even one low), 448 (e4m3, OCP); a code is the representable value
+ * NEAREST to the exact x / scale, ties to even.  A group of zeros has scale 0; a group with an infinite or NaN value has
+ * scale NaN and reads back as NaN.  ABI v8.
+ *   psl_rows_write : values[i] -> row rows[i] (or first + i when rows is NULL).  Ids outside [0, capacity) write nothing
+ *                    (padding: -1).  The same id more than once: with `owner` ([capacity] int32 scratch, any contents) the
+ *                    largest i wins; with owner NULL the caller vouches that the ids are distinct.
+ *   psl_rows_read  : the values of row rows[i] -> values[i], rounded once to dtype; ids outside [0, capacity) give zeros.
+ * Rows that are not named stay as they were.  heads, dim <= 4096; group <= 1024 divides dim (even for int4). */
+enum psl_dtype { PSL_F32 = 0, PSL_BF16 = 1, PSL_F16 = 2 };
+enum psl_row_format { PSL_ROWS_INT8 = 0, PSL_ROWS_E4M3 = 1, PSL_ROWS_INT4 = 2 };
+typedef struct psl_rows_args {
+  int32_t format;               /* psl_row_format */
+  int32_t dtype;                /* psl_dtype of `values` */
+  int32_t heads, dim, group;
+  int32_t rows_bits;            /* 32 or 64: width of the ids in `rows` */
+  int64_t n;                    /* rows of this call (0: nothing happens) */
+  int64_t capacity;             /* rows of the store */
+  int64_t first;                /* rows == NULL: rows [first, first + n) of the store */
+  const void* rows;             /* [n] row ids (device) or NULL */
+  void* values;                 /* [n][heads][dim], innermost contiguous; read by psl_rows_write, written by psl_rows_read */
+  int64_t value_row_stride, value_head_stride;   /* elements */
+  void* codes;                  /* row r at r * codes_row_stride bytes: [heads][dim * bits / 8] */
+  int64_t codes_row_stride;     /* bytes; codes and scales may lie interleaved in one record per row */
+  float* scales;                /* row r at r * scales_row_stride floats: [heads][dim / group] */
+  int64_t scales_row_stride;
+  int32_t* owner;               /* psl_rows_write only, see above */
+} psl_rows_args;
+int psl_rows_write(const psl_rows_args* a, void* stream);
+int psl_rows_read(const psl_rows_args* a, void* stream);
+
 /* ---- multi-GPU exchange ("periodic RCCL all-gather over xGMI of newly-added
  * neural points").  The reference has no distributed code (no NCCL / torch.distributed call anywhere in it); frames are
  * partitioned one per GPU and the replicas exchange record blocks.  librccl is resolved with dlopen at the first call.

@@ -17,10 +17,11 @@ class PslError(RuntimeError):
     pass
 
 
-ABI_VERSION = 7     # include/pointslam_hip.h: psl_abi_version(); v2: psl_render_args.z_vals; v3: exposure blocks,
+ABI_VERSION = 8     # include/pointslam_hip.h: psl_abi_version(); v2: psl_render_args.z_vals; v3: exposure blocks,
 #                     full-image pixel indices in psl_track_args, step0_params in psl_map_args; v4: psl_dedupe_count / psl_dedupe_blocks,
 #                     psl_comm_* / psl_allgather_new_points (RCCL inside the library), psl_map_args refinement fields;
-#                     v5: psl_allgather_decide (rank-invariant capacity decision), psl_selftest_math; v6: psl_comm_reserve, psl_pose_const_speed, psl_selftest_traffic
+#                     v5: psl_allgather_decide (rank-invariant capacity decision), psl_selftest_math; v6: psl_comm_reserve, psl_pose_const_speed, psl_selftest_traffic;
+#                     v8: psl_rows_write / psl_rows_read (feature rows in 8 or 4 bits)
 EXPOSURE_DIM, EXPOSURE_MLP_FLOATS = 8, 2700
 
 
@@ -85,6 +86,18 @@ class psl_map_args(C.Structure):
                 ("step0_params", C.c_int32)]
 
 
+class psl_rows_args(C.Structure):
+    _fields_ = [("format", C.c_int32), ("dtype", C.c_int32), ("heads", C.c_int32), ("dim", C.c_int32), ("group", C.c_int32),
+                ("rows_bits", C.c_int32), ("n", C.c_int64), ("capacity", C.c_int64), ("first", C.c_int64),
+                ("rows", C.c_void_p), ("values", C.c_void_p), ("value_row_stride", C.c_int64),
+                ("value_head_stride", C.c_int64), ("codes", C.c_void_p), ("codes_row_stride", C.c_int64),
+                ("scales", C.c_void_p), ("scales_row_stride", C.c_int64), ("owner", C.c_void_p)]
+
+
+# psl_dtype, psl_row_format
+F32, BF16, F16 = 0, 1, 2
+ROWS_INT8, ROWS_E4M3, ROWS_INT4 = 0, 1, 2
+
 # psl_render_flags
 STAGE_COLOR, PTS_GRAD, PARAM_GRAD, FEAT_GRAD, NO_SIGMOID, HAS_AFFINE = 1, 2, 4, 8, 16, 32
 
@@ -146,6 +159,8 @@ _SIGS = {
     "psl_map_iters": (C.c_int, [C.c_void_p, C.POINTER(psl_map_args), C.c_void_p]),
     "psl_frustum_select_sync": (C.c_int, [C.c_void_p, C.POINTER(C.c_float), psl_cam_intr, C.c_void_p, C.c_float,
                                           C.c_float, C.c_void_p, C.c_void_p, C.POINTER(C.c_int), C.c_void_p]),
+    "psl_rows_write": (C.c_int, [C.POINTER(psl_rows_args), C.c_void_p]),
+    "psl_rows_read": (C.c_int, [C.POINTER(psl_rows_args), C.c_void_p]),
     "psl_sync": (C.c_int, [C.c_void_p, C.c_void_p]),
     "psl_profile_enable": (C.c_int, [C.c_void_p, C.c_int]),
     "psl_knn_candidates": (C.c_int64, [C.c_void_p]),

@@ -1,0 +1,132 @@
+"""QuantizedRows: feature rows held in 8 or 4 bits, quantised as they are written and expanded as they are read
+(psl_rows_write / psl_rows_read; no reference counterpart -- the reference keeps every feature row in fp32).
+
+A row is `heads` x `dim` values -- the geometry and the colour feature of a neural point are two heads of 32 -- and every
+`group` of values shares one fp32 scale:
+
+    scale = max|x| / Q     Q = 127 ("int8"), 7 ("int4"), 448 ("e4m3")        code = nearest(x / scale), ties to even
+    value = code * scale   rounded once to the type that is read
+
+so a value is off by at most half a code step (scale / 2 for the integer formats, 2^-4 of the value for e4m3's normal
+range).  A group with an infinite or NaN value reads back as NaN throughout.  dist.FrameParallelSync(wire=...) sends new
+points and trained rows in this form, checkpoint.checkpoint_dict(feature_format=...) saves them in it.
+There is no torch fallback.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Optional
+
+import torch
+
+from . import _lib
+
+FORMATS = {"int8": _lib.ROWS_INT8, "e4m3": _lib.ROWS_E4M3, "int4": _lib.ROWS_INT4}
+BITS = {"int8": 8, "e4m3": 8, "int4": 4}
+_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _check_layout(heads, dim, fmt, group):
+    if fmt not in FORMATS:
+        raise ValueError(f"row format {fmt!r}: one of {sorted(FORMATS)}")
+    if not (1 <= heads <= 4096 and 1 <= dim <= 4096 and 1 <= group <= 1024) or dim % group:
+        raise ValueError(f"heads {heads}, dim {dim}, group {group}: heads and dim up to 4096, group up to 1024 and a divisor of dim")
+    if BITS[fmt] == 4 and group % 2:
+        raise ValueError(f"two int4 codes share a byte: group {group} must be even")
+
+
+def _call(entry, values, rows, first, n, fmt, group, capacity, codes, codes_row_stride, scales, scales_row_stride, owner=None):
+    """One psl_rows_* call.  values [n, heads, dim], rows ids or None; codes / scales: tensors whose data_ptr is row 0."""
+    if values.device.type != "cuda":
+        raise _lib.PslError(f"{entry}: tensors on {values.device}; the kernels run on the GPU and have no host fallback")
+    a = _lib.psl_rows_args(format=FORMATS[fmt], dtype=_DTYPES[values.dtype], heads=values.shape[1], dim=values.shape[2],
+                           group=group, rows_bits=0 if rows is None else rows.element_size() * 8, n=n, capacity=capacity,
+                           first=first, rows=None if rows is None else rows.data_ptr(), values=values.data_ptr(),
+                           value_row_stride=values.stride(0), value_head_stride=values.stride(1), codes=codes.data_ptr(),
+                           codes_row_stride=codes_row_stride, scales=scales.data_ptr(), scales_row_stride=scales_row_stride,
+                           owner=None if owner is None else owner.data_ptr())
+    with torch.cuda.device(values.device):       # the launch belongs to the tensors' device and its current stream
+        _lib.check(getattr(_lib.lib(), entry)(C.byref(a), _lib.stream_ptr()), entry)
+
+
+class QuantizedRows:
+    """A store of `capacity` rows.  codes: uint8 [capacity, heads, dim * bits / 8], scales: fp32 [capacity, heads, dim / group];
+    rows that were never written read as zeros."""
+
+    def __init__(self, capacity: int, heads: int = 2, dim: int = 32, fmt: str = "int8", group: Optional[int] = None,
+                 device="cuda:0"):
+        group = dim if group is None else group
+        _check_layout(heads, dim, fmt, group)
+        if capacity < 0:
+            raise ValueError(f"capacity {capacity}")
+        self.capacity, self.heads, self.dim, self.fmt, self.group = int(capacity), heads, dim, fmt, group
+        self.device = torch.device(device)
+        if self.device.type == "cuda" and self.device.index is None:
+            self.device = torch.device("cuda", torch.cuda.current_device())
+        self.codes = torch.zeros(self.capacity, heads, dim * BITS[fmt] // 8, dtype=torch.uint8, device=self.device)
+        self.scales = torch.zeros(self.capacity, heads, dim // group, dtype=torch.float32, device=self.device)
+
+    def bytes_per_row(self) -> int:
+        return self.heads * (self.dim * BITS[self.fmt] // 8 + 4 * (self.dim // self.group))
+
+    def _rows(self, rows):
+        if not torch.is_tensor(rows) or rows.dtype not in (torch.int32, torch.int64) or rows.dim() != 1:
+            raise ValueError("rows: a one-dimensional int32 or int64 tensor")
+        if rows.device != self.device:
+            raise ValueError(f"rows on {rows.device}, the store on {self.device}")
+        return rows.contiguous()
+
+    def _range(self, first, n):
+        if first < 0 or n < 0 or first + n > self.capacity:
+            raise ValueError(f"rows [{first}, {first + n}) of a store of {self.capacity}")
+
+    def _args(self):
+        return (self.fmt, self.group, self.capacity, self.codes, self.codes.stride(0), self.scales, self.scales.stride(0))
+
+    def write(self, values: torch.Tensor, rows: Optional[torch.Tensor] = None, first: int = 0, distinct: bool = False):
+        """values [n, heads, dim] (fp32, bf16 or fp16) into rows `rows` [n], or into [first, first + n) when rows is None.
+        Ids outside the store (padding: -1) are skipped.  When an id comes more than once the last one wins;
+        `distinct=True` vouches that none does and saves that bookkeeping (two launches)."""
+        if values.dtype not in _DTYPES or values.dim() != 3 or tuple(values.shape[1:]) != (self.heads, self.dim):
+            raise ValueError(f"values: [n, {self.heads}, {self.dim}] in float32, bfloat16 or float16, got {tuple(values.shape)} {values.dtype}")
+        if values.device != self.device:
+            raise ValueError(f"values on {values.device}, the store on {self.device}")
+        n = values.shape[0]
+        values = values.detach()
+        if values.stride(2) != 1 or min(values.stride()) < 0:
+            values = values.contiguous()
+        owner = None
+        if rows is None:
+            self._range(first, n)
+        else:
+            rows = self._rows(rows)
+            if rows.shape[0] != n:
+                raise ValueError(f"{n} rows of values for {rows.shape[0]} ids")
+            if not distinct and n > 1:
+                owner = torch.empty(self.capacity, dtype=torch.int32, device=self.device)
+        if n and self.capacity:
+            _call("psl_rows_write", values, rows, first, n, *self._args(), owner)
+        return self
+
+    def read(self, rows: Optional[torch.Tensor] = None, first: int = 0, count: Optional[int] = None,
+             dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The values [n, heads, dim] of rows `rows`, or of [first, first + count) (to the end by default).  Ids outside the
+        store give zeros; the same id may come any number of times."""
+        if rows is None:
+            n = self.capacity - first if count is None else int(count)
+            self._range(first, n)
+        else:
+            rows = self._rows(rows)
+            n = rows.shape[0]
+        if out is None:
+            if dtype not in _DTYPES:
+                raise ValueError(f"dtype {dtype}: float32, bfloat16 or float16")
+            out = torch.empty(n, self.heads, self.dim, dtype=dtype, device=self.device)
+        elif (tuple(out.shape) != (n, self.heads, self.dim) or out.dtype not in _DTYPES or out.device != self.device
+              or out.stride(2) != 1 or out.requires_grad):
+            raise ValueError(f"out: [{n}, {self.heads}, {self.dim}] on {self.device}, contiguous rows, no gradient")
+        if n and self.capacity:
+            _call("psl_rows_read", out, rows, first, n, *self._args())
+        elif n:
+            out.zero_()
+        return out
