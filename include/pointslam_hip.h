@@ -384,6 +384,40 @@ typedef struct psl_rows_args {
 int psl_rows_write(const psl_rows_args* a, void* stream);
 int psl_rows_read(const psl_rows_args* a, void* stream);
 
+/* ---- draws of indices from scores (beside psl_topgrad_select_sync, whose set has a hard edge; no reference counterpart) --
+ * Row r holds n_cols scores s; entries that are masked out, NaN or -inf are not drawn.  With M the row's largest score,
+ * w = exp((s - M) / T).  In the order (score descending, index ascending):
+ *   top_k > 0 keeps the first top_k; top_p < 1 keeps the shortest prefix whose weights sum to at least top_p times the sum
+ *   after top_k (that product rounded to fp64; at least one entry); min_p > 0 keeps w >= min_p (at most 1).
+ * A draw with the caller's u in [0, 1) is the LOWEST index whose running sum of kept weights passes u * (sum of all kept);
+ * prob (may be NULL) is its weight over that sum.  T <= 0 or top_p <= 0: the first entry of the order.  A score of +inf
+ * takes all.  A row with no entry to draw gives index -1, prob 0.  Weights and sums are fp64 and of one fixed order.
+ * Per-row parameters are device arrays [n_rows]; a NULL one means the value for all rows beside it.  ABI v8.
+ * ws: psl_draw_ws_bytes bytes, 256-byte aligned, in use until the work on `stream` has finished. */
+typedef struct psl_draw_args {
+  int32_t n_rows, n_cols, n_draws;      /* n_rows <= 65535; draws per row */
+  int32_t dtype;                        /* psl_dtype of scores */
+  const void* scores;                   /* [n_rows][n_cols], entries of a row contiguous */
+  int64_t score_stride;                 /* elements between rows (0: one row of scores for all) */
+  const uint8_t* mask;                  /* 0 = not to be drawn; NULL: every entry may be */
+  int64_t mask_stride;                  /* bytes between rows (0: one mask for all) */
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  double temperature_all, top_p_all, min_p_all;
+  int32_t top_k_all;
+  int32_t reserved;                     /* 0 */
+  const float* u;                       /* [n_rows][n_draws] */
+  int64_t u_stride;                     /* floats between rows (0: the same numbers for all) */
+  int32_t* idx;                         /* [n_rows][n_draws] */
+  float* prob;                          /* [n_rows][n_draws] or NULL */
+  void* ws;
+  int64_t ws_bytes;
+} psl_draw_args;
+int64_t psl_draw_ws_bytes(int32_t n_rows, int32_t n_cols);
+int psl_draw_indices(const psl_draw_args* a, void* stream);
+
 /* ---- multi-GPU exchange ("periodic RCCL all-gather over xGMI of newly-added
  * neural points").  The reference has no distributed code (no NCCL / torch.distributed call anywhere in it); frames are
  * partitioned one per GPU and the replicas exchange record blocks.  librccl is resolved with dlopen at the first call.

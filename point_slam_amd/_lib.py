@@ -21,7 +21,7 @@ ABI_VERSION = 8     # include/pointslam_hip.h: psl_abi_version(); v2: psl_render
 #                     full-image pixel indices in psl_track_args, step0_params in psl_map_args; v4: psl_dedupe_count / psl_dedupe_blocks,
 #                     psl_comm_* / psl_allgather_new_points (RCCL inside the library), psl_map_args refinement fields;
 #                     v5: psl_allgather_decide (rank-invariant capacity decision), psl_selftest_math; v6: psl_comm_reserve, psl_pose_const_speed, psl_selftest_traffic;
-#                     v8: psl_rows_write / psl_rows_read (feature rows in 8 or 4 bits)
+#                     v8: psl_rows_write / psl_rows_read (feature rows in 8 or 4 bits), psl_draw_ws_bytes / psl_draw_indices (draws from scores)
 EXPOSURE_DIM, EXPOSURE_MLP_FLOATS = 8, 2700
 
 
@@ -94,6 +94,15 @@ class psl_rows_args(C.Structure):
                 ("scales", C.c_void_p), ("scales_row_stride", C.c_int64), ("owner", C.c_void_p)]
 
 
+class psl_draw_args(C.Structure):
+    _fields_ = [("n_rows", C.c_int32), ("n_cols", C.c_int32), ("n_draws", C.c_int32), ("dtype", C.c_int32),
+                ("scores", C.c_void_p), ("score_stride", C.c_int64), ("mask", C.c_void_p), ("mask_stride", C.c_int64),
+                ("temperature", C.c_void_p), ("top_k", C.c_void_p), ("top_p", C.c_void_p), ("min_p", C.c_void_p),
+                ("temperature_all", C.c_double), ("top_p_all", C.c_double), ("min_p_all", C.c_double),
+                ("top_k_all", C.c_int32), ("reserved", C.c_int32), ("u", C.c_void_p), ("u_stride", C.c_int64),
+                ("idx", C.c_void_p), ("prob", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64)]
+
+
 # psl_dtype, psl_row_format
 F32, BF16, F16 = 0, 1, 2
 ROWS_INT8, ROWS_E4M3, ROWS_INT4 = 0, 1, 2
@@ -161,6 +170,8 @@ _SIGS = {
                                           C.c_float, C.c_void_p, C.c_void_p, C.POINTER(C.c_int), C.c_void_p]),
     "psl_rows_write": (C.c_int, [C.POINTER(psl_rows_args), C.c_void_p]),
     "psl_rows_read": (C.c_int, [C.POINTER(psl_rows_args), C.c_void_p]),
+    "psl_draw_ws_bytes": (C.c_int64, [C.c_int32, C.c_int32]),
+    "psl_draw_indices": (C.c_int, [C.POINTER(psl_draw_args), C.c_void_p]),
     "psl_sync": (C.c_int, [C.c_void_p, C.c_void_p]),
     "psl_profile_enable": (C.c_int, [C.c_void_p, C.c_int]),
     "psl_knn_candidates": (C.c_int64, [C.c_void_p]),

@@ -53,6 +53,77 @@ def get_selected_index_with_grad(npc, H0, H1, W0, W1, n, image, ratio=15, gt_dep
     return torch.sort(sel[:n_sel.value].long()).values, grad_mag
 
 
+_DRAW_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask=None, with_prob=False):
+    """Draws of indices from rows of scores (psl_draw_indices; no reference counterpart: the reference takes pixels uniformly
+    or from the hard top-k of get_selected_index_with_grad).
+
+    scores [R, V] (fp32, bf16 or fp16; pixels of a frame, entries of a vocabulary), u [R, n] fp32 in [0, 1): n draws from
+    each row, with replacement -- the random numbers are the caller's, as everywhere in this package.  An entry weighs
+    exp((score - max) / temperature); top_k (0: off), top_p (1: off) and min_p (0: off) cut the tail, in that order, ties to
+    the lower index; temperature or a limit may be a number or a tensor [R].  `mask` (bool or uint8, [R, V] or [V]): entries
+    that may be drawn -- what the others hold, NaN included, does not matter.  A vector of scores and a vector u make one row.
+    Returns indices int32 [R, n] (-1 where a row has nothing to draw) and, with_prob, their probabilities fp32 [R, n] under
+    the cut distribution (what an importance weight divides by)."""
+    one = scores.dim() == 1
+    if one:
+        scores, u = scores.unsqueeze(0), u.unsqueeze(0)
+        mask = mask.unsqueeze(0) if mask is not None and mask.dim() == 1 else mask
+    if scores.dim() != 2 or scores.dtype not in _DRAW_DTYPES:
+        raise ValueError(f"scores: [rows, entries] in float32, bfloat16 or float16, got {tuple(scores.shape)} {scores.dtype}")
+    R, V = scores.shape
+    dev = scores.device
+    if u.dim() != 2 or u.dtype != torch.float32 or u.shape[0] != R or u.device != dev:
+        raise ValueError(f"u: float32 [{R}, draws] on {dev}, got {tuple(u.shape)} {u.dtype} on {u.device}")
+    n = u.shape[1]
+    scores, u = scores.detach(), u.detach()
+    if V > 1 and scores.stride(1) != 1:
+        scores = scores.contiguous()
+    if n > 1 and u.stride(1) != 1:
+        u = u.contiguous()
+    a = _lib.psl_draw_args(n_rows=R, n_cols=V, n_draws=n, dtype=_DRAW_DTYPES[scores.dtype], scores=scores.data_ptr(),
+                           score_stride=scores.stride(0), u=u.data_ptr(), u_stride=u.stride(0))
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev or tuple(mask.shape) not in ((R, V), (V,)):
+            raise ValueError(f"mask: bool or uint8 [{R}, {V}] or [{V}] on {dev}, got {tuple(mask.shape)} {mask.dtype} on {mask.device}")
+        mask = mask.detach()
+        mask = mask.expand(R, V)
+        if V > 1 and mask.stride(1) != 1:
+            mask = mask.contiguous()
+        a.mask, a.mask_stride = mask.data_ptr(), mask.stride(0)
+    keep = []
+    for name, x, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32)):
+        if torch.is_tensor(x):
+            if tuple(x.shape) != (R,) or x.device != dev or x.dtype != dt:
+                raise ValueError(f"{name}: a number or {dt} [{R}] on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
+            x = x.detach().contiguous()
+            keep.append(x)
+            setattr(a, name, x.data_ptr())
+        elif name == "top_k":
+            a.top_k_all = max(0, min(int(x), 0x7fffffff))
+        elif x != x:
+            raise ValueError(f"{name} is NaN")
+        else:
+            setattr(a, name + "_all", float(x))
+    if dev.type != "cuda":
+        raise _lib.PslError(f"psl_draw_indices: tensors on {dev}; the kernels run on the GPU and have no host fallback")
+    idx = torch.empty(R, n, dtype=torch.int32, device=dev)
+    prob = torch.empty(R, n, dtype=torch.float32, device=dev) if with_prob else None
+    if R and n:
+        L = _lib.lib()
+        with torch.cuda.device(dev):
+            a.ws_bytes = _lib.check(L.psl_draw_ws_bytes(R, V), "psl_draw_ws_bytes")
+            ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
+            a.idx, a.prob, a.ws = idx.data_ptr(), prob.data_ptr() if with_prob else None, ws.data_ptr()
+            _lib.check(L.psl_draw_indices(C.byref(a), _lib.stream_ptr()), "psl_draw_indices")
+    if one:
+        idx, prob = idx[0], prob[0] if with_prob else None
+    return (idx, prob) if with_prob else idx
+
+
 def keyframe_overlap(rays_o, rays_d, gt_depth, keyframe_c2w, cam: dict, n_samples=8, edge=20):
     """percent_inside per keyframe (src/Mapper.py:197-229). keyframe_c2w: list of [4,4] (or [3,4]) poses, tensors or host
     float lists.  Rays with gt_depth <= 0 are skipped by the kernel (get_samples' depth_filter, Mapper.py:190-192): the
