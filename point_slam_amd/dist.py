@@ -41,6 +41,11 @@ Merge rule for the features of points several ranks trained (`merge=`): "mean" (
 changes; "owner" = SURVEY.md 8e's owner-writes policy: the rank that CREATED the point wins if it changed the row (points of
 the seed map and rows their creator did not touch: the lowest contributing rank).  Both are deterministic and
 rank-invariant; bench.py --merge reports the render loss after the exchange under either.
+
+Feature rows on the wire (`wire=`): None sends fp32 as above; "int8", "e4m3" or "int4" sends the feature rows of new points and
+the changes of touched rows as codes with one fp32 scale to a row (row_store.write_records: int8 88 B instead of 272 B per
+point, 76 B instead of 260 B per row).  Every rank, the sender included, goes on with what the codes stand for, so replicas
+stay identical; positions, radii, row ids and the decoder stay fp32.
 """
 from __future__ import annotations
 
@@ -55,6 +60,28 @@ import torch.distributed as dist
 
 REC = 3 + 32 + 32 + 1          # new-point record: xyz, geometry feature, colour feature, add-radius
 REC_ROW = 1 + 64               # touched-row record: row id (int32 bits), change of the geometry + colour feature row
+
+
+# ------------------------------------------------------------------------------------------------------- feature rows on the wire
+class _RowWire:
+    """Pairs of feature rows [n, 2, 32] as columns of fp32 records: 64 floats, or codes and scales (row_store)."""
+
+    def __init__(self, fmt: Optional[str]):
+        from . import row_store
+        self.fmt, self._rs = fmt, row_store
+        self.codes, self.scales = (64, 0) if fmt is None else row_store.record_floats(2, 32, fmt)
+        self.floats = self.codes + self.scales
+
+    def put(self, rec: torch.Tensor, col: int, pair: torch.Tensor):
+        if self.fmt is None:
+            rec[:, col:col + 64] = pair.reshape(-1, 64)
+        else:
+            self._rs.write_records(rec, pair, self.fmt, col, col + self.codes)
+
+    def get(self, rec: torch.Tensor, col: int) -> torch.Tensor:
+        if self.fmt is None:
+            return rec[:, col:col + 64].reshape(-1, 2, 32)
+        return self._rs.read_records(rec, 2, 32, self.fmt, col, col + self.codes)
 
 
 # ------------------------------------------------------------------------------------------------------- transport
@@ -176,21 +203,28 @@ def transport_name(tr) -> str:
 
 
 # ------------------------------------------------------------------------------------------------------- new points
-def merge_new_points(npc, n_base: int, group=None, dedupe: bool = True, transport=None, creators: Optional[list] = None) -> List[int]:
+def merge_new_points(npc, n_base: int, group=None, dedupe: bool = True, transport=None, creators: Optional[list] = None,
+                     wire: Optional[str] = None) -> List[int]:
     """Exchange the points `npc` gained since it had n_base points and rebuild the replica in global rank order
     (steps 1-2 of the module docstring).  Returns the number of points every rank CONTRIBUTED; the number admitted
     after the cross-rank dedupe is npc.pts_num() - n_base.  creators: a list that receives ONE int16 tensor, the
-    contributing rank of every admitted point in append order (the owner-writes merge rule needs it)."""
+    contributing rank of every admitted point in append order (the owner-writes merge rule needs it).  wire: form of the feature
+    rows in the records (module docstring)."""
     tr = transport or _TorchTransport(group)
+    rw = _RowWire(wire)
+    c_feat, c_rad = (3, 67) if wire is None else (4, 3)           # codes start on a 16-byte boundary
     n_now = npc.pts_num()
     n_new = n_now - n_base
     dev = npc.get_geo_feats().device
-    rec = torch.empty(n_new, REC, device=dev, dtype=torch.float32)
+    rec = torch.empty(n_new, REC - 64 + rw.floats, device=dev, dtype=torch.float32)
     if n_new:
         rec[:, :3] = npc.cloud_pos_device(n_base, n_new)          # tail only
-        rec[:, 3:35] = npc.get_geo_feats()[n_base:n_now]
-        rec[:, 35:67] = npc.get_col_feats()[n_base:n_now]
-        rec[:, 67] = npc.point_radius(n_base, n_new)
+        rec[:, c_rad] = npc.point_radius(n_base, n_new)
+        if wire is None:
+            rec[:, 3:35] = npc.get_geo_feats()[n_base:n_now]
+            rec[:, 35:67] = npc.get_col_feats()[n_base:n_now]
+        else:
+            rw.put(rec, c_feat, torch.stack([npc.get_geo_feats()[n_base:n_now], npc.get_col_feats()[n_base:n_now]], 1))
     allrec, counts = tr.allgather_v(rec)
     if sum(counts) == 0:
         return counts                                             # nobody added anything: the replica stands as it is
@@ -201,7 +235,7 @@ def merge_new_points(npc, n_base: int, group=None, dedupe: bool = True, transpor
     if dedupe:
         # locations are triplets (N_add = 3, neural_point.py:126-143); the middle point is the surface point
         loc = allrec[:, :3].reshape(-1, 3, 3)[:, 1, :].contiguous()
-        rad = allrec[:, 67].reshape(-1, 3)[:, 1].contiguous()
+        rad = allrec[:, c_rad].reshape(-1, 3)[:, 1].contiguous()
         first = next(k for k, c in enumerate(counts) if c > 0)    # the first non-empty block is admitted whole
         lo = offs[first + 1] // 3
         keep_loc = torch.ones(loc.shape[0], dtype=torch.uint8, device=dev)
@@ -210,7 +244,7 @@ def merge_new_points(npc, n_base: int, group=None, dedupe: bool = True, transpor
             # >= n_base are ignored) -- no rebuild before the test
             keep_loc[lo:] = (npc.count_within(loc[lo:], rad[lo:], n_base) == 0).to(torch.uint8)
         # vs the blocks before it, in rank order (one launch per block, flags final when the next block reads them)
-        npc.dedupe_blocks(allrec, 0, 67, [o // 3 for o in offs], keep_loc)
+        npc.dedupe_blocks(allrec, 0, c_rad, [o // 3 for o in offs], keep_loc)
         keep_loc = keep_loc.bool()
         keep = keep_loc[:, None].expand(-1, 3).reshape(-1)
     kept = allrec[keep]
@@ -220,8 +254,9 @@ def merge_new_points(npc, n_base: int, group=None, dedupe: bool = True, transpor
         creators.append(blk[keep])
     npc.truncate(n_base)
     # ONE append and ONE index rebuild for all blocks (also when nothing was kept: truncate left the index stale)
-    npc.append_points(kept[:, :3].contiguous(), kept[:, 3:35].contiguous(), kept[:, 35:67].contiguous(),
-                      radius=kept[:, 67].contiguous(), build=True)
+    feats = rw.get(kept, c_feat)
+    npc.append_points(kept[:, :3].contiguous(), feats[:, 0].contiguous(), feats[:, 1].contiguous(),
+                      radius=kept[:, c_rad].contiguous(), build=True)
     return counts
 
 
@@ -231,11 +266,13 @@ class FrameParallelSync:
     (`note_rows`) and of the colour-decoder blob."""
 
     def __init__(self, npc, theta: Optional[torch.Tensor] = None, n_color: int = 0, group=None,
-                 transport: Optional[str] = None, merge: str = "mean"):
+                 transport: Optional[str] = None, merge: str = "mean", wire: Optional[str] = None):
         if merge not in ("mean", "owner"):
             raise ValueError("merge must be 'mean' or 'owner'")
         self.group = group
         self.merge = merge
+        self.wire = wire
+        self._rw = _RowWire(wire)
         self._owner = None          # int16 [capacity]: rank that created a point, -1 = the seed map (owner-writes rule)
         self.n_color = n_color
         self.transport = make_transport(npc, group, transport)
@@ -281,10 +318,13 @@ class FrameParallelSync:
         else:
             rows_c = torch.zeros(0, dtype=torch.int64, device=dev)
             delta_c = snap_c = torch.zeros(0, 64, device=dev)
-        rec = torch.empty(rows_c.shape[0], REC_ROW, device=dev, dtype=torch.float32)
+        rw = self._rw
+        rec = torch.empty(rows_c.shape[0], REC_ROW - 64 + rw.floats, device=dev, dtype=torch.float32)
         rec[:, 0] = rows_c.to(torch.int32).view(torch.float32)      # the id travels as raw bits (collectives only copy)
-        rec[:, 1:] = delta_c
+        rw.put(rec, 1, delta_c.reshape(-1, 2, 32))
         allrec, counts = self.transport.allgather_v(rec)
+        if self.wire is not None:                                   # from here on the changes are what the codes stand for
+            allrec = torch.cat([allrec[:, :1], rw.get(allrec, 1).reshape(-1, 64)], 1)
         self.last_stats = dict(rows_noted=int(self._n_slots), rows_sent=int(rows_c.shape[0]), rows_received=int(sum(counts)))
         if sum(counts):
             ids = allrec[:, 0].contiguous().view(torch.int32).long()
@@ -346,7 +386,8 @@ class FrameParallelSync:
         t2 = time.perf_counter()
         # 1-2. new points
         creators: list = []
-        counts = merge_new_points(npc, self.n_base, self.group, dedupe, self.transport, creators if self.merge == "owner" else None)
+        counts = merge_new_points(npc, self.n_base, self.group, dedupe, self.transport, creators if self.merge == "owner" else None,
+                                  wire=self.wire)
         t3 = time.perf_counter()
         self.last_host_ms = dict(rows=round((t1 - t0) * 1e3, 3), decoder=round((t2 - t1) * 1e3, 3), new_points=round((t3 - t2) * 1e3, 3))
         if self.merge == "owner" and creators and creators[0].numel():     # the creator table only serves the owner-writes rule

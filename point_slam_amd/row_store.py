@@ -49,6 +49,43 @@ def _call(entry, values, rows, first, n, fmt, group, capacity, codes, codes_row_
         _lib.check(getattr(_lib.lib(), entry)(C.byref(a), _lib.stream_ptr()), entry)
 
 
+def record_floats(heads: int, dim: int, fmt: str, group: Optional[int] = None) -> tuple:
+    """(floats that the codes of a row fill, floats that its scales fill) inside a record of 32-bit words."""
+    group = dim if group is None else group
+    _check_layout(heads, dim, fmt, group)
+    bits = heads * dim * BITS[fmt]
+    if bits % 32:
+        raise ValueError(f"{heads} x {dim} codes of {BITS[fmt]} bits do not fill whole 32-bit words")
+    return bits // 32, heads * (dim // group)
+
+
+def write_records(rec: torch.Tensor, values: torch.Tensor, fmt: str, code_col: int, scale_col: int, group: Optional[int] = None):
+    """Quantise values [n, heads, dim] into columns of fp32 records [n, W]: codes from column code_col (as raw 32-bit words),
+    scales from column scale_col.  What the multi-GPU exchange sends; the other columns stay as they are."""
+    _record_call("psl_rows_write", rec, values.detach().contiguous(), fmt, code_col, scale_col, group)
+    return rec
+
+
+def read_records(rec: torch.Tensor, heads: int, dim: int, fmt: str, code_col: int, scale_col: int, group: Optional[int] = None) -> torch.Tensor:
+    """The values [n, heads, dim] fp32 that write_records put into `rec`."""
+    out = torch.empty(rec.shape[0], heads, dim, dtype=torch.float32, device=rec.device)
+    _record_call("psl_rows_read", rec, out, fmt, code_col, scale_col, group)
+    return out
+
+
+def _record_call(entry, rec, values, fmt, code_col, scale_col, group):
+    n, heads, dim = values.shape
+    group = dim if group is None else group
+    cw, sw = record_floats(heads, dim, fmt, group)
+    if rec.dtype != torch.float32 or rec.dim() != 2 or rec.shape[0] != n or not rec.is_contiguous() or values.dtype not in _DTYPES:
+        raise ValueError(f"records: contiguous float32 [{n}, width], got {tuple(rec.shape)} {rec.dtype}")
+    spans = sorted([(code_col, code_col + cw), (scale_col, scale_col + sw)])
+    if spans[0][0] < 0 or spans[0][1] > spans[1][0] or spans[1][1] > rec.shape[1] or rec.device != values.device:
+        raise ValueError(f"codes at {code_col} (+{cw}) and scales at {scale_col} (+{sw}) in records of {rec.shape[1]}")
+    if n:
+        _call(entry, values, None, 0, n, fmt, group, n, rec[:, code_col:], 4 * rec.shape[1], rec[:, scale_col:], rec.shape[1])
+
+
 class QuantizedRows:
     """A store of `capacity` rows.  codes: uint8 [capacity, heads, dim * bits / 8], scales: fp32 [capacity, heads, dim / group];
     rows that were never written read as zeros."""
@@ -130,3 +167,17 @@ class QuantizedRows:
         elif n:
             out.zero_()
         return out
+
+    def state_dict(self) -> dict:
+        """Codes and scales with their layout: what a checkpoint keeps."""
+        return {"capacity": self.capacity, "heads": self.heads, "dim": self.dim, "format": self.fmt, "group": self.group,
+                "codes": self.codes, "scales": self.scales}
+
+    @classmethod
+    def from_state(cls, state: dict, device="cuda:0") -> "QuantizedRows":
+        st = cls(state["capacity"], state["heads"], state["dim"], state["format"], state["group"], device)
+        if tuple(state["codes"].shape) != tuple(st.codes.shape) or tuple(state["scales"].shape) != tuple(st.scales.shape):
+            raise ValueError("codes and scales do not have the layout the state names")
+        st.codes.copy_(state["codes"])
+        st.scales.copy_(state["scales"])
+        return st

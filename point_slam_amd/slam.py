@@ -42,6 +42,7 @@ class Frame:
         self.c2w = c2w            # [4,4] estimated pose (device tensor)
         self.exposure = exposure  # [8] exposure latent of a keyframe (model.encode_exposure)
         self.grad_mag = None      # [H,W] f64 colour-gradient magnitude, filled on demand
+        self.grad_scores = None   # (floor, [H*W] f32 log(magnitude + floor)), filled on demand
 
     def c2w_host(self) -> list:
         """The pose as 12 host floats (row-major 3x4): ONE device-to-host copy per pose, shared by everything a mapped frame
@@ -90,6 +91,8 @@ class HipSLAM:
                                       "native engine, or HipRenderer inside the reference's own Tracker/Mapper")
         cfgd = dict(cfg)
         cfgd["mapping"] = dict(cfg["mapping"], device=str(device))
+        if engine != "native" and (cfg["tracking"].get("score_sampling") or cfg["mapping"].get("score_sampling")):
+            raise NotImplementedError("score_sampling draws full-image pixels for the native engine")
         self.npc = HipNeuralPointCloud(cfgd, max_points=max_points, device=str(device))
         import types
         self.renderer = HipRenderer(cfg, None, types.SimpleNamespace(**cam))
@@ -222,6 +225,30 @@ class HipSLAM:
         pick = torch.rand(n_iters, sel.numel(), device=self.device).topk(n_pix, dim=1).indices
         return sel[pick].to(torch.int32).contiguous()
 
+    def score_draws(self, frames: List[Frame], n_draws: int, cut: dict, edge_h=0, edge_w=0) -> torch.Tensor:
+        """Pixels drawn by how much happens in them: n_draws flat full-image indices of each frame, int32 [frames, n_draws],
+        with weights (colour-gradient magnitude + floor) ** (1 / temperature) over the pixels with sensor depth inside the
+        border, the tail cut by top_k / top_p / min_p (frame_ops.draw_indices; `cut` = tracking.score_sampling or
+        mapping.score_sampling, e.g. {"temperature": 0.7, "top_p": 0.9}).  A soft form of sample_with_color_grad, which takes
+        pixels of the hard top-k alike.  floor (default 1e-3) is what a flat pixel weighs."""
+        from . import frame_ops
+        par = dict(cut)
+        floor = float(par.pop("floor", 1e-3))
+        scores, mask = [], []
+        for f in frames:
+            if f.grad_scores is None or f.grad_scores[0] != floor:
+                f.grad_scores = (floor, torch.log(self.grad_mag(f) + floor).float().reshape(-1))
+            scores.append(f.grad_scores[1])
+            m = f.depth > 0
+            if edge_h or edge_w:
+                inside = torch.zeros_like(m)
+                inside[edge_h:m.shape[0] - edge_h, edge_w:m.shape[1] - edge_w] = True
+                m = m & inside
+            mask.append(m.reshape(-1))
+        u = torch.rand(len(frames), n_draws, device=self.device)
+        idx = frame_ops.draw_indices(torch.stack(scores), u, mask=torch.stack(mask), **par)
+        return idx.clamp_(min=0)          # a frame without any sensor depth: pixel 0, whose missing depth every loop filters
+
     def _exposure_block(self, feats, lr_mlp, lr_feat=0.001):
         """psl_exposure_args over the shared MLP blob and `feats` ([8] or [F,8]); returns (struct, keep-alive)."""
         adam = torch.zeros(2, _lib.EXPOSURE_MLP_FLOATS + _lib.EXPOSURE_DIM, device=self.device)
@@ -233,9 +260,13 @@ class HipSLAM:
         L = _lib.lib()
         tr, cam = self.cfg["tracking"], self.cam
         eh, ew = tr["ignore_edge_H"], tr["ignore_edge_W"]
-        full = bool(tr.get("sample_with_color_grad", False))
+        by_score = tr.get("score_sampling")
+        full = bool(tr.get("sample_with_color_grad", False) or by_score)
         if draws is not None:
             idx, fb = draws
+        elif by_score:
+            idx = self.score_draws([frame], n_iters * n_pix, by_score, eh, ew).reshape(n_iters, n_pix)
+            fb = torch.zeros(n_iters, 2, 32, device=self.device).normal_(mean=0, std=0.01)
         elif full:
             idx = self.color_grad_draws(frame, n_iters, n_pix)
             fb = torch.zeros(n_iters, 2, 32, device=self.device).normal_(mean=0, std=0.01)
@@ -470,7 +501,14 @@ class HipSLAM:
         mp, cam, dev = self.cfg["mapping"], self.cam, self.device
         W = len(window)
         n = W * ppf
-        idx, fb = draws if draws is not None else self._draws(n_iters, n, cam["H"] * cam["W"])
+        if draws is not None:
+            idx, fb = draws
+        elif mp.get("score_sampling"):
+            idx = self.score_draws(window, n_iters * ppf, mp["score_sampling"]).reshape(W, n_iters, ppf)
+            idx = idx.transpose(0, 1).reshape(n_iters, n).contiguous()
+            fb = torch.zeros(n_iters, 2, 32, device=dev).normal_(mean=0, std=0.01)
+        else:
+            idx, fb = self._draws(n_iters, n, cam["H"] * cam["W"])
         need = int(L.psl_map_ws_floats(n, W))
         if self._ws_map is None or self._ws_map.numel() < need:
             self._ws_map = torch.empty(need, device=dev)
