@@ -22,7 +22,12 @@ struct DrawArgs {
   const float* u; long long u_stride;
   int* idx; float* prob;
   // workspace
+  int cuts;                    // whether any row may have a limit (else the launches that find thresholds are left out)
+  int n_parts, part_len;       // pieces of a row in the launches before k_draw_sums
   struct DrawState* state;     // [n_rows]
+  unsigned* part_max; unsigned* part_min;       // [n_rows][n_parts] keys
+  unsigned* bin_cnt; unsigned long long* bin_mass;       // [n_rows][kBins]
+  unsigned long long* list_a; unsigned long long* list_b; int list_cap;      // [n_rows][list_cap] numbers of candidate entries
   double* chunk_sum;           // [n_rows][n_chunks]
   double* block_incl;          // [n_rows][n_chunks * chunk / 16]: running sums inside a chunk, at the end of each 16 entries
   int n_chunks, chunk;         // entries of a chunk (a multiple of kTile)
@@ -30,11 +35,15 @@ struct DrawArgs {
 struct DrawState {
   u64 thr;                     // kept: number(entry) >= thr
   float M; int any;            // largest allowed score; whether there is one
+  unsigned n_a, n_b;           // fill of the two lists
 };
 
 constexpr int kBlock = 16;     // entries to a stored running sum: one 64-byte line of fp32 scores
 constexpr int kTile = 4096;    // entries that a workgroup of k_draw_sums takes per step
 constexpr int kMaxChunks = 1024;
+constexpr int kMaxParts = 256;
+constexpr int kBins = 1024;
+constexpr double kRange = 48.0;
 
 // ---- an entry's order: excluded entries (masked, NaN, -inf) are 0, everything else grows with the score; -0 == +0
 __device__ __forceinline__ unsigned key_of(float s) {
@@ -84,15 +93,280 @@ __device__ __forceinline__ double weight_of(float s, float M, double inv_t) {
 
 __device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up(v, o); }
 
-// ---------------------------------------------------------------- the threshold of a row, by radix selection
-// 256 bins of (count, mass): masses are summed as integers, 32 bits before and 32 behind the point at 2^-32, so their sum has no order
+// ---------------------------------------------------------------- largest and smallest allowed score of a row's parts
+// A row is read in n_parts pieces of part_len entries, a workgroup to a piece; four entries to a lane and step.
+template <int DT> struct Four { float s[4]; unsigned live; };      // live: bit q = entry q is inside the row and not masked
+template <int DT> __device__ __forceinline__ Four<DT> load_four(const RowView& v, int i, int end) {
+  Four<DT> f;
+  f.live = 0;
+  if (i + 4 <= end) {
+    // rows begin anywhere: the loads are as wide as 16 bytes but aligned to an entry only
+    if constexpr (DT == PSL_F32) __builtin_memcpy(f.s, (const float*)v.s + i, 16);
+    else {
+      unsigned short h[4];
+      __builtin_memcpy(h, (const unsigned short*)v.s + i, 8);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if constexpr (DT == PSL_BF16) f.s[q] = __uint_as_float((unsigned)h[q] << 16);
+        else { _Float16 x; __builtin_memcpy(&x, &h[q], 2); f.s[q] = (float)x; }
+      }
+    }
+    f.live = 15u;
+    if (v.m) {
+      unsigned m;
+      __builtin_memcpy(&m, v.m + i, 4);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) if (!((m >> (8 * q)) & 255u)) f.live &= ~(1u << q);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f.s[q] = 0.f;
+      if (i + q < end) { f.s[q] = load_score<DT>(v.s, i + q); if (!v.m || v.m[i + q]) f.live |= 1u << q; }
+    }
+  }
+  return f;
+}
+template <int DT> __device__ __forceinline__ unsigned four_key(const Four<DT>& f, int q) { return (f.live >> q) & 1u ? key_of(f.s[q]) : 0u; }
+
+template <int DT> __global__ __launch_bounds__(256) void k_draw_range(DrawArgs a) {
+  __shared__ unsigned s_mx[4], s_mn[4];
+  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const RowView v = row_view<DT>(a, r);
+  const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
+  unsigned mx = 0u, mn = 0xffffffffu;
+  for (int i = i0 + tid * 4; i < i1; i += 1024) {
+    const Four<DT> f = load_four<DT>(v, i, i1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { const unsigned k = four_key(f, q); mx = max(mx, k); mn = min(mn, k ? k : 0xffffffffu); }
+  }
+  for (int o = 32; o > 0; o >>= 1) { mx = max(mx, (unsigned)__shfl_xor((int)mx, o)); mn = min(mn, (unsigned)__shfl_xor((int)mn, o)); }
+  if (lane == 0) { s_mx[tid >> 6] = mx; s_mn[tid >> 6] = mn; }
+  __syncthreads();
+  if (tid == 0) {
+    a.part_max[(long long)r * a.n_parts + blockIdx.x] = max(max(s_mx[0], s_mx[1]), max(s_mx[2], s_mx[3]));
+    a.part_min[(long long)r * a.n_parts + blockIdx.x] = min(min(s_mn[0], s_mn[1]), min(s_mn[2], s_mn[3]));
+  }
+  // what the next launches add to
+  if (a.cuts && blockIdx.x == 0) {
+    for (int j = tid; j < kBins; j += 256) { a.bin_cnt[(long long)r * kBins + j] = 0u; a.bin_mass[(long long)r * kBins + j] = 0ull; }
+    if (tid == 0) { a.state[r].n_a = 0u; a.state[r].n_b = 0u; }
+  }
+}
+// the same of the whole row, to every thread of a workgroup (n_parts <= kMaxParts)
+struct Range { unsigned mx, mn; };
+__device__ __forceinline__ Range row_range(const DrawArgs& a, int r) {
+  __shared__ unsigned s_mx, s_mn;
+  if (threadIdx.x < 64) {
+    unsigned mx = 0u, mn = 0xffffffffu;
+    for (int j = threadIdx.x; j < a.n_parts; j += 64) { mx = max(mx, a.part_max[(long long)r * a.n_parts + j]); mn = min(mn, a.part_min[(long long)r * a.n_parts + j]); }
+    for (int o = 32; o > 0; o >>= 1) { mx = max(mx, (unsigned)__shfl_xor((int)mx, o)); mn = min(mn, (unsigned)__shfl_xor((int)mn, o)); }
+    if (threadIdx.x == 0) { s_mx = mx; s_mn = mn; }
+  }
+  __syncthreads();
+  return Range{s_mx, s_mn};
+}
+__device__ __forceinline__ bool has_cut(const RowPar& p) { return p.k > 0 || p.p < 1.0; }
+
+// ---------------------------------------------------------------- bins of equal width in (M - s) / T
+// kBins of them over the row's range, at most kRange wide (what lies further weighs less than 2e-21 of the largest and is
+// in the last bin).  Rounding is monotone, so a bin is an interval of scores.  A bin's mass is a sum of integers, weights
+// scaled by 2^(q + the bin's own exponent): it has no order, and its rounding is 2^-q of the bin's own weights.
+struct Binning { double M, inv_t, c, oct; int q; };
+__device__ __forceinline__ Binning make_binning(const Range& g, double inv_t, int n_cols) {
+  Binning b;
+  b.M = (double)score_of(g.mx); b.inv_t = inv_t;
+  double range = (b.M - (double)score_of(g.mn)) * inv_t;
+  if (!(range < kRange)) range = kRange;
+  b.c = range > 0.0 ? (double)kBins / range : 0.0;
+  if (!(b.c < 1e300)) b.c = 1e300;
+  b.oct = range > 0.0 ? range / (double)kBins * 1.4426950408889634 : 0.0;        // binary orders per bin
+  b.q = 62 - (32 - __clz(n_cols));
+  return b;
+}
+__device__ __forceinline__ int bin_of(const Binning& b, float s) {
+  const double x = (b.M - (double)s) * b.inv_t * b.c;
+  return (double)s == b.M ? 0 : x < (double)(kBins - 1) ? (int)x : kBins - 1;
+}
+__device__ __forceinline__ int bin_shift(const Binning& b, int bin) { return b.q + (int)((double)bin * b.oct); }
+
+template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
+  __shared__ unsigned cnt[kBins];
+  __shared__ u64 mass[kBins];
+  const int r = blockIdx.y, tid = threadIdx.x;
+  const RowPar par = row_par(a, r);
+  if (!has_cut(par)) return;
+  for (int j = tid; j < kBins; j += 512) { cnt[j] = 0u; mass[j] = 0ull; }
+  const Range g = row_range(a, r);        // (its barrier also covers the bins)
+  if (!g.mx) return;
+  const Binning b = make_binning(g, par.inv_t, a.n_cols);
+  const float M = score_of(g.mx);
+  const RowView v = row_view<DT>(a, r);
+  const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
+  const bool weigh = par.p < 1.0;
+  for (int i = i0 + tid * 4; i < i1; i += 2048) {
+    const Four<DT> f = load_four<DT>(v, i, i1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned k = four_key(f, q);
+      if (k) {
+        const float s = score_of(k);
+        const int bin = bin_of(b, s);
+        atomicAdd(&cnt[bin], 1u);
+        if (weigh) atomicAdd(&mass[bin], (u64)(ldexp(weight_of(s, M, par.inv_t), bin_shift(b, bin)) + 0.5));
+      }
+    }
+  }
+  __syncthreads();
+  for (int j = tid; j < kBins; j += 512) {
+    if (cnt[j]) {
+      atomicAdd(&a.bin_cnt[(long long)r * kBins + j], cnt[j]);
+      if (weigh) atomicAdd(&a.bin_mass[(long long)r * kBins + j], mass[j]);
+    }
+  }
+}
+
+// Which bins the two limits fall into.  Wavefront 0; lane l holds bins 16 l .. 16 l + 15, the largest scores first.
+struct Cut {
+  unsigned n_valid, want;          // want: entries of k_bin that top-k keeps
+  int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
+  double above_k, total;           // mass of the bins before k_bin; of all
+  unsigned n_a, n_b;               // entries of k_bin; of [p_lo, p_hi]
+};
+struct LaneBins { unsigned c[16]; double m[16]; unsigned c_before; double m_before; };
+__device__ __forceinline__ LaneBins load_bins(const DrawArgs& a, int r, const Binning& b) {
+  LaneBins w;
+  const int lane = threadIdx.x & 63;
+  unsigned cs = 0; double ms = 0.0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int bin = 16 * lane + j;
+    w.c[j] = a.bin_cnt[(long long)r * kBins + bin];
+    w.m[j] = ldexp((double)a.bin_mass[(long long)r * kBins + bin], -bin_shift(b, bin));
+    cs += w.c[j]; ms += w.m[j];
+  }
+  unsigned ci = cs; double mi = ms;
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned cu = __shfl_up(ci, o); const double mu = shfl_up_d(mi, o);
+    if (lane >= o) { ci += cu; mi += mu; }
+  }
+  w.c_before = ci - cs;
+  w.m_before = __shfl_up(mi, 1);
+  if (lane == 0) w.m_before = 0.0;
+  return w;
+}
+struct Found { int bin; unsigned before_n, count; double before, mass; };
+// first bin where the running count (mass) reaches `want`; entries of bins behind `last` do not count and `last` itself
+// weighs last_mass.  No such bin (rounding): the last one that holds something.
+__device__ __forceinline__ Found find_bin(const LaneBins& w, bool by_mass, unsigned want_n, double want_m, int last, double last_mass) {
+  const int lane = threadIdx.x & 63;
+  unsigned cb = w.c_before; double mb = w.m_before;
+  Found hit{-1, 0u, 0u, 0.0, 0.0}, tail{-1, 0u, 0u, 0.0, 0.0};
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const int bin = 16 * lane + j;
+    const double m = bin == last ? last_mass : w.m[j];
+    if (w.c[j] && bin <= last) {
+      const Found here{bin, cb, w.c[j], mb, m};
+      tail = here;
+      if (hit.bin < 0 && (by_mass ? mb + m >= want_m : cb + w.c[j] >= want_n)) hit = here;
+    }
+    cb += w.c[j]; mb += m;
+  }
+  const u64 hits = __ballot(hit.bin >= 0), some = __ballot(tail.bin >= 0);
+  const int src = hits ? __ffsll((long long)hits) - 1 : some ? 63 - __clzll((long long)some) : 0;
+  const Found send = hits ? hit : tail;
+  Found f;
+  f.bin = __shfl(send.bin, src); f.before_n = __shfl(send.before_n, src); f.count = __shfl(send.count, src);
+  f.before = __shfl(send.before, src); f.mass = __shfl(send.mass, src);
+  return f;
+}
+__device__ __forceinline__ Cut make_cut(const LaneBins& w, const RowPar& par) {
+  Cut c;
+  unsigned cs = 0; double ms = 0.0;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) { cs += w.c[j]; ms += w.m[j]; }
+  c.n_valid = __shfl(w.c_before + cs, 63);
+  c.total = __shfl(w.m_before + ms, 63);
+  c.k_bin = kBins; c.want = 0u; c.above_k = c.total; c.n_a = 0u; c.n_b = 0u; c.p_lo = 0; c.p_hi = -1;
+  double most = c.total;
+  if (par.k > 0 && (unsigned)par.k < c.n_valid) {
+    const Found f = find_bin(w, false, (unsigned)par.k, 0.0, kBins - 1, __shfl(w.m[15], 63));
+    c.k_bin = f.bin; c.want = (unsigned)par.k - f.before_n; c.above_k = f.before; c.n_a = f.count;
+    most = f.before + f.mass;
+  }
+  if (par.p < 1.0 && par.k != 1) {
+    // top-k leaves a mass between above_k and `most`: the bins where its share can fall
+    const double last = __shfl(w.m[15], 63);
+    c.p_lo = find_bin(w, true, 0u, par.p * c.above_k, kBins - 1, last).bin;
+    c.p_hi = find_bin(w, true, 0u, par.p * most, kBins - 1, last).bin;
+    if (c.p_hi >= c.k_bin) c.p_hi = c.k_bin - 1;
+    unsigned n = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) { const int bin = 16 * (threadIdx.x & 63) + j; if (bin >= c.p_lo && bin <= c.p_hi) n += w.c[j]; }
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    c.n_b = n;
+  }
+  return c;
+}
+
+// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.
+template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs a) {
+  __shared__ Cut s_cut;
+  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const RowPar par = row_par(a, r);
+  if (!has_cut(par)) return;
+  const Range g = row_range(a, r);
+  if (!g.mx) return;
+  const Binning b = make_binning(g, par.inv_t, a.n_cols);
+  if (tid < 64) { const Cut c = make_cut(load_bins(a, r, b), par); if (tid == 0) s_cut = c; }
+  __syncthreads();
+  const Cut c = s_cut;
+  const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.n_b && c.n_b <= (unsigned)a.list_cap;
+  if (!do_a && !do_b) return;
+  const RowView v = row_view<DT>(a, r);
+  const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
+  u64* la = a.list_a + (long long)r * a.list_cap;
+  u64* lb = a.list_b + (long long)r * a.list_cap;
+  for (int base = i0; base < i1; base += 2048) {
+    const int i = base + tid * 4;
+    const Four<DT> f = load_four<DT>(v, i, i1);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned k = four_key(f, q);
+      const int bin = k ? bin_of(b, score_of(k)) : -1;
+      const bool in_a = do_a && bin == c.k_bin, in_b = do_b && bin >= c.p_lo && bin <= c.p_hi;
+      const u64 ba = __ballot(in_a), bb = __ballot(in_b);
+      const u64 below = (1ull << lane) - 1ull;
+      if (ba) {
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&a.state[r].n_a, (unsigned)__popcll(ba));
+        at = __shfl(at, 0);
+        if (in_a) la[at + (unsigned)__popcll(ba & below)] = number_of(k, i + q);
+      }
+      if (bb) {
+        unsigned at = 0;
+        if (lane == 0) at = atomicAdd(&a.state[r].n_b, (unsigned)__popcll(bb));
+        at = __shfl(at, 0);
+        if (in_b) lb[at + (unsigned)__popcll(bb & below)] = number_of(k, i + q);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the threshold among those entries, by radix selection
+// 256 digits of (count, mass): masses are summed as integers, 32 bits before and 32 behind the point at 2^-32, so their sum has no order
 struct RadixBins { unsigned cnt[256]; u64 hi[256], lo[256]; };
 struct RadixPick { int bin; unsigned above, count; double mass_above, mass; };
+struct RadixShared { RadixBins bins; RadixPick pick; u64 mx[16], mn[16]; u64 hi, lo; };
 
-__device__ __forceinline__ void radix_zero(RadixBins& b) {
-  for (int j = threadIdx.x; j < 256; j += blockDim.x) { b.cnt[j] = 0; b.hi[j] = 0; b.lo[j] = 0; }
-}
 __device__ __forceinline__ double fixed_d(u64 hi, u64 lo) { return (double)hi * 0x1p-32 + (double)lo * 0x1p-64; }
+__device__ __forceinline__ void fixed_add(u64* hi, u64* lo, double w) {
+  const double x = w * 0x1p32;
+  const u64 h = (u64)x;
+  atomicAdd(hi, h);
+  atomicAdd(lo, (u64)((x - (double)h) * 0x1p32));
+}
 
 // wavefront 0, all lanes: the first bin from the top where the running count (by_mass: mass) reaches `want`
 __device__ __forceinline__ RadixPick radix_pick(const RadixBins& b, bool by_mass, unsigned want_n, double want_m) {
@@ -131,101 +405,149 @@ __device__ __forceinline__ RadixPick radix_pick(const RadixBins& b, bool by_mass
   return r;
 }
 
-// One workgroup to a row.  Digits of eight bits of the entry's 64-bit number, from the top; a level counts the entries
-// whose higher digits are the ones found so far.  Stops as soon as the bin found is taken whole.
-template <int DT> __global__ __launch_bounds__(1024) void k_draw_select(DrawArgs a) {
-  __shared__ RadixBins bins;
-  __shared__ unsigned s_max[16], s_cnt[16];
-  __shared__ RadixPick s_pick;
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const RowView v = row_view<DT>(a, r);
-  const RowPar par = row_par(a, r);
-  unsigned top = 0, cnt = 0;
-  for (int i = tid; i < a.n_cols; i += 1024) {
-    const unsigned k = entry_key<DT>(v, i);
-    top = k > top ? k : top; cnt += k ? 1u : 0u;
+// Digits of eight bits of the numbers that src(i) gives for i < n (0: not among them), from the highest in which they differ;
+// a level counts the numbers whose higher digits are the ones found so far.  Ends as soon as the digit found is taken whole.
+// By count: the smallest of the first `want`.  By mass: the smallest of the shortest prefix that weighs want_mass.
+template <class Src> __device__ u64 radix_select(const Src& src, int n, bool by_mass, unsigned want, double want_mass, float M, double inv_t,
+                                                 RadixShared& sh) {
+  const int tid = threadIdx.x;
+  u64 mx = 0ull, mn = ~0ull;
+  for (int i = tid; i < n; i += 1024) { const u64 x = src(i); if (x) { mx = x > mx ? x : mx; mn = x < mn ? x : mn; } }
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 x = __shfl_xor(mx, o), y = __shfl_xor(mn, o);
+    mx = x > mx ? x : mx; mn = y < mn ? y : mn;
   }
-  for (int o = 32; o > 0; o >>= 1) { const unsigned t = __shfl_xor(top, o); top = t > top ? t : top; cnt += __shfl_xor(cnt, o); }
-  if (lane == 0) { s_max[tid >> 6] = top; s_cnt[tid >> 6] = cnt; }
   __syncthreads();
-  top = 0; cnt = 0;
-  for (int j = 0; j < 16; ++j) { top = s_max[j] > top ? s_max[j] : top; cnt += s_cnt[j]; }
-  const float M = score_of(top);
-  u64 thr = 1ull << 32;                             // every allowed entry
-  if (top && par.k > 0 && (unsigned)par.k < cnt) {
-    unsigned want = (unsigned)par.k;
-    u64 prefix = 0;
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      __syncthreads(); radix_zero(bins); __syncthreads();
-      for (int i = tid; i < a.n_cols; i += 1024) {
-        const unsigned k = entry_key<DT>(v, i);
-        const u64 num = number_of(k, i);
-        if (k && (shift == 56 || (num >> (shift + 8)) == prefix)) atomicAdd(&bins.cnt[(num >> shift) & 255], 1u);
+  if ((tid & 63) == 0) { sh.mx[tid >> 6] = mx; sh.mn[tid >> 6] = mn; }
+  __syncthreads();
+  for (int j = 0; j < 16; ++j) { mx = sh.mx[j] > mx ? sh.mx[j] : mx; mn = sh.mn[j] < mn ? sh.mn[j] : mn; }
+  if (mx <= mn) return mx == mn ? mx : 0ull;
+  int shift = (63 - __clzll((long long)(mx ^ mn))) & ~7;
+  u64 prefix = shift == 56 ? 0ull : mx >> (shift + 8), thr = mn;
+  bool mass_level = by_mass;
+  for (; shift >= 0; shift -= 8) {
+    if (mass_level && shift < 32) {
+      // one score is left: as many of its entries as the mass still wants, at least one (all of them: the bin just found)
+      const double k = ceil(want_mass / weight_of(score_of((unsigned)(mx >> 32)), M, inv_t));
+      want = k < 1.0 ? 1u : k < 4294967295.0 ? (unsigned)k : 0xffffffffu;
+      mass_level = false;
+    }
+    __syncthreads();
+    for (int j = tid; j < 256; j += 1024) { sh.bins.cnt[j] = 0u; sh.bins.hi[j] = 0ull; sh.bins.lo[j] = 0ull; }
+    __syncthreads();
+    for (int i = tid; i < n; i += 1024) {
+      const u64 x = src(i);
+      if (x && (shift == 56 || (x >> (shift + 8)) == prefix)) {
+        const int d = (int)((x >> shift) & 255);
+        atomicAdd(&sh.bins.cnt[d], 1u);
+        if (mass_level) fixed_add(&sh.bins.hi[d], &sh.bins.lo[d], weight_of(score_of((unsigned)(x >> 32)), M, inv_t));
       }
-      __syncthreads();
-      if (tid < 64) { const RadixPick p = radix_pick(bins, false, want, 0.0); if (tid == 0) s_pick = p; }
-      __syncthreads();
-      const RadixPick p = s_pick;
-      prefix = (prefix << 8) | (unsigned)p.bin;
+    }
+    __syncthreads();
+    if (tid < 64) { const RadixPick p = radix_pick(sh.bins, mass_level, want, want_mass); if (tid == 0) sh.pick = p; }
+    __syncthreads();
+    const RadixPick p = sh.pick;
+    prefix = (prefix << 8) | (unsigned)p.bin;
+    thr = prefix << shift;               // (exact once every digit is found)
+    if (mass_level) {
+      want_mass -= p.mass_above;
+      if (p.count == 1) break;
+      if (shift == 32) mx = prefix << 32;        // the score that is left
+    } else {
       want -= p.above;
-      thr = prefix << shift;
-      if (want == p.count) break;
+      if (want >= p.count) break;
     }
   }
-  const u64 thr_k = thr;
-  if (top && par.p < 1.0 && par.k != 1) {
-    double above = 0.0, want = 0.0;
-    u64 prefix = 0;
-    unsigned ties = 0;                              // > 0: inside entries of one score, counted instead of weighed
-    for (int shift = 56; shift >= 0; shift -= 8) {
-      __syncthreads(); radix_zero(bins); __syncthreads();
-      for (int i = tid; i < a.n_cols; i += 1024) {
-        const unsigned k = entry_key<DT>(v, i);
-        const u64 num = number_of(k, i);
-        if (k && num >= thr_k && (shift == 56 || (num >> (shift + 8)) == prefix)) {
-          const int bin = (int)((num >> shift) & 255);
-          atomicAdd(&bins.cnt[bin], 1u);
-          if (shift >= 32) {
-            const double w = weight_of(score_of(k), M, par.inv_t) * 0x1p32;
-            const u64 hi = (u64)w;
-            atomicAdd(&bins.hi[bin], hi);
-            atomicAdd(&bins.lo[bin], (u64)((w - (double)hi) * 0x1p32));
-          }
-        }
+  if (shift <= 0) return thr;
+  // The digit is taken whole.  Its smallest number, not its lower end: below that end of src's scores others may begin.
+  mn = ~0ull;
+  for (int i = tid; i < n; i += 1024) { const u64 x = src(i); if (x && (x >> shift) == prefix) mn = x < mn ? x : mn; }
+  for (int o = 32; o > 0; o >>= 1) { const u64 y = __shfl_xor(mn, o); mn = y < mn ? y : mn; }
+  __syncthreads();
+  if ((tid & 63) == 0) sh.mn[tid >> 6] = mn;
+  __syncthreads();
+  for (int j = 0; j < 16; ++j) mn = sh.mn[j] < mn ? sh.mn[j] : mn;
+  return mn;
+}
+
+template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
+  __shared__ RadixShared sh;
+  __shared__ Cut s_cut;
+  __shared__ Found s_found;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  const RowPar par = row_par(a, r);
+  const Range g = row_range(a, r);
+  const float M = score_of(g.mx);
+  u64 thr = 1ull << 32;                             // every allowed entry
+  if (g.mx && has_cut(par)) {
+    const Binning b = make_binning(g, par.inv_t, a.n_cols);
+    const RowView v = row_view<DT>(a, r);
+    const u64* la = a.list_a + (long long)r * a.list_cap;
+    const u64* lb = a.list_b + (long long)r * a.list_cap;
+    LaneBins w;
+    if (tid < 64) { w = load_bins(a, r, b); const Cut c = make_cut(w, par); if (tid == 0) s_cut = c; }
+    __syncthreads();
+    const Cut c = s_cut;
+    const bool listed_a = c.n_a <= (unsigned)a.list_cap, listed_b = c.n_b <= (unsigned)a.list_cap;
+    // a list that was too long to be written: the row itself, entry by entry
+    auto from_row = [&](int i, int lo, int hi) -> u64 {
+      const unsigned k = entry_key<DT>(v, i);
+      const int bin = k ? bin_of(b, score_of(k)) : -1;
+      return bin >= lo && bin <= hi && k ? number_of(k, i) : 0ull;
+    };
+    auto src_a = [&](int i) -> u64 { return listed_a ? la[i] : from_row(i, c.k_bin, c.k_bin); };
+    const int len_a = listed_a ? (int)c.n_a : a.n_cols;
+    u64 thr_k = thr;
+    double kept = 0.0;                              // mass of what top-k keeps of its bin
+    const bool cut_k = c.k_bin < kBins, cut_p = par.p < 1.0 && par.k != 1;
+    if (cut_k) {
+      thr_k = radix_select(src_a, len_a, false, c.want, 0.0, M, par.inv_t, sh);
+      if (cut_p) {
+        __syncthreads();
+        if (tid == 0) { sh.hi = 0ull; sh.lo = 0ull; }
+        __syncthreads();
+        for (int i = tid; i < len_a; i += 1024) { const u64 x = src_a(i); if (x && x >= thr_k) fixed_add(&sh.hi, &sh.lo, weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t)); }
+        __syncthreads();
+        kept = fixed_d(sh.hi, sh.lo);
+      }
+      thr = thr_k;
+    }
+    if (cut_p) {
+      const double total = cut_k ? c.above_k + kept : c.total;
+      const double target = par.p * total;
+      if (tid < 64) {
+        const Found f = find_bin(w, true, 0u, target, cut_k ? c.k_bin : kBins - 1, cut_k ? kept : __shfl(w.m[15], 63));
+        if (tid == 0) s_found = f;
       }
       __syncthreads();
-      if (shift == 56) {
-        u64 hi = 0, lo = 0;
-        for (int j = 0; j < 256; ++j) { hi += bins.hi[j]; lo += bins.lo[j]; }
-        want = par.p * fixed_d(hi, lo);
-      }
-      if (tid < 64) { const RadixPick p = radix_pick(bins, shift >= 32, ties, want - above); if (tid == 0) s_pick = p; }
-      __syncthreads();
-      const RadixPick p = s_pick;
-      prefix = (prefix << 8) | (unsigned)p.bin;
-      thr = prefix << shift;
-      if (shift >= 32) {
-        above += p.mass_above;
-        if (p.count == 1) break;
-        if (shift == 32) {
-          // p.count entries of one score are left: as many of them as the mass still wants, at least one
-          const double n = ceil((want - above) / weight_of(score_of((unsigned)prefix), M, par.inv_t));
-          ties = n < 1.0 ? 1u : n < (double)p.count ? (unsigned)n : p.count;
-          if (ties == p.count) break;
-        }
+      const Found f = s_found;
+      if (cut_k && f.bin >= c.k_bin) {
+        auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
+        thr = radix_select(src, len_a, true, 0u, target - c.above_k, M, par.inv_t, sh);
       } else {
-        ties -= p.above;
-        if (ties == p.count) break;
+        const int bin = f.bin < c.p_lo ? c.p_lo : f.bin > c.p_hi ? c.p_hi : f.bin;
+        auto src = [&](int i) -> u64 {
+          if (!listed_b) return from_row(i, bin, bin);
+          const u64 x = lb[i];
+          return bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
+        };
+        thr = radix_select(src, listed_b ? (int)c.n_b : a.n_cols, true, 0u, target - f.before, M, par.inv_t, sh);
       }
+      if (thr < thr_k) thr = thr_k;                 // (an empty source gives 0)
     }
   }
-  // (the lower end of the bin found may lie below what top-k keeps)
-  if (tid == 0) a.state[r] = DrawState{thr > thr_k ? thr : thr_k, M, top ? 1 : 0};
+  if (tid == 0) { a.state[r].thr = thr; a.state[r].M = M; a.state[r].any = g.mx ? 1 : 0; }
+}
+
+// a row's threshold, largest score, and whether it has one
+__device__ __forceinline__ DrawState row_state(const DrawArgs& a, int r) {
+  if (a.cuts) return a.state[r];
+  const Range g = row_range(a, r);
+  return DrawState{1ull << 32, score_of(g.mx), g.mx ? 1 : 0, 0u, 0u};
 }
 
 // ---------------------------------------------------------------- running sums of the kept weights
-template <int DT> __device__ __forceinline__ double kept_weight(const RowView& v, int i, const DrawState& st, const RowPar& par) {
-  const unsigned k = entry_key<DT>(v, i);
+__device__ __forceinline__ double kept_of(unsigned k, int i, const DrawState& st, const RowPar& par) {
   if (number_of(k, i) < st.thr) return 0.0;
   const double w = weight_of(score_of(k), st.M, par.inv_t);
   return w >= par.m ? w : 0.0;
@@ -237,7 +559,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
   __shared__ double wsum[4];
   const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const RowView v = row_view<DT>(a, r);
-  const DrawState st = a.state[r];
+  const DrawState st = row_state(a, r);
   const RowPar par = row_par(a, r);
   double carry = 0.0;
   const int per_chunk = a.chunk / kBlock;
@@ -248,9 +570,11 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
     for (int j = 0; j < kTile / 1024; ++j) {
       const long long e = base + j * 1024 + tid * 4;
       double w = 0.0;
+      if (e < a.n_cols) {
+        const Four<DT> f = load_four<DT>(v, (int)e, a.n_cols);
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (e + q < a.n_cols) w += kept_weight<DT>(v, (int)(e + q), st, par);
+        for (int q = 0; q < 4; ++q) w += kept_of(four_key(f, q), (int)e + q, st, par);
+      }
       w += __shfl_xor(w, 1);
       w += __shfl_xor(w, 2);
       if ((tid & 3) == 0) blk[j * 64 + (tid >> 2)] = w;
@@ -277,7 +601,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a)
   __shared__ double wsum[4];
   const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const long long d = (long long)blockIdx.x * 256 + tid;
-  const DrawState st = a.state[r];
+  const DrawState st = row_state(a, r);
   const int nc = a.n_chunks;
   if (!st.any) {
     if (d < a.n_draws) { a.idx[(long long)r * a.n_draws + d] = -1; if (a.prob) a.prob[(long long)r * a.n_draws + d] = 0.f; }
@@ -323,7 +647,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a)
   for (int j = 0; j < kBlock; ++j) {
     const int i = i0 + j;
     if (i >= a.n_cols) break;
-    const double w = kept_weight<DT>(v, i, st, par);
+    const double w = kept_of(entry_key<DT>(v, i), i, st, par);
     if (w > 0.0) { at = i; w_at = w; }
     acc += w;
     if (acc > in_block && w > 0.0) break;
@@ -333,7 +657,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a)
 }
 
 // ---------------------------------------------------------------- host side
-struct DrawLayout { int chunk, n_chunks; size_t state, chunk_sum, block_incl, total; };
+struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, chunk_sum, block_incl, part_max, part_min, bin_cnt, bin_mass, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   DrawLayout l;
   // chunks of one tile; of more where a row would have over kMaxChunks of them
@@ -346,11 +670,32 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.state = take(sizeof(DrawState) * n_rows);
   l.chunk_sum = take(sizeof(double) * n_rows * l.n_chunks);
   l.block_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kBlock));
+  // Parts: about 1 024 workgroups over all rows, but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
+  // row's, which costs what reading some thousand entries does).
+  const long long cols = n_cols > 0 ? n_cols : 1;
+  long long parts = (1024 + n_rows - 1) / (n_rows > 0 ? n_rows : 1);
+  if (parts > (cols + 8191) / 8192) parts = (cols + 8191) / 8192;
+  if (parts > kMaxParts) parts = kMaxParts;
+  l.part_len = (int)(((cols + parts - 1) / parts + 2047) / 2048 * 2048);
+  l.n_parts = (int)((cols + l.part_len - 1) / l.part_len);
+  // Lists hold a quarter of a row: more entries in one bin mean that many equal scores, and then the row itself is read.
+  l.list_cap = (int)(cols / 4 > 4096 ? cols / 4 : 4096);
+  l.part_max = take(sizeof(unsigned) * n_rows * l.n_parts);
+  l.part_min = take(sizeof(unsigned) * n_rows * l.n_parts);
+  l.bin_cnt = take(sizeof(unsigned) * n_rows * kBins);
+  l.bin_mass = take(sizeof(u64) * n_rows * kBins);
+  l.list_a = take(sizeof(u64) * n_rows * l.list_cap);
+  l.list_b = take(sizeof(u64) * n_rows * l.list_cap);
   l.total = o;
   return l;
 }
 template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
-  hipLaunchKernelGGL(k_draw_select<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL(k_draw_range<DT>, dim3(a.n_parts, a.n_rows), dim3(256), 0, s, a);
+  if (a.cuts) {
+    hipLaunchKernelGGL(k_draw_hist<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
+    hipLaunchKernelGGL(k_draw_gather<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
+    hipLaunchKernelGGL(k_draw_cut<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
+  }
   hipLaunchKernelGGL(k_draw_sums<DT>, dim3(a.n_chunks, a.n_rows), dim3(256), 0, s, a);
   hipLaunchKernelGGL(k_draw_pick<DT>, dim3((unsigned)(((long long)a.n_draws + 255) / 256), a.n_rows), dim3(256), 0, s, a);
 }
@@ -359,7 +704,7 @@ template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
 using namespace psl;
 
 extern "C" int64_t psl_draw_ws_bytes(int32_t n_rows, int32_t n_cols) {
-  if (n_rows < 0 || n_cols < 0 || n_rows > 65535 || n_cols > 0x7ffff000) { set_error("psl_draw_ws_bytes: %d rows of %d", n_rows, n_cols); return PSL_ERR_ARG; }
+  if (n_rows < 0 || n_cols < 0 || n_rows > 65535 || n_cols > 0x7f000000) { set_error("psl_draw_ws_bytes: %d rows of %d", n_rows, n_cols); return PSL_ERR_ARG; }
   return (int64_t)draw_layout(n_rows, n_cols).total;
 }
 
@@ -367,7 +712,7 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
 #define PSL_BAD(...) do { set_error(__VA_ARGS__); return PSL_ERR_ARG; } while (0)
   if (!q) PSL_BAD("psl_draw_indices: null argument");
   if (q->dtype < PSL_F32 || q->dtype > PSL_F16) PSL_BAD("psl_draw_indices: unknown dtype %d", q->dtype);
-  if (q->n_rows < 0 || q->n_rows > 65535 || q->n_cols < 0 || q->n_cols > 0x7ffff000 || q->n_draws < 0)
+  if (q->n_rows < 0 || q->n_rows > 65535 || q->n_cols < 0 || q->n_cols > 0x7f000000 || q->n_draws < 0)
     PSL_BAD("psl_draw_indices: %d rows (up to 65535) of %d entries, %d draws", q->n_rows, q->n_cols, q->n_draws);
   if (q->n_rows == 0 || q->n_draws == 0) return PSL_OK;
   if ((!q->scores && q->n_cols) || !q->u || !q->idx || !q->ws) PSL_BAD("psl_draw_indices: missing pointer");
@@ -392,6 +737,10 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   char* w = (char*)q->ws;
   a.state = (DrawState*)(w + l.state); a.chunk_sum = (double*)(w + l.chunk_sum); a.block_incl = (double*)(w + l.block_incl);
   a.n_chunks = l.n_chunks; a.chunk = l.chunk;
+  a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
+  a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass);
+  a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
+  a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
   hipStream_t s = (hipStream_t)stream;
   if (q->dtype == PSL_F32) launch_draw<PSL_F32>(a, s);
   else if (q->dtype == PSL_BF16) launch_draw<PSL_BF16>(a, s);

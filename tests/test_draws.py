@@ -66,7 +66,7 @@ def test_workspace_sizes_and_nothing_to_do():
     assert L.psl_draw_ws_bytes(-1, 5) < 0 and L.psl_draw_ws_bytes(5, -1) < 0 and L.psl_draw_ws_bytes(70000, 5) < 0
     assert L.psl_draw_ws_bytes(0, 0) >= 0 and L.psl_draw_ws_bytes(1, 0) > 0
     assert L.psl_draw_ws_bytes(12, 816000) < 12 * 816000 * 8          # below one double to an entry
-    assert L.psl_draw_ws_bytes(65535, 0x7ffff000) > 1 << 40
+    assert L.psl_draw_ws_bytes(65535, 0x7f000000) > 1 << 40
     assert L.psl_draw_indices(None, None) == -1
     assert L.psl_draw_indices(C.byref(_args(n_rows=0, scores=None)), None) == 0
     assert L.psl_draw_indices(C.byref(_args(n_draws=0, u=None)), None) == 0
@@ -320,3 +320,34 @@ def test_tensors_of_another_device():
     _check(s, u, dev="cuda:1", top_k=30)
     with pytest.raises(ValueError):
         frame_ops.draw_indices(s.to("cuda:1"), u.to("cuda:0"))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_many_equal_scores_in_a_long_row(dtype):
+    """More candidates in the deciding bin than its list holds (a quarter of the row), and just fewer."""
+    V = 60000
+    g = torch.Generator().manual_seed(4)
+    for share in (0.1, 0.24, 0.26, 0.6):
+        s = torch.randn(2, V, generator=g)
+        flat = torch.rand(2, V, generator=g) < share
+        s[flat] = 0.5
+        s = s.to(DT[dtype])
+        u = torch.rand(2, 200, generator=g)
+        above = int((s[0] > 0.5).sum())
+        for cut in (dict(top_k=above + 1), dict(top_k=above + int(share * V / 3)), dict(top_p=0.7), dict(top_p=0.6, top_k=above + int(share * V / 2)),
+                    dict(top_k=V - 5), dict(top_p=0.99, temperature=0.5), dict(top_p=0.2, top_k=above)):
+            _check(s, u, where=f"{share} {cut}", **cut)
+
+
+@gpu
+def test_wide_and_narrow_ranges():
+    """Scores that fill one bin, a few, or mostly the last one."""
+    V = 30011
+    g = torch.Generator().manual_seed(6)
+    u = torch.rand(1, 300, generator=g)
+    base = torch.randn(1, V, generator=g)
+    for s in (base * 1e-6, base * 1e-30, base * 1e4, base * 1e30, base.exp().exp(), torch.cat([base[:, :V - 1] * 1e-3, torch.tensor([[50.0]])], 1),
+              torch.where(base > 2.5, base, torch.full_like(base, torch.finfo(torch.float32).min))):
+        for cut in (dict(top_k=1000), dict(top_p=0.9), dict(top_k=20000, top_p=0.99), dict(top_p=0.5, temperature=1e-3), dict(top_k=5000, temperature=1e4), dict(top_p=1 - 1e-9), dict(top_k=V - 1)):
+            _check(s, u, where=str(cut), **cut)
