@@ -25,8 +25,9 @@ struct DrawArgs {
   int cuts;                    // whether any row may have a limit (else the launches that find thresholds are left out)
   int n_parts, part_len;       // pieces of a row in the launches before k_draw_sums
   struct DrawState* state;     // [n_rows]
+  struct DrawCut* cut;         // [n_rows]
   unsigned* part_max; unsigned* part_min;       // [n_rows][n_parts] keys
-  unsigned* bin_cnt; unsigned long long* bin_mass;       // [n_rows][kBins]
+  unsigned* bin_cnt; unsigned long long* bin_mass;       // [n_rows][kBins]; k_draw_bins leaves running sums (double) in bin_mass
   unsigned long long* list_a; unsigned long long* list_b; int list_cap;      // [n_rows][list_cap] numbers of candidate entries
   double* chunk_sum;           // [n_rows][n_chunks]
   double* block_incl;          // [n_rows][n_chunks * chunk / 16]: running sums inside a chunk, at the end of each 16 entries
@@ -36,6 +37,14 @@ struct DrawState {
   u64 thr;                     // kept: number(entry) >= thr
   float M; int any;            // largest allowed score; whether there is one
   unsigned n_a, n_b;           // fill of the two lists
+};
+
+struct DrawCut {
+  unsigned n_valid, want;          // want: entries of k_bin that top-k keeps
+  int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
+  unsigned n_a, n_b;               // entries of k_bin; of [p_lo, p_hi]
+  unsigned key[4];                 // keys of k_bin: [0] .. [1] - 1; of [p_lo, p_hi]: [2] .. [3] - 1
+  double above_k, total;           // mass of the bins before k_bin; of all
 };
 
 constexpr int kBlock = 16;     // entries to a stored running sum: one 64-byte line of fp32 scores
@@ -226,13 +235,7 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   }
 }
 
-// Which bins the two limits fall into.  Wavefront 0; lane l holds bins 16 l .. 16 l + 15, the largest scores first.
-struct Cut {
-  unsigned n_valid, want;          // want: entries of k_bin that top-k keeps
-  int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
-  double above_k, total;           // mass of the bins before k_bin; of all
-  unsigned n_a, n_b;               // entries of k_bin; of [p_lo, p_hi]
-};
+// Which bins the two limits fall into.  One wavefront; lane l holds bins 16 l .. 16 l + 15, the largest scores first.
 struct LaneBins { unsigned c[16]; double m[16]; unsigned c_before; double m_before; };
 __device__ __forceinline__ LaneBins load_bins(const DrawArgs& a, int r, const Binning& b) {
   LaneBins w;
@@ -281,8 +284,8 @@ __device__ __forceinline__ Found find_bin(const LaneBins& w, bool by_mass, unsig
   f.before = __shfl(send.before, src); f.mass = __shfl(send.mass, src);
   return f;
 }
-__device__ __forceinline__ Cut make_cut(const LaneBins& w, const RowPar& par) {
-  Cut c;
+__device__ __forceinline__ DrawCut make_cut(const LaneBins& w, const RowPar& par) {
+  DrawCut c;
   unsigned cs = 0; double ms = 0.0;
 #pragma unroll
   for (int j = 0; j < 16; ++j) { cs += w.c[j]; ms += w.m[j]; }
@@ -310,48 +313,86 @@ __device__ __forceinline__ Cut make_cut(const LaneBins& w, const RowPar& par) {
   return c;
 }
 
-// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.
-template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs a) {
-  __shared__ Cut s_cut;
-  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+// smallest key of the row whose bin is at most `bin` (bins fall as keys rise; the row's largest key is in bin 0)
+__device__ __forceinline__ unsigned first_key(const Binning& b, const Range& g, int bin) {
+  unsigned lo = g.mn, hi = g.mx;
+  while (lo < hi) {
+    const unsigned mid = lo + ((hi - lo) >> 1);
+    if (bin_of(b, score_of(mid)) <= bin) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+// One wavefront to a row (in every workgroup of k_draw_gather instead, this cost each of them 8 us).
+__global__ __launch_bounds__(64) void k_draw_bins(DrawArgs a) {
+  const int r = blockIdx.x, lane = threadIdx.x;
   const RowPar par = row_par(a, r);
   if (!has_cut(par)) return;
   const Range g = row_range(a, r);
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
-  if (tid < 64) { const Cut c = make_cut(load_bins(a, r, b), par); if (tid == 0) s_cut = c; }
-  __syncthreads();
-  const Cut c = s_cut;
+  const LaneBins w = load_bins(a, r, b);
+  DrawCut c = make_cut(w, par);
+  double* cum = (double*)(a.bin_mass + (long long)r * kBins) + 16 * lane;
+  double m = w.m_before;
+#pragma unroll
+  for (int j = 0; j < 16; ++j) { m += w.m[j]; cum[j] = m; }
+  if (lane < 4) {
+    const int bin = lane == 0 ? c.k_bin : lane == 1 ? c.k_bin - 1 : lane == 2 ? c.p_hi : c.p_lo - 1;
+    const unsigned key = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
+    a.cut[r].key[lane] = key;
+  }
+  if (lane == 0) {
+    DrawCut* o = a.cut + r;
+    o->n_valid = c.n_valid; o->want = c.want; o->k_bin = c.k_bin; o->p_lo = c.p_lo; o->p_hi = c.p_hi; o->n_a = c.n_a; o->n_b = c.n_b;
+    o->above_k = c.above_k; o->total = c.total;
+  }
+}
+
+// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.  A bin
+// is an interval of keys: an entry costs integer comparisons only.  A workgroup collects in LDS and asks once for its
+// places in the row's list (a global atomic for every wavefront that found something made this 112 us for twelve rows of
+// 816 000); what does not fit there goes to the list by itself.
+constexpr int kListBuf = 1024;
+struct ListBuf { u64 e[kListBuf]; unsigned n, at; };
+__device__ __forceinline__ void list_add(ListBuf& b, u64 x, u64* dst, unsigned* fill) {
+  const unsigned j = atomicAdd(&b.n, 1u);
+  if (j < kListBuf) b.e[j] = x;
+  else dst[atomicAdd(fill, 1u)] = x;
+}
+template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs a) {
+  __shared__ ListBuf buf_a, buf_b;
+  const int r = blockIdx.y, tid = threadIdx.x;
+  const RowPar par = row_par(a, r);
+  if (!has_cut(par)) return;
+  if (tid == 0) { buf_a.n = 0u; buf_b.n = 0u; }
+  const Range g = row_range(a, r);
+  if (!g.mx) return;
+  const DrawCut& c = a.cut[r];
   const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.n_b && c.n_b <= (unsigned)a.list_cap;
   if (!do_a && !do_b) return;
+  // (no such bin: an empty interval)
+  const unsigned a0 = do_a ? c.key[0] : 1u, a1 = do_a ? c.key[1] : 0u, b0 = do_b ? c.key[2] : 1u, b1 = do_b ? c.key[3] : 0u;
   const RowView v = row_view<DT>(a, r);
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
   u64* la = a.list_a + (long long)r * a.list_cap;
   u64* lb = a.list_b + (long long)r * a.list_cap;
-  for (int base = i0; base < i1; base += 2048) {
-    const int i = base + tid * 4;
+#pragma unroll 2
+  for (int i = i0 + tid * 4; i < i1; i += 2048) {
     const Four<DT> f = load_four<DT>(v, i, i1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const unsigned k = four_key(f, q);
-      const int bin = k ? bin_of(b, score_of(k)) : -1;
-      const bool in_a = do_a && bin == c.k_bin, in_b = do_b && bin >= c.p_lo && bin <= c.p_hi;
-      const u64 ba = __ballot(in_a), bb = __ballot(in_b);
-      const u64 below = (1ull << lane) - 1ull;
-      if (ba) {
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(&a.state[r].n_a, (unsigned)__popcll(ba));
-        at = __shfl(at, 0);
-        if (in_a) la[at + (unsigned)__popcll(ba & below)] = number_of(k, i + q);
-      }
-      if (bb) {
-        unsigned at = 0;
-        if (lane == 0) at = atomicAdd(&a.state[r].n_b, (unsigned)__popcll(bb));
-        at = __shfl(at, 0);
-        if (in_b) lb[at + (unsigned)__popcll(bb & below)] = number_of(k, i + q);
-      }
+      if (k >= a0 && k < a1) list_add(buf_a, number_of(k, i + q), la, &a.state[r].n_a);
+      if (k >= b0 && k < b1) list_add(buf_b, number_of(k, i + q), lb, &a.state[r].n_b);
     }
   }
+  __syncthreads();
+  const unsigned na = min(buf_a.n, (unsigned)kListBuf), nb = min(buf_b.n, (unsigned)kListBuf);
+  if (tid == 0 && na) buf_a.at = atomicAdd(&a.state[r].n_a, na);
+  if (tid == 64 && nb) buf_b.at = atomicAdd(&a.state[r].n_b, nb);
+  __syncthreads();
+  for (unsigned j = tid; j < na; j += 512) la[buf_a.at + j] = buf_a.e[j];
+  for (unsigned j = tid; j < nb; j += 512) lb[buf_b.at + j] = buf_b.e[j];
 }
 
 // ---------------------------------------------------------------- the threshold among those entries, by radix selection
@@ -405,29 +446,52 @@ __device__ __forceinline__ RadixPick radix_pick(const RadixBins& b, bool by_mass
   return r;
 }
 
-// Digits of eight bits of the numbers that src(i) gives for i < n (0: not among them), from the highest in which they differ;
-// a level counts the numbers whose higher digits are the ones found so far.  Ends as soon as the digit found is taken whole.
-// By count: the smallest of the first `want`.  By mass: the smallest of the shortest prefix that weighs want_mass.
-template <class Src> __device__ u64 radix_select(const Src& src, int n, bool by_mass, unsigned want, double want_mass, float M, double inv_t,
-                                                 RadixShared& sh) {
-  const int tid = threadIdx.x;
-  u64 mx = 0ull, mn = ~0ull;
-  for (int i = tid; i < n; i += 1024) { const u64 x = src(i); if (x) { mx = x > mx ? x : mx; mn = x < mn ? x : mn; } }
+// The numbers that src(i) gives for i < n (0: not among them), up to four of them to a thread in registers.
+constexpr int kHeld = 4;
+template <class Src> struct Numbers {
+  const Src& src; int n; u64 x[kHeld];
+  __device__ __forceinline__ Numbers(const Src& src_, int n_) : src(src_), n(n_) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) { const int i = threadIdx.x + 1024 * j; x[j] = n <= kHeld * 1024 && i < n ? src(i) : 0ull; }
+  }
+  template <class F> __device__ __forceinline__ void each(const F& f) const {
+    if (n <= kHeld * 1024) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) if (x[j]) f(x[j]);
+    } else {
+      for (int i = threadIdx.x; i < n; i += 1024) { const u64 y = src(i); if (y) f(y); }
+    }
+  }
+};
+__device__ __forceinline__ void block_bounds(u64& mx, u64& mn, RadixShared& sh) {
   for (int o = 32; o > 0; o >>= 1) {
     const u64 x = __shfl_xor(mx, o), y = __shfl_xor(mn, o);
     mx = x > mx ? x : mx; mn = y < mn ? y : mn;
   }
   __syncthreads();
-  if ((tid & 63) == 0) { sh.mx[tid >> 6] = mx; sh.mn[tid >> 6] = mn; }
+  if ((threadIdx.x & 63) == 0) { sh.mx[threadIdx.x >> 6] = mx; sh.mn[threadIdx.x >> 6] = mn; }
   __syncthreads();
   for (int j = 0; j < 16; ++j) { mx = sh.mx[j] > mx ? sh.mx[j] : mx; mn = sh.mn[j] < mn ? sh.mn[j] : mn; }
+}
+
+// Digits of up to eight bits, from the highest in which the numbers differ (none across bit 32, where the score ends); a
+// level counts the numbers whose higher digits are the ones found so far.  Ends as soon as the digit found is taken whole.
+// By count: the smallest of the first `want`.  By mass: the smallest of the shortest prefix that weighs want_mass.
+template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool by_mass, unsigned want, double want_mass, float M, double inv_t,
+                                                 RadixShared& sh) {
+  const int tid = threadIdx.x;
+  u64 mx = 0ull, mn = ~0ull;
+  num.each([&](u64 x) { mx = x > mx ? x : mx; mn = x < mn ? x : mn; });
+  block_bounds(mx, mn, sh);
   if (mx <= mn) return mx == mn ? mx : 0ull;
-  int shift = (63 - __clzll((long long)(mx ^ mn))) & ~7;
-  u64 prefix = shift == 56 ? 0ull : mx >> (shift + 8), thr = mn;
+  int hi = 64 - __clzll((long long)(mx ^ mn));          // bits from here on are equal
+  u64 prefix = hi == 64 ? 0ull : mx >> hi;
   bool mass_level = by_mass;
-  for (; shift >= 0; shift -= 8) {
-    if (mass_level && shift < 32) {
-      // one score is left: as many of its entries as the mass still wants, at least one (all of them: the bin just found)
+  int lo = hi;
+  while (hi > 0) {
+    lo = hi > 32 ? (hi - 8 > 32 ? hi - 8 : 32) : (hi - 8 > 0 ? hi - 8 : 0);
+    if (mass_level && hi <= 32) {
+      // one score is left: as many of its entries as the mass still wants, at least one (all of them: the last)
       const double k = ceil(want_mass / weight_of(score_of((unsigned)(mx >> 32)), M, inv_t));
       want = k < 1.0 ? 1u : k < 4294967295.0 ? (unsigned)k : 0xffffffffu;
       mass_level = false;
@@ -435,105 +499,100 @@ template <class Src> __device__ u64 radix_select(const Src& src, int n, bool by_
     __syncthreads();
     for (int j = tid; j < 256; j += 1024) { sh.bins.cnt[j] = 0u; sh.bins.hi[j] = 0ull; sh.bins.lo[j] = 0ull; }
     __syncthreads();
-    for (int i = tid; i < n; i += 1024) {
-      const u64 x = src(i);
-      if (x && (shift == 56 || (x >> (shift + 8)) == prefix)) {
-        const int d = (int)((x >> shift) & 255);
+    num.each([&](u64 x) {
+      if (hi == 64 || (x >> hi) == prefix) {
+        const int d = (int)((x >> lo) & ((1u << (hi - lo)) - 1u));
         atomicAdd(&sh.bins.cnt[d], 1u);
         if (mass_level) fixed_add(&sh.bins.hi[d], &sh.bins.lo[d], weight_of(score_of((unsigned)(x >> 32)), M, inv_t));
       }
-    }
+    });
     __syncthreads();
     if (tid < 64) { const RadixPick p = radix_pick(sh.bins, mass_level, want, want_mass); if (tid == 0) sh.pick = p; }
     __syncthreads();
     const RadixPick p = sh.pick;
-    prefix = (prefix << 8) | (unsigned)p.bin;
-    thr = prefix << shift;               // (exact once every digit is found)
+    prefix = (prefix << (hi - lo)) | (unsigned)p.bin;
+    hi = lo;
     if (mass_level) {
       want_mass -= p.mass_above;
       if (p.count == 1) break;
-      if (shift == 32) mx = prefix << 32;        // the score that is left
+      if (lo == 32) mx = prefix << 32;        // the score that is left
     } else {
       want -= p.above;
       if (want >= p.count) break;
     }
   }
-  if (shift <= 0) return thr;
+  if (lo == 0) return prefix;
   // The digit is taken whole.  Its smallest number, not its lower end: below that end of src's scores others may begin.
-  mn = ~0ull;
-  for (int i = tid; i < n; i += 1024) { const u64 x = src(i); if (x && (x >> shift) == prefix) mn = x < mn ? x : mn; }
-  for (int o = 32; o > 0; o >>= 1) { const u64 y = __shfl_xor(mn, o); mn = y < mn ? y : mn; }
-  __syncthreads();
-  if ((tid & 63) == 0) sh.mn[tid >> 6] = mn;
-  __syncthreads();
-  for (int j = 0; j < 16; ++j) mn = sh.mn[j] < mn ? sh.mn[j] : mn;
+  mx = 0ull; mn = ~0ull;
+  num.each([&](u64 x) { if ((x >> lo) == prefix) mn = x < mn ? x : mn; });
+  block_bounds(mx, mn, sh);
   return mn;
 }
 
 template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
   __shared__ RadixShared sh;
-  __shared__ Cut s_cut;
-  __shared__ Found s_found;
+  __shared__ int s_bin;
   const int r = blockIdx.x, tid = threadIdx.x;
   const RowPar par = row_par(a, r);
   const Range g = row_range(a, r);
   const float M = score_of(g.mx);
   u64 thr = 1ull << 32;                             // every allowed entry
   if (g.mx && has_cut(par)) {
-    const Binning b = make_binning(g, par.inv_t, a.n_cols);
     const RowView v = row_view<DT>(a, r);
     const u64* la = a.list_a + (long long)r * a.list_cap;
     const u64* lb = a.list_b + (long long)r * a.list_cap;
-    LaneBins w;
-    if (tid < 64) { w = load_bins(a, r, b); const Cut c = make_cut(w, par); if (tid == 0) s_cut = c; }
-    __syncthreads();
-    const Cut c = s_cut;
+    const double* cum = (const double*)(a.bin_mass + (long long)r * kBins);
+    const DrawCut& c = a.cut[r];
     const bool listed_a = c.n_a <= (unsigned)a.list_cap, listed_b = c.n_b <= (unsigned)a.list_cap;
     // a list that was too long to be written: the row itself, entry by entry
-    auto from_row = [&](int i, int lo, int hi) -> u64 {
+    const unsigned a0 = c.key[0], a1 = c.key[1];
+    auto src_a = [&](int i) -> u64 {
+      if (listed_a) return la[i];
       const unsigned k = entry_key<DT>(v, i);
-      const int bin = k ? bin_of(b, score_of(k)) : -1;
-      return bin >= lo && bin <= hi && k ? number_of(k, i) : 0ull;
+      return k >= a0 && k < a1 ? number_of(k, i) : 0ull;
     };
-    auto src_a = [&](int i) -> u64 { return listed_a ? la[i] : from_row(i, c.k_bin, c.k_bin); };
     const int len_a = listed_a ? (int)c.n_a : a.n_cols;
-    u64 thr_k = thr;
-    double kept = 0.0;                              // mass of what top-k keeps of its bin
     const bool cut_k = c.k_bin < kBins, cut_p = par.p < 1.0 && par.k != 1;
+    double kept = 0.0;                              // mass of what top-k keeps of its bin
+    bool p_in_a = false;
     if (cut_k) {
-      thr_k = radix_select(src_a, len_a, false, c.want, 0.0, M, par.inv_t, sh);
+      const Numbers<decltype(src_a)> num(src_a, len_a);
+      const u64 thr_k = radix_select(num, false, c.want, 0.0, M, par.inv_t, sh);
+      thr = thr_k;
       if (cut_p) {
         __syncthreads();
         if (tid == 0) { sh.hi = 0ull; sh.lo = 0ull; }
         __syncthreads();
-        for (int i = tid; i < len_a; i += 1024) { const u64 x = src_a(i); if (x && x >= thr_k) fixed_add(&sh.hi, &sh.lo, weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t)); }
+        num.each([&](u64 x) { if (x >= thr_k) fixed_add(&sh.hi, &sh.lo, weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t)); });
         __syncthreads();
         kept = fixed_d(sh.hi, sh.lo);
+        const double target = par.p * (c.above_k + kept);
+        p_in_a = target > c.above_k;                // (the running sums before k_bin end at above_k)
+        if (p_in_a) {
+          auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
+          thr = radix_select(Numbers<decltype(src)>(src, len_a), true, 0u, target - c.above_k, M, par.inv_t, sh);
+        }
       }
-      thr = thr_k;
     }
-    if (cut_p) {
-      const double total = cut_k ? c.above_k + kept : c.total;
-      const double target = par.p * total;
-      if (tid < 64) {
-        const Found f = find_bin(w, true, 0u, target, cut_k ? c.k_bin : kBins - 1, cut_k ? kept : __shfl(w.m[15], 63));
-        if (tid == 0) s_found = f;
-      }
+    if (cut_p && !p_in_a && c.p_hi >= c.p_lo) {
+      const double target = par.p * (cut_k ? c.above_k + kept : c.total);
+      // first bin of [p_lo, p_hi] whose running sum reaches the target
+      if (tid == 0) s_bin = c.p_hi;
       __syncthreads();
-      const Found f = s_found;
-      if (cut_k && f.bin >= c.k_bin) {
-        auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
-        thr = radix_select(src, len_a, true, 0u, target - c.above_k, M, par.inv_t, sh);
-      } else {
-        const int bin = f.bin < c.p_lo ? c.p_lo : f.bin > c.p_hi ? c.p_hi : f.bin;
-        auto src = [&](int i) -> u64 {
-          if (!listed_b) return from_row(i, bin, bin);
-          const u64 x = lb[i];
-          return bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
-        };
-        thr = radix_select(src, listed_b ? (int)c.n_b : a.n_cols, true, 0u, target - f.before, M, par.inv_t, sh);
-      }
-      if (thr < thr_k) thr = thr_k;                 // (an empty source gives 0)
+      for (int j = c.p_lo + tid; j < c.p_hi; j += 1024) if (cum[j] >= target) atomicMin(&s_bin, j);
+      __syncthreads();
+      const int bin = s_bin;
+      const Binning b = make_binning(g, par.inv_t, a.n_cols);
+      const unsigned b0 = c.key[2], b1 = c.key[3];
+      auto src = [&](int i) -> u64 {
+        u64 x = 0ull;
+        if (listed_b) x = lb[i];
+        else { const unsigned k = entry_key<DT>(v, i); if (k >= b0 && k < b1) x = number_of(k, i); }
+        return x && bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
+      };
+      const double before = bin ? cum[bin - 1] : 0.0;
+      const u64 t = radix_select(Numbers<decltype(src)>(src, listed_b ? (int)c.n_b : a.n_cols), true, 0u, target - before, M, par.inv_t, sh);
+      if (t > thr) thr = t;                         // (an empty source gives 0)
     }
   }
   if (tid == 0) { a.state[r].thr = thr; a.state[r].M = M; a.state[r].any = g.mx ? 1 : 0; }
@@ -657,7 +716,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a)
 }
 
 // ---------------------------------------------------------------- host side
-struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, chunk_sum, block_incl, part_max, part_min, bin_cnt, bin_mass, list_a, list_b, total; };
+struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, block_incl, part_max, part_min, bin_cnt, bin_mass, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   DrawLayout l;
   // chunks of one tile; of more where a row would have over kMaxChunks of them
@@ -668,6 +727,7 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   size_t o = 0;
   auto take = [&o](size_t bytes) { const size_t at = o; o += (bytes + 255) & ~(size_t)255; return at; };
   l.state = take(sizeof(DrawState) * n_rows);
+  l.cut = take(sizeof(DrawCut) * n_rows);
   l.chunk_sum = take(sizeof(double) * n_rows * l.n_chunks);
   l.block_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kBlock));
   // Parts: about 1 024 workgroups over all rows, but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
@@ -693,6 +753,7 @@ template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(k_draw_range<DT>, dim3(a.n_parts, a.n_rows), dim3(256), 0, s, a);
   if (a.cuts) {
     hipLaunchKernelGGL(k_draw_hist<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
+    hipLaunchKernelGGL(k_draw_bins, dim3(a.n_rows), dim3(64), 0, s, a);
     hipLaunchKernelGGL(k_draw_gather<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
     hipLaunchKernelGGL(k_draw_cut<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
   }
@@ -735,7 +796,7 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.t_all = q->temperature_all; a.p_all = q->top_p_all; a.m_all = q->min_p_all; a.k_all = q->top_k_all;
   a.u = q->u; a.u_stride = q->u_stride; a.idx = q->idx; a.prob = q->prob;
   char* w = (char*)q->ws;
-  a.state = (DrawState*)(w + l.state); a.chunk_sum = (double*)(w + l.chunk_sum); a.block_incl = (double*)(w + l.block_incl);
+  a.state = (DrawState*)(w + l.state); a.cut = (DrawCut*)(w + l.cut); a.chunk_sum = (double*)(w + l.chunk_sum); a.block_incl = (double*)(w + l.block_incl);
   a.n_chunks = l.n_chunks; a.chunk = l.chunk;
   a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
   a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass);
