@@ -31,7 +31,9 @@ struct DrawArgs {
   unsigned long long* list_a; unsigned long long* list_b; int list_cap;      // [n_rows][list_cap] numbers of candidate entries
   double* chunk_sum;           // [n_rows][n_chunks]
   double* block_incl;          // [n_rows][n_chunks * chunk / 16]: running sums inside a chunk, at the end of each 16 entries
+  unsigned short* block_kept;  // [n_rows][n_chunks * chunk / 16]: which of a block's entries are kept
   int n_chunks, chunk;         // entries of a chunk (a multiple of kTile)
+  int pick_wgs, coarse_blocks; long long pick_len;      // k_draw_pick: workgroups and draws to a workgroup; blocks between places in LDS
 };
 struct DrawState {
   u64 thr;                     // kept: number(entry) >= thr
@@ -93,11 +95,29 @@ __device__ __forceinline__ RowPar row_par(const DrawArgs& a, int r) {
   q.inv_t = t > 0.0 ? 1.0 / t : 1.0;
   return q;
 }
+// exp(-x) for x >= 0 to about one unit of the last place, in 14 fp64 instructions and one LDS read (the library's takes about
+// 35, and the weights of a pass are what it computes): x = (n + f) ln2 / 64 with |f| <= 1/2, 2^(-(n mod 64) / 64) from a table of
+// 64, e^-r = 1 - r + r^2/2 - r^3/6 + r^4/24 - r^5/120 for the rest |r| <= ln2 / 128 (the next term is below 4e-17), 2^-(n / 64)
+// into the exponent.  Beyond x = 1100 the result is 0; a NaN counts as that.
+struct ExpTable { double t[64]; };
+__device__ __forceinline__ void exp_table_init(ExpTable& e) { if (threadIdx.x < 64) e.t[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0); }
+__device__ __forceinline__ double exp_neg(double x, const ExpTable& e) {
+  x = fmin(x, 1100.0);
+  const double n = rint(x * 92.332482616893656);        // 64 / ln2
+  double r = fma(n, -0x1.62e42fefa39efp-7, x);          // ln2 / 64, and what that number leaves of it
+  r = fma(n, -0x1.abc9e3b39803fp-62, r);
+  const int k = (int)n;
+  double p = fma(r, -1.0 / 120.0, 1.0 / 24.0);
+  p = fma(r, p, -1.0 / 6.0);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, -1.0);
+  p = fma(r, p, 1.0);
+  return ldexp(e.t[k & 63] * p, -(k >> 6));
+}
 // weight of an allowed score; +inf among the scores takes all
-__device__ __forceinline__ double weight_of(float s, float M, double inv_t) {
-  if (s == M) return 1.0;
-  if (M == __builtin_inff()) return 0.0;
-  return exp(((double)s - (double)M) * inv_t);
+__device__ __forceinline__ double weight_of(float s, float M, double inv_t, const ExpTable& e) {
+  const double w = exp_neg(((double)M - (double)s) * inv_t, e);
+  return s == M ? 1.0 : M == __builtin_inff() ? 0.0 : w;
 }
 
 __device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up(v, o); }
@@ -190,7 +210,7 @@ __device__ __forceinline__ Binning make_binning(const Range& g, double inv_t, in
   b.c = range > 0.0 ? (double)kBins / range : 0.0;
   if (!(b.c < 1e300)) b.c = 1e300;
   b.oct = range > 0.0 ? range / (double)kBins * 1.4426950408889634 : 0.0;        // binary orders per bin
-  b.q = 62 - (32 - __clz(n_cols));
+  b.q = min(62 - (32 - __clz(n_cols)), 51);        // the row's sum below 2^63, an entry's below to_integer's limit
   return b;
 }
 __device__ __forceinline__ int bin_of(const Binning& b, float s) {
@@ -199,14 +219,19 @@ __device__ __forceinline__ int bin_of(const Binning& b, float s) {
 }
 __device__ __forceinline__ int bin_shift(const Binning& b, int bin) { return b.q + (int)((double)bin * b.oct); }
 
+// 0 <= x < 2^52 to the nearest integer: 2^52 + x has it in its low bits
+__device__ __forceinline__ u64 to_integer(double x) { return (u64)__double_as_longlong(x + 0x1p52) & 0xfffffffffffffull; }
+
 template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
   __shared__ unsigned cnt[kBins];
   __shared__ u64 mass[kBins];
+  __shared__ ExpTable s_exp;
   const int r = blockIdx.y, tid = threadIdx.x;
   const RowPar par = row_par(a, r);
   if (!has_cut(par)) return;
+  exp_table_init(s_exp);
   for (int j = tid; j < kBins; j += 512) { cnt[j] = 0u; mass[j] = 0ull; }
-  const Range g = row_range(a, r);        // (its barrier also covers the bins)
+  const Range g = row_range(a, r);        // (its barrier also covers the bins and the table)
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
   const float M = score_of(g.mx);
@@ -222,7 +247,7 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
         const float s = score_of(k);
         const int bin = bin_of(b, s);
         atomicAdd(&cnt[bin], 1u);
-        if (weigh) atomicAdd(&mass[bin], (u64)(ldexp(weight_of(s, M, par.inv_t), bin_shift(b, bin)) + 0.5));
+        if (weigh) atomicAdd(&mass[bin], to_integer(ldexp(weight_of(s, M, par.inv_t, s_exp), bin_shift(b, bin))));
       }
     }
   }
@@ -399,7 +424,7 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
 // 256 digits of (count, mass): masses are summed as integers, 32 bits before and 32 behind the point at 2^-32, so their sum has no order
 struct RadixBins { unsigned cnt[256]; u64 hi[256], lo[256]; };
 struct RadixPick { int bin; unsigned above, count; double mass_above, mass; };
-struct RadixShared { RadixBins bins; RadixPick pick; u64 mx[16], mn[16]; u64 hi, lo; };
+struct RadixShared { RadixBins bins; RadixPick pick; u64 mx[16], mn[16]; u64 hi, lo; ExpTable exp; };
 
 __device__ __forceinline__ double fixed_d(u64 hi, u64 lo) { return (double)hi * 0x1p-32 + (double)lo * 0x1p-64; }
 __device__ __forceinline__ void fixed_add(u64* hi, u64* lo, double w) {
@@ -492,7 +517,7 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
     lo = hi > 32 ? (hi - 8 > 32 ? hi - 8 : 32) : (hi - 8 > 0 ? hi - 8 : 0);
     if (mass_level && hi <= 32) {
       // one score is left: as many of its entries as the mass still wants, at least one (all of them: the last)
-      const double k = ceil(want_mass / weight_of(score_of((unsigned)(mx >> 32)), M, inv_t));
+      const double k = ceil(want_mass / weight_of(score_of((unsigned)(mx >> 32)), M, inv_t, sh.exp));
       want = k < 1.0 ? 1u : k < 4294967295.0 ? (unsigned)k : 0xffffffffu;
       mass_level = false;
     }
@@ -503,7 +528,7 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
       if (hi == 64 || (x >> hi) == prefix) {
         const int d = (int)((x >> lo) & ((1u << (hi - lo)) - 1u));
         atomicAdd(&sh.bins.cnt[d], 1u);
-        if (mass_level) fixed_add(&sh.bins.hi[d], &sh.bins.lo[d], weight_of(score_of((unsigned)(x >> 32)), M, inv_t));
+        if (mass_level) fixed_add(&sh.bins.hi[d], &sh.bins.lo[d], weight_of(score_of((unsigned)(x >> 32)), M, inv_t, sh.exp));
       }
     });
     __syncthreads();
@@ -532,6 +557,8 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
 template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
   __shared__ RadixShared sh;
   __shared__ int s_bin;
+  const ExpTable& s_exp = sh.exp;
+  exp_table_init(sh.exp);               // (row_range's barrier covers it)
   const int r = blockIdx.x, tid = threadIdx.x;
   const RowPar par = row_par(a, r);
   const Range g = row_range(a, r);
@@ -563,7 +590,7 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
         __syncthreads();
         if (tid == 0) { sh.hi = 0ull; sh.lo = 0ull; }
         __syncthreads();
-        num.each([&](u64 x) { if (x >= thr_k) fixed_add(&sh.hi, &sh.lo, weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t)); });
+        num.each([&](u64 x) { if (x >= thr_k) fixed_add(&sh.hi, &sh.lo, weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp)); });
         __syncthreads();
         kept = fixed_d(sh.hi, sh.lo);
         const double target = par.p * (c.above_k + kept);
@@ -606,37 +633,56 @@ __device__ __forceinline__ DrawState row_state(const DrawArgs& a, int r) {
 }
 
 // ---------------------------------------------------------------- running sums of the kept weights
-__device__ __forceinline__ double kept_of(unsigned k, int i, const DrawState& st, const RowPar& par) {
+__device__ __forceinline__ double kept_of(unsigned k, int i, const DrawState& st, const RowPar& par, const ExpTable& e) {
   if (number_of(k, i) < st.thr) return 0.0;
-  const double w = weight_of(score_of(k), st.M, par.inv_t);
+  const double w = weight_of(score_of(k), st.M, par.inv_t, e);
   return w >= par.m ? w : 0.0;
 }
 
-// One workgroup to a chunk: four entries to a lane, four lanes to a block of 16.
+// One workgroup to a chunk: four entries to a lane, four lanes to a block of 16.  Leaves the running sums at the end of each
+// block and which of its entries are kept (16 bits): a draw then reads neither mask nor threshold.
 template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a) {
   __shared__ double blk[kTile / kBlock];
   __shared__ double wsum[4];
+  __shared__ ExpTable s_exp;
   const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  exp_table_init(s_exp);
   const RowView v = row_view<DT>(a, r);
   const DrawState st = row_state(a, r);
   const RowPar par = row_par(a, r);
+  __syncthreads();
   double carry = 0.0;
   const int per_chunk = a.chunk / kBlock;
-  double* out = a.block_incl + ((long long)r * a.n_chunks + blockIdx.x) * per_chunk;
+  const long long out0 = ((long long)r * a.n_chunks + blockIdx.x) * per_chunk;
   for (int t0 = 0; t0 < a.chunk; t0 += kTile) {
     const long long base = (long long)blockIdx.x * a.chunk + t0;
     if (base >= a.n_cols) break;                    // (uniform; nothing reads the sums behind the row's end)
-    for (int j = 0; j < kTile / 1024; ++j) {
-      const long long e = base + j * 1024 + tid * 4;
-      double w = 0.0;
-      if (e < a.n_cols) {
-        const Four<DT> f = load_four<DT>(v, (int)e, a.n_cols);
+    Four<DT> f[kTile / 1024];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) w += kept_of(four_key(f, q), (int)e + q, st, par);
+    for (int j = 0; j < kTile / 1024; ++j) {        // all of a thread's loads before any of its weights
+      const long long e = base + j * 1024 + tid * 4;
+      if (e < a.n_cols) f[j] = load_four<DT>(v, (int)e, a.n_cols);
+      else f[j].live = 0u;
+    }
+#pragma unroll
+    for (int j = 0; j < kTile / 1024; ++j) {
+      const int e = (int)(base + j * 1024 + tid * 4);
+      double w = 0.0;
+      unsigned bits = 0u;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const double x = kept_of(four_key(f[j], q), e + q, st, par, s_exp);
+        w += x;
+        bits |= (x > 0.0 ? 1u : 0u) << (4 * (lane & 3) + q);
       }
       w += __shfl_xor(w, 1);
       w += __shfl_xor(w, 2);
-      if ((tid & 3) == 0) blk[j * 64 + (tid >> 2)] = w;
+      bits |= (unsigned)__shfl_xor((int)bits, 1);
+      bits |= (unsigned)__shfl_xor((int)bits, 2);
+      if ((tid & 3) == 0) {
+        blk[j * 64 + (tid >> 2)] = w;
+        a.block_kept[out0 + t0 / kBlock + j * 64 + (tid >> 2)] = (unsigned short)bits;
+      }
     }
     __syncthreads();
     // inclusive sums over the tile's 256 blocks, one to a thread
@@ -647,76 +693,110 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
     double before = carry;
     for (int j = 0; j < (tid >> 6); ++j) before += wsum[j];
     s += before;
-    out[t0 / kBlock + tid] = s;
+    a.block_incl[out0 + t0 / kBlock + tid] = s;
     carry = ((((carry + wsum[0]) + wsum[1]) + wsum[2]) + wsum[3]);
     __syncthreads();
   }
   if (tid == 0) a.chunk_sum[(long long)r * a.n_chunks + blockIdx.x] = carry;
 }
 
-// ---------------------------------------------------------------- the draws: a thread to a draw
-template <int DT> __global__ __launch_bounds__(256) void k_draw_pick(DrawArgs a) {
-  __shared__ double incl[kMaxChunks];
-  __shared__ double wsum[4];
-  const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const long long d = (long long)blockIdx.x * 256 + tid;
+// ---------------------------------------------------------------- the draws
+// A workgroup holds its row's running sums at up to kCoarse places in LDS, so that a draw searches in LDS first, then among
+// the few blocks between two places, then in one block of 16 entries.  Bound: the scattered reads of the last two.  The
+// workgroups of a row run on one XCD (consecutive ones are dealt out to the eight in turn), whose L2 then holds the row.
+constexpr int kCoarse = 2048, kPickThreads = 512;
+template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(DrawArgs a) {
+  __shared__ double coarse[kCoarse];
+  __shared__ double chunk_incl[kMaxChunks];
+  __shared__ double wsum[kPickThreads / 64];
+  __shared__ ExpTable s_exp;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const unsigned total_wg = (unsigned)a.n_rows * (unsigned)a.pick_wgs, per_xcd = (total_wg + 7) / 8;
+  const unsigned work = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+  if (work >= total_wg) return;
+  const int r = (int)(work / (unsigned)a.pick_wgs);
+  const long long d0 = (long long)(work - (unsigned)r * (unsigned)a.pick_wgs) * a.pick_len;
+  const long long d1 = d0 + a.pick_len < a.n_draws ? d0 + a.pick_len : a.n_draws;
+  const long long out0 = (long long)r * a.n_draws;
+  exp_table_init(s_exp);
   const DrawState st = row_state(a, r);
   const int nc = a.n_chunks;
   if (!st.any) {
-    if (d < a.n_draws) { a.idx[(long long)r * a.n_draws + d] = -1; if (a.prob) a.prob[(long long)r * a.n_draws + d] = 0.f; }
+    for (long long d = d0 + tid; d < d1; d += kPickThreads) { a.idx[out0 + d] = -1; if (a.prob) a.prob[out0 + d] = 0.f; }
     return;
   }
-  // running sums over the row's chunks, four to a thread
-  double c[4], s = 0.0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) { const int k = 4 * tid + j; c[j] = k < nc ? a.chunk_sum[(long long)r * nc + k] : 0.0; s += c[j]; c[j] = s; }
-  double t = s;
+  // running sums over the row's chunks, two to a thread
+  double c0 = 2 * tid < nc ? a.chunk_sum[(long long)r * nc + 2 * tid] : 0.0;
+  double c1 = 2 * tid + 1 < nc ? a.chunk_sum[(long long)r * nc + 2 * tid + 1] : 0.0;
+  double t = c0 + c1;
   for (int o = 1; o < 64; o <<= 1) { const double x = shfl_up_d(t, o); if (lane >= o) t += x; }
   double before = __shfl_up(t, 1);
   if (lane == 0) before = 0.0;
   if (lane == 63) wsum[tid >> 6] = t;
   __syncthreads();
   for (int j = 0; j < (tid >> 6); ++j) before += wsum[j];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) incl[4 * tid + j] = before + c[j];
+  chunk_incl[2 * tid] = before + c0;
+  chunk_incl[2 * tid + 1] = before + c0 + c1;
   __syncthreads();
-  if (d >= a.n_draws) return;
-  const double total = incl[kMaxChunks - 1];
-  double u = (double)a.u[(long long)r * a.u_stride + d];
-  u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
-  const double target = u * total;
-  // first chunk whose running sum passes the target (the last one that adds anything, should rounding leave none)
-  int lo = 0, hi = nc - 1;
-  while (lo < hi) { const int mid = (lo + hi) >> 1; if (incl[mid] > target || incl[mid] >= total) hi = mid; else lo = mid + 1; }
-  const double in_chunk = target - (lo ? incl[lo - 1] : 0.0);
-  const int per_chunk = a.chunk / kBlock;
-  const double* bi = a.block_incl + ((long long)r * nc + lo) * per_chunk;
-  const long long first = (long long)lo * a.chunk;
-  const long long left = a.n_cols - first;
-  const int nb = (int)(((left < a.chunk ? left : a.chunk) + kBlock - 1) / kBlock);
-  const double chunk_total = a.chunk_sum[(long long)r * nc + lo];
-  int b0 = 0, b1 = nb - 1;
-  while (b0 < b1) { const int mid = (b0 + b1) >> 1; const double x = bi[mid]; if (x > in_chunk || x >= chunk_total) b1 = mid; else b0 = mid + 1; }
-  const double in_block = in_chunk - (b0 ? bi[b0 - 1] : 0.0);
+  const double total = chunk_incl[kMaxChunks - 1];
+  const int per_chunk = a.chunk / kBlock, step = a.coarse_blocks, per = per_chunk / step, n_coarse = nc * per;
+  const long long blocks0 = (long long)r * nc * per_chunk;
+  const int n_blocks = (int)(((long long)a.n_cols + kBlock - 1) / kBlock);
+  for (int j = tid; j < n_coarse; j += kPickThreads) {
+    const int ch = j / per;
+    // (the last chunk's sums end with the row's last tile: what lies behind holds the row's total)
+    const int end = (j + 1) * step - 1;
+    const double base = ch ? chunk_incl[ch - 1] : 0.0;
+    coarse[j] = (j + 1) % per == 0 || end >= n_blocks ? chunk_incl[ch] : base + a.block_incl[blocks0 + end];
+  }
+  __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const RowPar par = row_par(a, r);
-  const int i0 = (int)(first + (long long)b0 * kBlock);
-  double acc = 0.0, w_at = 0.0;
-  int at = -1;
-  for (int j = 0; j < kBlock; ++j) {
-    const int i = i0 + j;
-    if (i >= a.n_cols) break;
-    const double w = kept_of(entry_key<DT>(v, i), i, st, par);
-    if (w > 0.0) { at = i; w_at = w; }
-    acc += w;
-    if (acc > in_block && w > 0.0) break;
+  for (long long d = d0 + tid; d < d1; d += kPickThreads) {
+    double u = (double)a.u[(long long)r * a.u_stride + d];
+    u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
+    const double target = u * total;
+    // first place whose running sum passes the target (the first that reaches the total, should rounding leave none)
+    int lo = 0, hi = n_coarse - 1;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; const double x = coarse[mid]; if (x > target || x >= total) hi = mid; else lo = mid + 1; }
+    const int ch = lo / per;
+    const double chunk_before = ch ? chunk_incl[ch - 1] : 0.0;
+    const double* bi = a.block_incl + blocks0;
+    int b0 = lo * step, b1 = min(b0 + step, n_blocks) - 1;
+    const double in_chunk = target - chunk_before;
+    const double most = a.block_incl[blocks0 + b1];        // what the running sum is worth there
+    while (b0 < b1) { const int mid = (b0 + b1) >> 1; const double x = bi[mid]; if (x > in_chunk || x >= most) b1 = mid; else b0 = mid + 1; }
+    double in_block = in_chunk - (b0 % per_chunk ? bi[b0 - 1] : 0.0);
+    unsigned kept = a.block_kept[blocks0 + b0];
+    if (!kept) {
+      // the target lies within rounding of a border between places: the first kept entry behind it, or the last before
+      while (!kept && b0 + 1 < n_blocks) kept = a.block_kept[blocks0 + ++b0];
+      while (!kept && b0 > 0) kept = a.block_kept[blocks0 + --b0];
+      in_block = 0.0;
+    }
+    const int i0 = b0 * kBlock;
+    Four<DT> f[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = load_four<DT>(RowView{v.s, nullptr}, i0 + 4 * j, a.n_cols);
+    double acc = 0.0, w_at = 0.0;
+    int at = -1;
+    bool open = true;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      if (open && ((kept >> j) & 1u)) {
+        const double w = weight_of(f[j >> 2].s[j & 3], st.M, par.inv_t, s_exp);
+        at = i0 + j; w_at = w;
+        acc += w;
+        open = !(acc > in_block);
+      }
+    }
+    a.idx[out0 + d] = at;
+    if (a.prob) a.prob[out0 + d] = (float)(w_at / total);
   }
-  a.idx[(long long)r * a.n_draws + d] = at;
-  if (a.prob) a.prob[(long long)r * a.n_draws + d] = (float)(w_at / total);
 }
 
 // ---------------------------------------------------------------- host side
-struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, block_incl, part_max, part_min, bin_cnt, bin_mass, list_a, list_b, total; };
+struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, block_incl, block_kept, part_max, part_min, bin_cnt, bin_mass, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   DrawLayout l;
   // chunks of one tile; of more where a row would have over kMaxChunks of them
@@ -730,6 +810,7 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.cut = take(sizeof(DrawCut) * n_rows);
   l.chunk_sum = take(sizeof(double) * n_rows * l.n_chunks);
   l.block_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kBlock));
+  l.block_kept = take(sizeof(unsigned short) * n_rows * l.n_chunks * (l.chunk / kBlock));
   // Parts: about 1 024 workgroups over all rows, but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
   // row's, which costs what reading some thousand entries does).
   const long long cols = n_cols > 0 ? n_cols : 1;
@@ -758,7 +839,7 @@ template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(k_draw_cut<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
   }
   hipLaunchKernelGGL(k_draw_sums<DT>, dim3(a.n_chunks, a.n_rows), dim3(256), 0, s, a);
-  hipLaunchKernelGGL(k_draw_pick<DT>, dim3((unsigned)(((long long)a.n_draws + 255) / 256), a.n_rows), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(k_draw_pick<DT>, dim3((unsigned)(((long long)a.n_rows * a.pick_wgs + 7) / 8 * 8)), dim3(kPickThreads), 0, s, a);
 }
 
 }  // namespace psl
@@ -775,6 +856,7 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   if (q->dtype < PSL_F32 || q->dtype > PSL_F16) PSL_BAD("psl_draw_indices: unknown dtype %d", q->dtype);
   if (q->n_rows < 0 || q->n_rows > 65535 || q->n_cols < 0 || q->n_cols > 0x7f000000 || q->n_draws < 0)
     PSL_BAD("psl_draw_indices: %d rows (up to 65535) of %d entries, %d draws", q->n_rows, q->n_cols, q->n_draws);
+  if ((long long)q->n_rows * q->n_draws > (1ll << 38)) PSL_BAD("psl_draw_indices: %d x %d draws", q->n_rows, q->n_draws);
   if (q->n_rows == 0 || q->n_draws == 0) return PSL_OK;
   if ((!q->scores && q->n_cols) || !q->u || !q->idx || !q->ws) PSL_BAD("psl_draw_indices: missing pointer");
   const int es = q->dtype == PSL_F32 ? 4 : 2;
@@ -797,11 +879,19 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.u = q->u; a.u_stride = q->u_stride; a.idx = q->idx; a.prob = q->prob;
   char* w = (char*)q->ws;
   a.state = (DrawState*)(w + l.state); a.cut = (DrawCut*)(w + l.cut); a.chunk_sum = (double*)(w + l.chunk_sum); a.block_incl = (double*)(w + l.block_incl);
+  a.block_kept = (unsigned short*)(w + l.block_kept);
   a.n_chunks = l.n_chunks; a.chunk = l.chunk;
   a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
   a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass);
   a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
   a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
+  // Draws to a workgroup: its start costs a pass over kCoarse sums, so eight to a thread once every CU has work.
+  a.pick_len = kPickThreads;
+  while (a.pick_len < 8 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len > 2048) a.pick_len *= 2;
+  a.pick_wgs = (int)((a.n_draws + a.pick_len - 1) / a.pick_len);
+  // Places in LDS as close as kCoarse of them reach; few draws do not repay filling them and start from the chunks.
+  a.coarse_blocks = a.chunk / kBlock;
+  if (a.n_draws > 64) while (a.coarse_blocks % 2 == 0 && (long long)a.n_chunks * (a.chunk / kBlock) / (a.coarse_blocks / 2) <= kCoarse) a.coarse_blocks /= 2;
   hipStream_t s = (hipStream_t)stream;
   if (q->dtype == PSL_F32) launch_draw<PSL_F32>(a, s);
   else if (q->dtype == PSL_BF16) launch_draw<PSL_BF16>(a, s);

@@ -52,7 +52,7 @@ def _args(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=3), dict(dtype=-1), dict(n_rows=-1), dict(n_rows=65536), dict(n_cols=-1), dict(n_cols=0x7fffffff), dict(n_draws=-1),
+    dict(dtype=3), dict(dtype=-1), dict(n_rows=-1), dict(n_rows=65536), dict(n_cols=-1), dict(n_cols=0x7fffffff), dict(n_draws=-1), dict(n_rows=65535, n_draws=1 << 30),
     dict(scores=None), dict(u=None), dict(idx=None), dict(ws=None), dict(ws_bytes=16), dict(score_stride=-1), dict(u_stride=-1),
     dict(mask_stride=-1), dict(ws=264), dict(scores=258), dict(idx=258), dict(temperature=257), dict(top_k=258),
     dict(temperature_all=float("nan")), dict(top_p_all=float("nan")), dict(min_p_all=float("nan"))])
