@@ -27,7 +27,8 @@ struct DrawArgs {
   struct DrawState* state;     // [n_rows]
   struct DrawCut* cut;         // [n_rows]
   unsigned* part_max; unsigned* part_min;       // [n_rows][n_parts] keys
-  unsigned* bin_cnt; unsigned long long* bin_mass;       // [n_rows][kBins]; k_draw_bins leaves running sums (double) in bin_mass
+  unsigned* bin_cnt; unsigned long long* bin_mass;       // [n_rows][kBins]
+  double* bin_excl;            // [n_rows][kBins]: running sums in front of the bins; those behind them replace bin_mass
   unsigned long long* list_a; unsigned long long* list_b; int list_cap;      // [n_rows][list_cap] numbers of candidate entries
   double* chunk_sum;           // [n_rows][n_chunks]
   double* block_incl;          // [n_rows][n_chunks * chunk / 16]: running sums inside a chunk, at the end of each 16 entries
@@ -201,7 +202,7 @@ __device__ __forceinline__ bool has_cut(const RowPar& p) { return p.k > 0 || p.p
 // kBins of them over the row's range, at most kRange wide (what lies further weighs less than 2e-21 of the largest and is
 // in the last bin).  Rounding is monotone, so a bin is an interval of scores.  A bin's mass is a sum of integers, weights
 // scaled by 2^(q + the bin's own exponent): it has no order, and its rounding is 2^-q of the bin's own weights.
-struct Binning { double M, inv_t, c, oct; int q; };
+struct Binning { double M, inv_t, c, width, oct; int q; };
 __device__ __forceinline__ Binning make_binning(const Range& g, double inv_t, int n_cols) {
   Binning b;
   b.M = (double)score_of(g.mx); b.inv_t = inv_t;
@@ -209,45 +210,69 @@ __device__ __forceinline__ Binning make_binning(const Range& g, double inv_t, in
   if (!(range < kRange)) range = kRange;
   b.c = range > 0.0 ? (double)kBins / range : 0.0;
   if (!(b.c < 1e300)) b.c = 1e300;
-  b.oct = range > 0.0 ? range / (double)kBins * 1.4426950408889634 : 0.0;        // binary orders per bin
-  b.q = min(62 - (32 - __clz(n_cols)), 51);        // the row's sum below 2^63, an entry's below to_integer's limit
+  b.width = range / (double)kBins;
+  b.oct = b.width * 1.4426950408889634;             // binary orders per bin
+  b.q = min(62 - (32 - __clz(n_cols)), 51);         // the row's sum below 2^63, an entry's below to_integer's limit
   return b;
 }
-__device__ __forceinline__ int bin_of(const Binning& b, float s) {
-  const double x = (b.M - (double)s) * b.inv_t * b.c;
-  return (double)s == b.M ? 0 : x < (double)(kBins - 1) ? (int)x : kBins - 1;
+__device__ __forceinline__ double distance_of(const Binning& b, float s) { return (b.M - (double)s) * b.inv_t; }
+__device__ __forceinline__ int bin_at(const Binning& b, float s, double x) {
+  const double y = x * b.c;
+  return (double)s == b.M ? 0 : y < (double)(kBins - 1) ? (int)y : kBins - 1;
 }
+__device__ __forceinline__ int bin_of(const Binning& b, float s) { return bin_at(b, s, distance_of(b, s)); }
 __device__ __forceinline__ int bin_shift(const Binning& b, int bin) { return b.q + (int)((double)bin * b.oct); }
 
 // 0 <= x < 2^52 to the nearest integer: 2^52 + x has it in its low bits
 __device__ __forceinline__ u64 to_integer(double x) { return (u64)__double_as_longlong(x + 0x1p52) & 0xfffffffffffffull; }
 
+// An entry's scaled weight is its bin's first weight (a table) times e^-f, f < kRange / kBins = 0.047 behind the bin's begin:
+// the terms to the seventh leave 1e-15 of it.  Beyond kRange the last bin goes on and takes the long way.
 template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
   __shared__ unsigned cnt[kBins];
   __shared__ u64 mass[kBins];
-  __shared__ ExpTable s_exp;
+  __shared__ double first[kBins];
   const int r = blockIdx.y, tid = threadIdx.x;
   const RowPar par = row_par(a, r);
   if (!has_cut(par)) return;
-  exp_table_init(s_exp);
-  for (int j = tid; j < kBins; j += 512) { cnt[j] = 0u; mass[j] = 0ull; }
-  const Range g = row_range(a, r);        // (its barrier also covers the bins and the table)
+  const bool weigh = par.p < 1.0;
+  const Range g = row_range(a, r);
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
-  const float M = score_of(g.mx);
+  for (int j = tid; j < kBins; j += 512) {
+    cnt[j] = 0u; mass[j] = 0ull;
+    if (weigh) first[j] = ldexp(exp(-(double)j * b.width), bin_shift(b, j));
+  }
+  __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
-  const bool weigh = par.p < 1.0;
+#pragma unroll 2
   for (int i = i0 + tid * 4; i < i1; i += 2048) {
     const Four<DT> f = load_four<DT>(v, i, i1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const unsigned k = four_key(f, q);
-      if (k) {
-        const float s = score_of(k);
-        const int bin = bin_of(b, s);
+      const float s = f.s[q];
+      if (((f.live >> q) & 1u) && s > -__builtin_inff()) {
+        const double x = distance_of(b, s);
+        const int bin = bin_at(b, s, x);
         atomicAdd(&cnt[bin], 1u);
-        if (weigh) atomicAdd(&mass[bin], to_integer(ldexp(weight_of(s, M, par.inv_t, s_exp), bin_shift(b, bin))));
+        if (weigh) {
+          double y = fma(-(double)bin, b.width, x);
+          double w;
+          if (bin < kBins - 1 || y <= b.width) {
+            double p = fma(y, -1.0 / 5040.0, 1.0 / 720.0);
+            p = fma(y, p, -1.0 / 120.0);
+            p = fma(y, p, 1.0 / 24.0);
+            p = fma(y, p, -1.0 / 6.0);
+            p = fma(y, p, 0.5);
+            p = fma(y, p, -1.0);
+            p = fma(y, p, 1.0);
+            w = b.width > 0.0 && (double)s < b.M ? first[bin] * p : first[0];
+          } else {
+            w = first[kBins - 1] * exp(-fmin(y, 1100.0));
+          }
+          atomicAdd(&mass[bin], to_integer(w));
+        }
       }
     }
   }
@@ -260,84 +285,6 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   }
 }
 
-// Which bins the two limits fall into.  One wavefront; lane l holds bins 16 l .. 16 l + 15, the largest scores first.
-struct LaneBins { unsigned c[16]; double m[16]; unsigned c_before; double m_before; };
-__device__ __forceinline__ LaneBins load_bins(const DrawArgs& a, int r, const Binning& b) {
-  LaneBins w;
-  const int lane = threadIdx.x & 63;
-  unsigned cs = 0; double ms = 0.0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int bin = 16 * lane + j;
-    w.c[j] = a.bin_cnt[(long long)r * kBins + bin];
-    w.m[j] = ldexp((double)a.bin_mass[(long long)r * kBins + bin], -bin_shift(b, bin));
-    cs += w.c[j]; ms += w.m[j];
-  }
-  unsigned ci = cs; double mi = ms;
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned cu = __shfl_up(ci, o); const double mu = shfl_up_d(mi, o);
-    if (lane >= o) { ci += cu; mi += mu; }
-  }
-  w.c_before = ci - cs;
-  w.m_before = __shfl_up(mi, 1);
-  if (lane == 0) w.m_before = 0.0;
-  return w;
-}
-struct Found { int bin; unsigned before_n, count; double before, mass; };
-// first bin where the running count (mass) reaches `want`; entries of bins behind `last` do not count and `last` itself
-// weighs last_mass.  No such bin (rounding): the last one that holds something.
-__device__ __forceinline__ Found find_bin(const LaneBins& w, bool by_mass, unsigned want_n, double want_m, int last, double last_mass) {
-  const int lane = threadIdx.x & 63;
-  unsigned cb = w.c_before; double mb = w.m_before;
-  Found hit{-1, 0u, 0u, 0.0, 0.0}, tail{-1, 0u, 0u, 0.0, 0.0};
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int bin = 16 * lane + j;
-    const double m = bin == last ? last_mass : w.m[j];
-    if (w.c[j] && bin <= last) {
-      const Found here{bin, cb, w.c[j], mb, m};
-      tail = here;
-      if (hit.bin < 0 && (by_mass ? mb + m >= want_m : cb + w.c[j] >= want_n)) hit = here;
-    }
-    cb += w.c[j]; mb += m;
-  }
-  const u64 hits = __ballot(hit.bin >= 0), some = __ballot(tail.bin >= 0);
-  const int src = hits ? __ffsll((long long)hits) - 1 : some ? 63 - __clzll((long long)some) : 0;
-  const Found send = hits ? hit : tail;
-  Found f;
-  f.bin = __shfl(send.bin, src); f.before_n = __shfl(send.before_n, src); f.count = __shfl(send.count, src);
-  f.before = __shfl(send.before, src); f.mass = __shfl(send.mass, src);
-  return f;
-}
-__device__ __forceinline__ DrawCut make_cut(const LaneBins& w, const RowPar& par) {
-  DrawCut c;
-  unsigned cs = 0; double ms = 0.0;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) { cs += w.c[j]; ms += w.m[j]; }
-  c.n_valid = __shfl(w.c_before + cs, 63);
-  c.total = __shfl(w.m_before + ms, 63);
-  c.k_bin = kBins; c.want = 0u; c.above_k = c.total; c.n_a = 0u; c.n_b = 0u; c.p_lo = 0; c.p_hi = -1;
-  double most = c.total;
-  if (par.k > 0 && (unsigned)par.k < c.n_valid) {
-    const Found f = find_bin(w, false, (unsigned)par.k, 0.0, kBins - 1, __shfl(w.m[15], 63));
-    c.k_bin = f.bin; c.want = (unsigned)par.k - f.before_n; c.above_k = f.before; c.n_a = f.count;
-    most = f.before + f.mass;
-  }
-  if (par.p < 1.0 && par.k != 1) {
-    // top-k leaves a mass between above_k and `most`: the bins where its share can fall
-    const double last = __shfl(w.m[15], 63);
-    c.p_lo = find_bin(w, true, 0u, par.p * c.above_k, kBins - 1, last).bin;
-    c.p_hi = find_bin(w, true, 0u, par.p * most, kBins - 1, last).bin;
-    if (c.p_hi >= c.k_bin) c.p_hi = c.k_bin - 1;
-    unsigned n = 0;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) { const int bin = 16 * (threadIdx.x & 63) + j; if (bin >= c.p_lo && bin <= c.p_hi) n += w.c[j]; }
-    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
-    c.n_b = n;
-  }
-  return c;
-}
-
 // smallest key of the row whose bin is at most `bin` (bins fall as keys rise; the row's largest key is in bin 0)
 __device__ __forceinline__ unsigned first_key(const Binning& b, const Range& g, int bin) {
   unsigned lo = g.mn, hi = g.mx;
@@ -347,29 +294,75 @@ __device__ __forceinline__ unsigned first_key(const Binning& b, const Range& g, 
   }
   return lo;
 }
-// One wavefront to a row (in every workgroup of k_draw_gather instead, this cost each of them 8 us).
-__global__ __launch_bounds__(64) void k_draw_bins(DrawArgs a) {
-  const int r = blockIdx.x, lane = threadIdx.x;
+// smallest / largest thread of the workgroup for which a condition holds: a ballot per wavefront, then one LDS atomic each
+// (an atomic per thread to one address is run lane by lane)
+__device__ __forceinline__ void note_first(int* at, bool cond) {
+  const u64 m = __ballot(cond);
+  if (m && (threadIdx.x & 63) == 0) atomicMin(at, (int)(threadIdx.x & ~63u) + __ffsll((long long)m) - 1);
+}
+__device__ __forceinline__ void note_last(int* at, bool cond) {
+  const u64 m = __ballot(cond);
+  if (m && (threadIdx.x & 63) == 0) atomicMax(at, (int)(threadIdx.x & ~63u) + 63 - __clzll((long long)m));
+}
+// Which bins the two limits fall into: one workgroup to a row, a thread to a bin, the largest scores first.  (In every
+// workgroup of k_draw_gather instead, this cost each of them 8 us.)
+__global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
+  __shared__ unsigned s_cnt[kBins / 64], s_n_incl[kBins];
+  __shared__ double s_mass[kBins / 64], s_above_k, s_most;
+  __shared__ int s_k, s_lo, s_hi, s_last;
+  __shared__ unsigned s_want, s_na;
+  const int r = blockIdx.x, j = threadIdx.x, lane = j & 63, wave = j >> 6;
   const RowPar par = row_par(a, r);
   if (!has_cut(par)) return;
+  if (j == 0) { s_k = kBins; s_lo = kBins; s_hi = kBins; s_last = -1; s_want = 0u; s_na = 0u; }
   const Range g = row_range(a, r);
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
-  const LaneBins w = load_bins(a, r, b);
-  DrawCut c = make_cut(w, par);
-  double* cum = (double*)(a.bin_mass + (long long)r * kBins) + 16 * lane;
-  double m = w.m_before;
-#pragma unroll
-  for (int j = 0; j < 16; ++j) { m += w.m[j]; cum[j] = m; }
-  if (lane < 4) {
-    const int bin = lane == 0 ? c.k_bin : lane == 1 ? c.k_bin - 1 : lane == 2 ? c.p_hi : c.p_lo - 1;
-    const unsigned key = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
-    a.cut[r].key[lane] = key;
+  const unsigned c = a.bin_cnt[(long long)r * kBins + j];
+  const double m = ldexp((double)a.bin_mass[(long long)r * kBins + j], -bin_shift(b, j));
+  unsigned n_incl = c; double incl = m;
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned cu = __shfl_up(n_incl, o); const double mu = shfl_up_d(incl, o);
+    if (lane >= o) { n_incl += cu; incl += mu; }
   }
-  if (lane == 0) {
-    DrawCut* o = a.cut + r;
-    o->n_valid = c.n_valid; o->want = c.want; o->k_bin = c.k_bin; o->p_lo = c.p_lo; o->p_hi = c.p_hi; o->n_a = c.n_a; o->n_b = c.n_b;
-    o->above_k = c.above_k; o->total = c.total;
+  if (lane == 63) { s_cnt[wave] = n_incl; s_mass[wave] = incl; }
+  __syncthreads();
+  unsigned n_valid = 0u, n_before = 0u; double total = 0.0, before = 0.0;
+  for (int w = 0; w < kBins / 64; ++w) {
+    if (w == wave) { n_before = n_valid; before = total; }
+    n_valid += s_cnt[w]; total += s_mass[w];
+  }
+  // running sums in front of and behind this bin; only bins that hold something are ever chosen
+  const double up = __shfl_up(incl, 1), excl = lane ? before + up : before;
+  n_incl += n_before; incl += before;
+  s_n_incl[j] = n_incl;
+  ((double*)(a.bin_mass + (long long)r * kBins))[j] = c ? incl : -1.0;
+  a.bin_excl[(long long)r * kBins + j] = excl;
+  const bool cut_k = par.k > 0 && (unsigned)par.k < n_valid, cut_p = par.p < 1.0 && par.k != 1;
+  if (cut_k && n_incl >= (unsigned)par.k && n_incl - c < (unsigned)par.k) {
+    s_k = j; s_want = (unsigned)par.k - (n_incl - c); s_na = c; s_most = incl; s_above_k = excl;
+  }
+  __syncthreads();
+  const int k_bin = s_k;
+  const double above_k = cut_k ? s_above_k : total, most = cut_k ? s_most : total;
+  if (cut_p) {
+    // top-k leaves a mass between above_k and `most`: the bins before k_bin where its share can fall (none, by rounding: the last)
+    const bool held = c && j < k_bin;
+    note_last(&s_last, held);
+    note_first(&s_lo, held && incl >= par.p * above_k);
+    note_first(&s_hi, held && incl >= par.p * most);
+  }
+  __syncthreads();
+  const int p_lo = cut_p ? min(s_lo, s_last) : 0, p_hi = cut_p ? min(s_hi, s_last) : -1;
+  DrawCut* o = a.cut + r;
+  if (j < 4) {
+    const int bin = j == 0 ? k_bin : j == 1 ? k_bin - 1 : j == 2 ? p_hi : p_lo - 1;
+    o->key[j] = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
+  }
+  if (j == 64) {
+    o->n_valid = n_valid; o->want = s_want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = s_na;
+    o->n_b = p_hi >= 0 ? s_n_incl[p_hi] - (p_lo ? s_n_incl[p_lo - 1] : 0u) : 0u;
+    o->above_k = above_k; o->total = total;
   }
 }
 
@@ -427,11 +420,11 @@ struct RadixPick { int bin; unsigned above, count; double mass_above, mass; };
 struct RadixShared { RadixBins bins; RadixPick pick; u64 mx[16], mn[16]; u64 hi, lo; ExpTable exp; };
 
 __device__ __forceinline__ double fixed_d(u64 hi, u64 lo) { return (double)hi * 0x1p-32 + (double)lo * 0x1p-64; }
-__device__ __forceinline__ void fixed_add(u64* hi, u64* lo, double w) {
+struct Fixed { u64 hi, lo; };
+__device__ __forceinline__ Fixed to_fixed(double w) {
   const double x = w * 0x1p32;
   const u64 h = (u64)x;
-  atomicAdd(hi, h);
-  atomicAdd(lo, (u64)((x - (double)h) * 0x1p32));
+  return Fixed{h, (u64)((x - (double)h) * 0x1p32)};
 }
 
 // wavefront 0, all lanes: the first bin from the top where the running count (by_mass: mass) reaches `want`
@@ -528,7 +521,10 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
       if (hi == 64 || (x >> hi) == prefix) {
         const int d = (int)((x >> lo) & ((1u << (hi - lo)) - 1u));
         atomicAdd(&sh.bins.cnt[d], 1u);
-        if (mass_level) fixed_add(&sh.bins.hi[d], &sh.bins.lo[d], weight_of(score_of((unsigned)(x >> 32)), M, inv_t, sh.exp));
+        if (mass_level) {
+          const Fixed f = to_fixed(weight_of(score_of((unsigned)(x >> 32)), M, inv_t, sh.exp));
+          atomicAdd(&sh.bins.hi[d], f.hi); atomicAdd(&sh.bins.lo[d], f.lo);
+        }
       }
     });
     __syncthreads();
@@ -554,9 +550,43 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
   return mn;
 }
 
+// Up to 1 024 numbers, one to a thread, in descending order (zeros behind them): exchanges inside a wavefront through
+// shuffles, between wavefronts through LDS.
+constexpr int kSorted = 1024;
+__device__ __forceinline__ u64 block_sort(u64 x, int n, u64* lds) {
+  const int tid = threadIdx.x;
+  for (int k = 2; k < 2 * n && k <= kSorted; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      u64 y;
+      if (j >= 64) {
+        __syncthreads();
+        lds[tid] = x;
+        __syncthreads();
+        y = lds[tid ^ j];
+      } else y = __shfl_xor(x, j);
+      const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
+      x = (x > y) == larger ? x : y;
+    }
+  }
+  return x;
+}
+// sums of the sorted weights up to each thread's, in that order
+__device__ __forceinline__ double block_running(double w, double* lds16) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int o = 1; o < 64; o <<= 1) { const double t = shfl_up_d(w, o); if (lane >= o) w += t; }
+  __syncthreads();
+  if (lane == 63) lds16[wave] = w;
+  __syncthreads();
+  double before = 0.0;
+  for (int j = 0; j < wave; ++j) before += lds16[j];
+  return before + w;
+}
+
 template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
   __shared__ RadixShared sh;
-  __shared__ int s_bin;
+  __shared__ u64 s_sort[kSorted], s_thr;
+  __shared__ double s_wave[16], s_kept;
+  __shared__ int s_bin, s_at, s_end;
   const ExpTable& s_exp = sh.exp;
   exp_table_init(sh.exp);               // (row_range's barrier covers it)
   const int r = blockIdx.x, tid = threadIdx.x;
@@ -582,7 +612,29 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
     const bool cut_k = c.k_bin < kBins, cut_p = par.p < 1.0 && par.k != 1;
     double kept = 0.0;                              // mass of what top-k keeps of its bin
     bool p_in_a = false;
-    if (cut_k) {
+    if (cut_k && len_a <= kSorted) {
+      const u64 x = block_sort(tid < len_a ? src_a(tid) : 0ull, len_a, s_sort);
+      if (tid == 0) s_at = (int)c.want - 1;
+      if (tid == (int)c.want - 1) s_thr = x;
+      double incl = 0.0;
+      if (cut_p) {
+        incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp) : 0.0, s_wave);
+        if (tid == (int)c.want - 1) s_kept = incl;
+      }
+      __syncthreads();
+      if (cut_p) {
+        kept = s_kept;
+        const double target = par.p * (c.above_k + kept);
+        p_in_a = target > c.above_k;
+        if (p_in_a) {
+          note_first(&s_at, incl >= target - c.above_k);
+          __syncthreads();
+          if (tid == s_at) s_thr = x;
+          __syncthreads();
+        }
+      }
+      thr = s_thr;
+    } else if (cut_k) {
       const Numbers<decltype(src_a)> num(src_a, len_a);
       const u64 thr_k = radix_select(num, false, c.want, 0.0, M, par.inv_t, sh);
       thr = thr_k;
@@ -590,20 +642,23 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
         __syncthreads();
         if (tid == 0) { sh.hi = 0ull; sh.lo = 0ull; }
         __syncthreads();
-        num.each([&](u64 x) { if (x >= thr_k) fixed_add(&sh.hi, &sh.lo, weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp)); });
+        u64 hi = 0ull, lo = 0ull;
+        num.each([&](u64 x) { if (x >= thr_k) { const Fixed f = to_fixed(weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp)); hi += f.hi; lo += f.lo; } });
+        for (int o = 32; o > 0; o >>= 1) { hi += __shfl_xor(hi, o); lo += __shfl_xor(lo, o); }
+        if ((tid & 63) == 0) { atomicAdd(&sh.hi, hi); atomicAdd(&sh.lo, lo); }
         __syncthreads();
         kept = fixed_d(sh.hi, sh.lo);
         const double target = par.p * (c.above_k + kept);
-        p_in_a = target > c.above_k;                // (the running sums before k_bin end at above_k)
+        p_in_a = target > c.above_k;
         if (p_in_a) {
           auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
           thr = radix_select(Numbers<decltype(src)>(src, len_a), true, 0u, target - c.above_k, M, par.inv_t, sh);
         }
       }
     }
-    if (cut_p && !p_in_a && c.p_hi >= c.p_lo) {
+    if (cut_p && !p_in_a && c.p_hi >= 0) {
       const double target = par.p * (cut_k ? c.above_k + kept : c.total);
-      // first bin of [p_lo, p_hi] whose running sum reaches the target
+      // first bin of [p_lo, p_hi] whose running sum reaches the target (empty ones hold -1; p_hi is not empty)
       if (tid == 0) s_bin = c.p_hi;
       __syncthreads();
       for (int j = c.p_lo + tid; j < c.p_hi; j += 1024) if (cum[j] >= target) atomicMin(&s_bin, j);
@@ -617,8 +672,22 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
         else { const unsigned k = entry_key<DT>(v, i); if (k >= b0 && k < b1) x = number_of(k, i); }
         return x && bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
       };
-      const double before = bin ? cum[bin - 1] : 0.0;
-      const u64 t = radix_select(Numbers<decltype(src)>(src, listed_b ? (int)c.n_b : a.n_cols), true, 0u, target - before, M, par.inv_t, sh);
+      const double before = a.bin_excl[(long long)r * kBins + bin];
+      const int len_b = listed_b ? (int)c.n_b : a.n_cols;
+      u64 t;
+      if (len_b <= kSorted) {
+        const u64 x = block_sort(tid < len_b ? src(tid) : 0ull, len_b, s_sort);
+        const double incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp) : 0.0, s_wave);
+        // (none reaches it, by rounding: the last one)
+        if (tid == 0) { s_at = kSorted; s_end = 0; }
+        __syncthreads();
+        note_first(&s_at, x && incl >= target - before);
+        note_last(&s_end, x != 0ull);
+        __syncthreads();
+        if (tid == min(s_at, s_end)) s_thr = x;
+        __syncthreads();
+        t = s_thr;
+      } else t = radix_select(Numbers<decltype(src)>(src, len_b), true, 0u, target - before, M, par.inv_t, sh);
       if (t > thr) thr = t;                         // (an empty source gives 0)
     }
   }
@@ -796,7 +865,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(Dr
 }
 
 // ---------------------------------------------------------------- host side
-struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, block_incl, block_kept, part_max, part_min, bin_cnt, bin_mass, list_a, list_b, total; };
+struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, block_incl, block_kept, part_max, part_min, bin_cnt, bin_mass, bin_excl, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   DrawLayout l;
   // chunks of one tile; of more where a row would have over kMaxChunks of them
@@ -825,6 +894,7 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.part_min = take(sizeof(unsigned) * n_rows * l.n_parts);
   l.bin_cnt = take(sizeof(unsigned) * n_rows * kBins);
   l.bin_mass = take(sizeof(u64) * n_rows * kBins);
+  l.bin_excl = take(sizeof(double) * n_rows * kBins);
   l.list_a = take(sizeof(u64) * n_rows * l.list_cap);
   l.list_b = take(sizeof(u64) * n_rows * l.list_cap);
   l.total = o;
@@ -834,7 +904,7 @@ template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(k_draw_range<DT>, dim3(a.n_parts, a.n_rows), dim3(256), 0, s, a);
   if (a.cuts) {
     hipLaunchKernelGGL(k_draw_hist<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
-    hipLaunchKernelGGL(k_draw_bins, dim3(a.n_rows), dim3(64), 0, s, a);
+    hipLaunchKernelGGL(k_draw_bins, dim3(a.n_rows), dim3(kBins), 0, s, a);
     hipLaunchKernelGGL(k_draw_gather<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
     hipLaunchKernelGGL(k_draw_cut<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
   }
@@ -882,7 +952,7 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.block_kept = (unsigned short*)(w + l.block_kept);
   a.n_chunks = l.n_chunks; a.chunk = l.chunk;
   a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
-  a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass);
+  a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
   a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
   a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
   // Draws to a workgroup: its start costs a pass over kCoarse sums, so eight to a thread once every CU has work.
