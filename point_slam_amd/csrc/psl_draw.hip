@@ -43,9 +43,9 @@ struct DrawState {
 };
 
 struct DrawCut {
-  unsigned n_valid, want;          // want: entries of k_bin that top-k keeps
+  unsigned want;                   // entries of k_bin that top-k keeps
   int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
-  unsigned n_a, n_b;               // entries of k_bin; of [p_lo, p_hi]
+  unsigned n_a;                    // entries of k_bin
   unsigned key[4];                 // keys of k_bin: [0] .. [1] - 1; of [p_lo, p_hi]: [2] .. [3] - 1
   double above_k, total;           // mass of the bins before k_bin; of all
 };
@@ -93,7 +93,7 @@ __device__ __forceinline__ RowPar row_par(const DrawArgs& a, int r) {
   q.m = q.m > 1.0 ? 1.0 : q.m;
   // no temperature, or nothing but the first entry asked for: the first of the order, whatever the weights
   if (!(t > 0.0) || q.p <= 0.0) q.k = 1;
-  q.inv_t = t > 0.0 ? 1.0 / t : 1.0;
+  q.inv_t = t > 0.0 ? fmin(1.0 / t, 1e300) : 1.0;       // (finite: no difference times it stays 0)
   return q;
 }
 // exp(-x) for x >= 0 to about one unit of the last place, in 14 fp64 instructions and one LDS read (the library's takes about
@@ -117,8 +117,8 @@ __device__ __forceinline__ double exp_neg(double x, const ExpTable& e) {
 }
 // weight of an allowed score; +inf among the scores takes all
 __device__ __forceinline__ double weight_of(float s, float M, double inv_t, const ExpTable& e) {
-  const double w = exp_neg(((double)M - (double)s) * inv_t, e);
-  return s == M ? 1.0 : M == __builtin_inff() ? 0.0 : w;
+  if (M == __builtin_inff()) return s == M ? 1.0 : 0.0;
+  return exp_neg(((double)M - (double)s) * inv_t, e);
 }
 
 __device__ __forceinline__ double shfl_up_d(double v, int o) { return __shfl_up(v, o); }
@@ -198,54 +198,66 @@ __device__ __forceinline__ Range row_range(const DrawArgs& a, int r) {
 }
 __device__ __forceinline__ bool has_cut(const RowPar& p) { return p.k > 0 || p.p < 1.0; }
 
-// ---------------------------------------------------------------- bins of equal width in (M - s) / T
-// kBins of them over the row's range, at most kRange wide (what lies further weighs less than 2e-21 of the largest and is
-// in the last bin).  Rounding is monotone, so a bin is an interval of scores.  A bin's mass is a sum of integers, weights
-// scaled by 2^(q + the bin's own exponent): it has no order, and its rounding is 2^-q of the bin's own weights.
-struct Binning { double M, inv_t, c, width, oct; int q; };
+// ---------------------------------------------------------------- bins of equal width in M - s
+// kBins of them over the row's range, at most kRange temperatures wide; the last one goes on beyond that.  fp32 decides the
+// bin: a difference, a product and a truncation never fall as the score falls, so a bin is an interval of scores, and that is
+// all it has to be.  A bin's mass is a sum of integers, weights scaled by 2^(q + the bin's own exponent): it has no order, and its
+// rounding is 2^-q of the bin's own weights.
+struct Binning { float M, scale; double inv_t, width, oct; int q; };
 __device__ __forceinline__ Binning make_binning(const Range& g, double inv_t, int n_cols) {
   Binning b;
-  b.M = (double)score_of(g.mx); b.inv_t = inv_t;
-  double range = (b.M - (double)score_of(g.mn)) * inv_t;
+  b.M = score_of(g.mx); b.inv_t = inv_t;
+  double range = ((double)b.M - (double)score_of(g.mn)) * inv_t;
   if (!(range < kRange)) range = kRange;
-  b.c = range > 0.0 ? (double)kBins / range : 0.0;
-  if (!(b.c < 1e300)) b.c = 1e300;
-  b.width = range / (double)kBins;
+  // An infinite largest score: it in the first bin, everything else in the last, which weighs nothing (k_draw_hist).
+  const bool inf_row = b.M == __builtin_inff();
+  b.width = inf_row ? 0.0 : range / (double)kBins;              // in temperatures
+  b.scale = inf_row ? 1.f : (float)(inv_t / b.width);           // bins per unit of score (inf: no other score than M)
   b.oct = b.width * 1.4426950408889634;             // binary orders per bin
   b.q = min(62 - (32 - __clz(n_cols)), 51);         // the row's sum below 2^63, an entry's below to_integer's limit
   return b;
 }
-__device__ __forceinline__ double distance_of(const Binning& b, float s) { return (b.M - (double)s) * b.inv_t; }
-__device__ __forceinline__ int bin_at(const Binning& b, float s, double x) {
-  const double y = x * b.c;
-  return (double)s == b.M ? 0 : y < (double)(kBins - 1) ? (int)y : kBins - 1;
+__device__ __forceinline__ int bin_of(const Binning& b, float s) {
+  // (NaN, from inf - inf or 0 * inf, converts to 0: the largest score's bin)
+  return (int)min(__float2uint_rz((b.M - s) * b.scale), (unsigned)(kBins - 1));
 }
-__device__ __forceinline__ int bin_of(const Binning& b, float s) { return bin_at(b, s, distance_of(b, s)); }
 __device__ __forceinline__ int bin_shift(const Binning& b, int bin) { return b.q + (int)((double)bin * b.oct); }
 
 // 0 <= x < 2^52 to the nearest integer: 2^52 + x has it in its low bits
 __device__ __forceinline__ u64 to_integer(double x) { return (u64)__double_as_longlong(x + 0x1p52) & 0xfffffffffffffull; }
 
 // An entry's scaled weight is its bin's first weight (a table) times e^-f, f < kRange / kBins = 0.047 behind the bin's begin:
-// the terms to the seventh leave 1e-15 of it.  Beyond kRange the last bin goes on and takes the long way.
+// the terms to the seventh leave 1e-15 of it.  What lies beyond kRange counts as lying at the last bin's end: 1e-21 of the
+// largest weight, a million of which do not reach the sum's rounding.  Bound: instructions (65 per entry made this 25 us for
+// twelve rows of 816 000), then the LDS atomics: entries are counted only where top-k asks and weighed only where top-p
+// does, and neighbouring lanes use different copies.
+constexpr int kCopies = 2;
 template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
-  __shared__ unsigned cnt[kBins];
-  __shared__ u64 mass[kBins];
+  __shared__ unsigned cnt[kCopies][kBins];
+  __shared__ u64 mass[kCopies][kBins];
   __shared__ double first[kBins];
   const int r = blockIdx.y, tid = threadIdx.x;
   const RowPar par = row_par(a, r);
   if (!has_cut(par)) return;
-  const bool weigh = par.p < 1.0;
+  const bool weigh = par.p < 1.0, count = par.k > 0;
   const Range g = row_range(a, r);
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
+  const bool inf_row = b.M == __builtin_inff();
   for (int j = tid; j < kBins; j += 512) {
-    cnt[j] = 0u; mass[j] = 0ull;
-    if (weigh) first[j] = ldexp(exp(-(double)j * b.width), bin_shift(b, j));
+#pragma unroll
+    for (int q = 0; q < kCopies; ++q) { cnt[q][j] = 0u; mass[q][j] = 0ull; }
+    if (weigh) first[j] = inf_row && j ? 0.0 : ldexp(exp(-(double)j * b.width), bin_shift(b, j));
   }
   __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
+  unsigned* const my_cnt = cnt[tid & (kCopies - 1)];
+  u64* const my_mass = mass[tid & (kCopies - 1)];
+  const double M = (double)b.M;
+  // the coefficients stay in registers (the compiler would write them anew for every entry: they are not inline constants)
+  double c7 = -1.0 / 5040.0, c6 = 1.0 / 720.0, c5 = -1.0 / 120.0, c4 = 1.0 / 24.0, c3 = -1.0 / 6.0;
+  asm("" : "+v"(c7), "+v"(c6), "+v"(c5), "+v"(c4), "+v"(c3));
 #pragma unroll 2
   for (int i = i0 + tid * 4; i < i1; i += 2048) {
     const Four<DT> f = load_four<DT>(v, i, i1);
@@ -253,35 +265,29 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
     for (int q = 0; q < 4; ++q) {
       const float s = f.s[q];
       if (((f.live >> q) & 1u) && s > -__builtin_inff()) {
-        const double x = distance_of(b, s);
-        const int bin = bin_at(b, s, x);
-        atomicAdd(&cnt[bin], 1u);
+        const int bin = bin_of(b, s);
+        if (count) atomicAdd(&my_cnt[bin], 1u);
         if (weigh) {
-          double y = fma(-(double)bin, b.width, x);
-          double w;
-          if (bin < kBins - 1 || y <= b.width) {
-            double p = fma(y, -1.0 / 5040.0, 1.0 / 720.0);
-            p = fma(y, p, -1.0 / 120.0);
-            p = fma(y, p, 1.0 / 24.0);
-            p = fma(y, p, -1.0 / 6.0);
-            p = fma(y, p, 0.5);
-            p = fma(y, p, -1.0);
-            p = fma(y, p, 1.0);
-            w = b.width > 0.0 && (double)s < b.M ? first[bin] * p : first[0];
-          } else {
-            w = first[kBins - 1] * exp(-fmin(y, 1100.0));
-          }
-          atomicAdd(&mass[bin], to_integer(w));
+          const double y = fmin(fma((double)bin, -b.width, (M - (double)s) * b.inv_t), b.width);      // (a NaN gives the width)
+          double p = fma(y, c7, c6);
+          p = fma(y, p, c5);
+          p = fma(y, p, c4);
+          p = fma(y, p, c3);
+          p = fma(y, p, 0.5);
+          p = fma(y, p, -1.0);
+          p = fma(y, p, 1.0);
+          atomicAdd(&my_mass[bin], to_integer(first[bin] * p));
         }
       }
     }
   }
   __syncthreads();
   for (int j = tid; j < kBins; j += 512) {
-    if (cnt[j]) {
-      atomicAdd(&a.bin_cnt[(long long)r * kBins + j], cnt[j]);
-      if (weigh) atomicAdd(&a.bin_mass[(long long)r * kBins + j], mass[j]);
-    }
+    unsigned c = 0u; u64 m = 0ull;
+#pragma unroll
+    for (int q = 0; q < kCopies; ++q) { c += cnt[q][j]; m += mass[q][j]; }
+    if (c) atomicAdd(&a.bin_cnt[(long long)r * kBins + j], c);
+    if (m) atomicAdd(&a.bin_mass[(long long)r * kBins + j], m);
   }
 }
 
@@ -294,6 +300,7 @@ __device__ __forceinline__ unsigned first_key(const Binning& b, const Range& g, 
   }
   return lo;
 }
+
 // smallest / largest thread of the workgroup for which a condition holds: a ballot per wavefront, then one LDS atomic each
 // (an atomic per thread to one address is run lane by lane)
 __device__ __forceinline__ void note_first(int* at, bool cond) {
@@ -307,7 +314,7 @@ __device__ __forceinline__ void note_last(int* at, bool cond) {
 // Which bins the two limits fall into: one workgroup to a row, a thread to a bin, the largest scores first.  (In every
 // workgroup of k_draw_gather instead, this cost each of them 8 us.)
 __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
-  __shared__ unsigned s_cnt[kBins / 64], s_n_incl[kBins];
+  __shared__ unsigned s_cnt[kBins / 64];
   __shared__ double s_mass[kBins / 64], s_above_k, s_most;
   __shared__ int s_k, s_lo, s_hi, s_last;
   __shared__ unsigned s_want, s_na;
@@ -335,8 +342,7 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
   // running sums in front of and behind this bin; only bins that hold something are ever chosen
   const double up = __shfl_up(incl, 1), excl = lane ? before + up : before;
   n_incl += n_before; incl += before;
-  s_n_incl[j] = n_incl;
-  ((double*)(a.bin_mass + (long long)r * kBins))[j] = c ? incl : -1.0;
+  ((double*)(a.bin_mass + (long long)r * kBins))[j] = m > 0.0 ? incl : -1.0;
   a.bin_excl[(long long)r * kBins + j] = excl;
   const bool cut_k = par.k > 0 && (unsigned)par.k < n_valid, cut_p = par.p < 1.0 && par.k != 1;
   if (cut_k && n_incl >= (unsigned)par.k && n_incl - c < (unsigned)par.k) {
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
   const double above_k = cut_k ? s_above_k : total, most = cut_k ? s_most : total;
   if (cut_p) {
     // top-k leaves a mass between above_k and `most`: the bins before k_bin where its share can fall (none, by rounding: the last)
-    const bool held = c && j < k_bin;
+    const bool held = m > 0.0 && j < k_bin;
     note_last(&s_last, held);
     note_first(&s_lo, held && incl >= par.p * above_k);
     note_first(&s_hi, held && incl >= par.p * most);
@@ -360,8 +366,7 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
     o->key[j] = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
   }
   if (j == 64) {
-    o->n_valid = n_valid; o->want = s_want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = s_na;
-    o->n_b = p_hi >= 0 ? s_n_incl[p_hi] - (p_lo ? s_n_incl[p_lo - 1] : 0u) : 0u;
+    o->want = s_want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = s_na;
     o->above_k = above_k; o->total = total;
   }
 }
@@ -372,10 +377,10 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
 // 816 000); what does not fit there goes to the list by itself.
 constexpr int kListBuf = 1024;
 struct ListBuf { u64 e[kListBuf]; unsigned n, at; };
-__device__ __forceinline__ void list_add(ListBuf& b, u64 x, u64* dst, unsigned* fill) {
+__device__ __forceinline__ void list_add(ListBuf& b, u64 x, u64* dst, unsigned* fill, unsigned cap) {
   const unsigned j = atomicAdd(&b.n, 1u);
   if (j < kListBuf) b.e[j] = x;
-  else dst[atomicAdd(fill, 1u)] = x;
+  else { const unsigned at = atomicAdd(fill, 1u); if (at < cap) dst[at] = x; }
 }
 template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs a) {
   __shared__ ListBuf buf_a, buf_b;
@@ -386,7 +391,7 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
   const Range g = row_range(a, r);
   if (!g.mx) return;
   const DrawCut& c = a.cut[r];
-  const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.n_b && c.n_b <= (unsigned)a.list_cap;
+  const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.p_hi >= 0;
   if (!do_a && !do_b) return;
   // (no such bin: an empty interval)
   const unsigned a0 = do_a ? c.key[0] : 1u, a1 = do_a ? c.key[1] : 0u, b0 = do_b ? c.key[2] : 1u, b1 = do_b ? c.key[3] : 0u;
@@ -394,14 +399,15 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
   u64* la = a.list_a + (long long)r * a.list_cap;
   u64* lb = a.list_b + (long long)r * a.list_cap;
+  const unsigned cap = (unsigned)a.list_cap;
 #pragma unroll 2
   for (int i = i0 + tid * 4; i < i1; i += 2048) {
     const Four<DT> f = load_four<DT>(v, i, i1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const unsigned k = four_key(f, q);
-      if (k >= a0 && k < a1) list_add(buf_a, number_of(k, i + q), la, &a.state[r].n_a);
-      if (k >= b0 && k < b1) list_add(buf_b, number_of(k, i + q), lb, &a.state[r].n_b);
+      if (k >= a0 && k < a1) list_add(buf_a, number_of(k, i + q), la, &a.state[r].n_a, cap);
+      if (k >= b0 && k < b1) list_add(buf_b, number_of(k, i + q), lb, &a.state[r].n_b, cap);
     }
   }
   __syncthreads();
@@ -409,8 +415,8 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
   if (tid == 0 && na) buf_a.at = atomicAdd(&a.state[r].n_a, na);
   if (tid == 64 && nb) buf_b.at = atomicAdd(&a.state[r].n_b, nb);
   __syncthreads();
-  for (unsigned j = tid; j < na; j += 512) la[buf_a.at + j] = buf_a.e[j];
-  for (unsigned j = tid; j < nb; j += 512) lb[buf_b.at + j] = buf_b.e[j];
+  for (unsigned j = tid; j < na; j += 512) if (buf_a.at + j < cap) la[buf_a.at + j] = buf_a.e[j];
+  for (unsigned j = tid; j < nb; j += 512) if (buf_b.at + j < cap) lb[buf_b.at + j] = buf_b.e[j];
 }
 
 // ---------------------------------------------------------------- the threshold among those entries, by radix selection
@@ -600,8 +606,9 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
     const u64* lb = a.list_b + (long long)r * a.list_cap;
     const double* cum = (const double*)(a.bin_mass + (long long)r * kBins);
     const DrawCut& c = a.cut[r];
-    const bool listed_a = c.n_a <= (unsigned)a.list_cap, listed_b = c.n_b <= (unsigned)a.list_cap;
-    // a list that was too long to be written: the row itself, entry by entry
+    const unsigned n_b = a.state[r].n_b;
+    const bool listed_a = c.n_a <= (unsigned)a.list_cap, listed_b = n_b <= (unsigned)a.list_cap;
+    // a list that its entries do not fit into: the row itself, entry by entry
     const unsigned a0 = c.key[0], a1 = c.key[1];
     auto src_a = [&](int i) -> u64 {
       if (listed_a) return la[i];
@@ -673,7 +680,7 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
         return x && bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
       };
       const double before = a.bin_excl[(long long)r * kBins + bin];
-      const int len_b = listed_b ? (int)c.n_b : a.n_cols;
+      const int len_b = listed_b ? (int)n_b : a.n_cols;
       u64 t;
       if (len_b <= kSorted) {
         const u64 x = block_sort(tid < len_b ? src(tid) : 0ull, len_b, s_sort);
@@ -702,11 +709,14 @@ __device__ __forceinline__ DrawState row_state(const DrawArgs& a, int r) {
 }
 
 // ---------------------------------------------------------------- running sums of the kept weights
-__device__ __forceinline__ double kept_of(unsigned k, int i, const DrawState& st, const RowPar& par, const ExpTable& e) {
-  if (number_of(k, i) < st.thr) return 0.0;
-  const double w = weight_of(score_of(k), st.M, par.inv_t, e);
-  return w >= par.m ? w : 0.0;
+// An entry is kept iff its number is at least the threshold, which in scores is: above thr_s, or thr_s itself at an index up to
+// thr_i.  (No limit: every score above -inf.)
+struct Kept { float thr_s; int thr_i; };
+__device__ __forceinline__ Kept kept_from(u64 thr) {
+  const unsigned key = (unsigned)(thr >> 32);
+  return key <= 1u ? Kept{-__builtin_inff(), -1} : Kept{score_of(key), (int)~(unsigned)thr};
 }
+__device__ __forceinline__ bool is_kept(float s, int i, const Kept& k) { return s > k.thr_s || (s == k.thr_s && i <= k.thr_i); }
 
 // One workgroup to a chunk: four entries to a lane, four lanes to a block of 16.  Leaves the running sums at the end of each
 // block and which of its entries are kept (16 bits): a draw then reads neither mask nor threshold.
@@ -719,6 +729,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
   const RowView v = row_view<DT>(a, r);
   const DrawState st = row_state(a, r);
   const RowPar par = row_par(a, r);
+  const Kept kp = kept_from(st.thr);
   __syncthreads();
   double carry = 0.0;
   const int per_chunk = a.chunk / kBlock;
@@ -740,10 +751,12 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
       unsigned bits = 0u;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const double x = kept_of(four_key(f[j], q), e + q, st, par, s_exp);
-        w += x;
-        bits |= (x > 0.0 ? 1u : 0u) << (4 * (lane & 3) + q);
+        if (((f[j].live >> q) & 1u) && is_kept(f[j].s[q], e + q, kp)) {
+          const double x = weight_of(f[j].s[q], st.M, par.inv_t, s_exp);
+          if (x > 0.0 && x >= par.m) { w += x; bits |= 1u << q; }
+        }
       }
+      bits <<= 4 * (lane & 3);
       w += __shfl_xor(w, 1);
       w += __shfl_xor(w, 2);
       bits |= (unsigned)__shfl_xor((int)bits, 1);
@@ -811,7 +824,10 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(Dr
   const int per_chunk = a.chunk / kBlock, step = a.coarse_blocks, per = per_chunk / step, n_coarse = nc * per;
   const long long blocks0 = (long long)r * nc * per_chunk;
   const int n_blocks = (int)(((long long)a.n_cols + kBlock - 1) / kBlock);
-  for (int j = tid; j < n_coarse; j += kPickThreads) {
+  int coarse_top = 1;
+  while (2 * coarse_top < n_coarse) coarse_top <<= 1;        // the search below ends at 2 coarse_top - 1, up to kCoarse - 1
+  for (int j = tid; j < 2 * coarse_top; j += kPickThreads) {
+    if (j >= n_coarse) { coarse[j] = __builtin_inf(); continue; }
     const int ch = j / per;
     // (the last chunk's sums end with the row's last tile: what lies behind holds the row's total)
     const int end = (j + 1) * step - 1;
@@ -821,46 +837,69 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(Dr
   __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const RowPar par = row_par(a, r);
+  const float per_octave = (float)(par.inv_t * 1.4426950408889634);
   for (long long d = d0 + tid; d < d1; d += kPickThreads) {
     double u = (double)a.u[(long long)r * a.u_stride + d];
     u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
-    const double target = u * total;
-    // first place whose running sum passes the target (the first that reaches the total, should rounding leave none)
-    int lo = 0, hi = n_coarse - 1;
-    while (lo < hi) { const int mid = (lo + hi) >> 1; const double x = coarse[mid]; if (x > target || x >= total) hi = mid; else lo = mid + 1; }
+    const double target = u * total;                 // below the total: the last place passes it
+    int lo = 0;
+    for (int k = coarse_top; k > 0; k >>= 1) { if (coarse[lo + k - 1] <= target) lo += k; }      // first place that passes the target
     const int ch = lo / per;
-    const double chunk_before = ch ? chunk_incl[ch - 1] : 0.0;
+    const double in_chunk = target - (ch ? chunk_incl[ch - 1] : 0.0);
     const double* bi = a.block_incl + blocks0;
     int b0 = lo * step, b1 = min(b0 + step, n_blocks) - 1;
-    const double in_chunk = target - chunk_before;
-    const double most = a.block_incl[blocks0 + b1];        // what the running sum is worth there
-    while (b0 < b1) { const int mid = (b0 + b1) >> 1; const double x = bi[mid]; if (x > in_chunk || x >= most) b1 = mid; else b0 = mid + 1; }
-    double in_block = in_chunk - (b0 % per_chunk ? bi[b0 - 1] : 0.0);
+    while (b0 < b1) { const int mid = (b0 + b1) >> 1; if (bi[mid] > in_chunk) b1 = mid; else b0 = mid + 1; }
+    const double front = b0 % per_chunk ? bi[b0 - 1] : 0.0;
+    double in_block = in_chunk - front;
+    const double mass = bi[b0] - front;
     unsigned kept = a.block_kept[blocks0 + b0];
     if (!kept) {
       // the target lies within rounding of a border between places: the first kept entry behind it, or the last before
       while (!kept && b0 + 1 < n_blocks) kept = a.block_kept[blocks0 + ++b0];
       while (!kept && b0 > 0) kept = a.block_kept[blocks0 + --b0];
-      in_block = 0.0;
+      in_block = -1.0;
     }
     const int i0 = b0 * kBlock;
     Four<DT> f[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = load_four<DT>(RowView{v.s, nullptr}, i0 + 4 * j, a.n_cols);
-    double acc = 0.0, w_at = 0.0;
-    int at = -1;
-    bool open = true;
+    // In fp32 first, weights relative to the block's largest: 16 exponentials of at most one unit of the last place and 15 sums
+    // are within 35 * 2^-24 of the block's mass (x 2^-x <= 0.53 bounds what the rounded exponent does), so a border that
+    // is 2^-18 of it away is on the side it seems to be on.  One draw in ten thousand is not that clear.
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) if ((kept >> j) & 1u) top = fmaxf(top, f[j >> 2].s[j & 3]);
+    float run[16], sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      if (open && ((kept >> j) & 1u)) {
-        const double w = weight_of(f[j >> 2].s[j & 3], st.M, par.inv_t, s_exp);
-        at = i0 + j; w_at = w;
-        acc += w;
-        open = !(acc > in_block);
+      const float w = __builtin_amdgcn_exp2f((f[j >> 2].s[j & 3] - top) * per_octave);
+      sum += (kept >> j) & 1u ? w : 0.f;
+      run[j] = sum;
+    }
+    const float share = (float)(in_block / mass) * sum, room = sum * 0x1p-18f;
+    unsigned passed = 0u, near = 0u;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      passed |= (run[j] > share ? 1u : 0u) << j;
+      near |= (fabsf(run[j] - share) <= room ? 1u : 0u) << j;
+    }
+    passed &= kept;
+    int at = __ffs((int)passed) - 1;
+    if (at < 0 || near || !(sum < 1e30f)) {
+      // in fp64, entry by entry
+      double acc = 0.0;
+      at = -1;
+      for (int j = 0; j < 16; ++j) {
+        if ((kept >> j) & 1u) {
+          const double w = weight_of(load_score<DT>(v.s, i0 + j), st.M, par.inv_t, s_exp);
+          at = j;
+          acc += w;
+          if (acc > in_block) break;
+        }
       }
     }
-    a.idx[out0 + d] = at;
-    if (a.prob) a.prob[out0 + d] = (float)(w_at / total);
+    a.idx[out0 + d] = i0 + at;
+    if (a.prob) a.prob[out0 + d] = (float)(weight_of(load_score<DT>(v.s, i0 + at), st.M, par.inv_t, s_exp) / total);
   }
 }
 
@@ -880,10 +919,11 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.chunk_sum = take(sizeof(double) * n_rows * l.n_chunks);
   l.block_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kBlock));
   l.block_kept = take(sizeof(unsigned short) * n_rows * l.n_chunks * (l.chunk / kBlock));
-  // Parts: about 1 024 workgroups over all rows, but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
+  // Parts: up to 1 024 workgroups over all rows (four of 512 threads on each of 256 CUs: one round), but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
   // row's, which costs what reading some thousand entries does).
   const long long cols = n_cols > 0 ? n_cols : 1;
-  long long parts = (1024 + n_rows - 1) / (n_rows > 0 ? n_rows : 1);
+  long long parts = 1024 / (n_rows > 0 ? n_rows : 1);
+  if (parts < 1) parts = 1;
   if (parts > (cols + 8191) / 8192) parts = (cols + 8191) / 8192;
   if (parts > kMaxParts) parts = kMaxParts;
   l.part_len = (int)(((cols + parts - 1) / parts + 2047) / 2048 * 2048);
@@ -955,9 +995,10 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
   a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
   a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
-  // Draws to a workgroup: its start costs a pass over kCoarse sums, so eight to a thread once every CU has work.
+  // Draws to a workgroup: its start costs a pass over kCoarse sums, so up to eight to a thread once the card is full (six
+  // workgroups on each of 256 CUs).
   a.pick_len = kPickThreads;
-  while (a.pick_len < 8 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len > 2048) a.pick_len *= 2;
+  while (a.pick_len < 8 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len > 1536) a.pick_len *= 2;
   a.pick_wgs = (int)((a.n_draws + a.pick_len - 1) / a.pick_len);
   // Places in LDS as close as kCoarse of them reach; few draws do not repay filling them and start from the chunks.
   a.coarse_blocks = a.chunk / kBlock;
