@@ -31,10 +31,10 @@ struct DrawArgs {
   double* bin_excl;            // [n_rows][kBins]: running sums in front of the bins; those behind them replace bin_mass
   unsigned long long* list_a; unsigned long long* list_b; int list_cap;      // [n_rows][list_cap] numbers of candidate entries
   double* chunk_sum;           // [n_rows][n_chunks]
-  double* block_incl;          // [n_rows][n_chunks * chunk / 16]: running sums inside a chunk, at the end of each 16 entries
-  unsigned short* block_kept;  // [n_rows][n_chunks * chunk / 16]: which of a block's entries are kept
+  struct DrawGroup* group;     // [n_rows][n_chunks * chunk / kGroup]
+  double* group_incl;          // [n_rows][n_chunks * chunk / kGroup]: a group's last running sum once more, packed
   int n_chunks, chunk;         // entries of a chunk (a multiple of kTile)
-  int pick_wgs, coarse_blocks; long long pick_len;      // k_draw_pick: workgroups and draws to a workgroup; blocks between places in LDS
+  int pick_wgs, place_groups; long long pick_len;       // k_draw_pick: workgroups and draws to a workgroup; groups between places in LDS
 };
 struct DrawState {
   u64 thr;                     // kept: number(entry) >= thr
@@ -50,7 +50,12 @@ struct DrawCut {
   double above_k, total;           // mass of the bins before k_bin; of all
 };
 
+// Eight blocks of 16 entries, one 128-byte line: the running sums inside their chunk at the end of each block, and which of
+// a block's entries are kept.
+struct alignas(128) DrawGroup { double incl[8]; unsigned short kept[8]; };
+
 constexpr int kBlock = 16;     // entries to a stored running sum: one 64-byte line of fp32 scores
+constexpr int kGroup = 8 * kBlock;
 constexpr int kTile = 4096;    // entries that a workgroup of k_draw_sums takes per step
 constexpr int kMaxChunks = 1024;
 constexpr int kMaxParts = 256;
@@ -719,7 +724,7 @@ __device__ __forceinline__ Kept kept_from(u64 thr) {
 __device__ __forceinline__ bool is_kept(float s, int i, const Kept& k) { return s > k.thr_s || (s == k.thr_s && i <= k.thr_i); }
 
 // One workgroup to a chunk: four entries to a lane, four lanes to a block of 16.  Leaves the running sums at the end of each
-// block and which of its entries are kept (16 bits): a draw then reads neither mask nor threshold.
+// block and which of its entries are kept: a draw then reads neither mask nor threshold.
 template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a) {
   __shared__ double blk[kTile / kBlock];
   __shared__ double wsum[4];
@@ -732,8 +737,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
   const Kept kp = kept_from(st.thr);
   __syncthreads();
   double carry = 0.0;
-  const int per_chunk = a.chunk / kBlock;
-  const long long out0 = ((long long)r * a.n_chunks + blockIdx.x) * per_chunk;
+  const long long out0 = ((long long)r * a.n_chunks + blockIdx.x) * (a.chunk / kGroup);
   for (int t0 = 0; t0 < a.chunk; t0 += kTile) {
     const long long base = (long long)blockIdx.x * a.chunk + t0;
     if (base >= a.n_cols) break;                    // (uniform; nothing reads the sums behind the row's end)
@@ -762,8 +766,9 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
       bits |= (unsigned)__shfl_xor((int)bits, 1);
       bits |= (unsigned)__shfl_xor((int)bits, 2);
       if ((tid & 3) == 0) {
-        blk[j * 64 + (tid >> 2)] = w;
-        a.block_kept[out0 + t0 / kBlock + j * 64 + (tid >> 2)] = (unsigned short)bits;
+        const int q = j * 64 + (tid >> 2);
+        blk[q] = w;
+        a.group[out0 + t0 / kGroup + (q >> 3)].kept[q & 7] = (unsigned short)bits;
       }
     }
     __syncthreads();
@@ -775,7 +780,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
     double before = carry;
     for (int j = 0; j < (tid >> 6); ++j) before += wsum[j];
     s += before;
-    a.block_incl[out0 + t0 / kBlock + tid] = s;
+    a.group[out0 + t0 / kGroup + (tid >> 3)].incl[tid & 7] = s;
+    if ((tid & 7) == 7) a.group_incl[out0 + t0 / kGroup + (tid >> 3)] = s;
     carry = ((((carry + wsum[0]) + wsum[1]) + wsum[2]) + wsum[3]);
     __syncthreads();
   }
@@ -783,12 +789,13 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
 }
 
 // ---------------------------------------------------------------- the draws
-// A workgroup holds its row's running sums at up to kCoarse places in LDS, so that a draw searches in LDS first, then among
-// the few blocks between two places, then in one block of 16 entries.  Bound: the scattered reads of the last two.  The
-// workgroups of a row run on one XCD (consecutive ones are dealt out to the eight in turn), whose L2 then holds the row.
-constexpr int kCoarse = 2048, kPickThreads = 512;
-template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(DrawArgs a) {
-  __shared__ double coarse[kCoarse];
+// A workgroup holds its row's running sums in LDS, at the end of every group if they fit, so that a draw searches there and
+// then reads two lines: its group's, and the scores of one block.  Bound: these scattered lines -- about one request per
+// clock and L2 channel; a search in global memory made twelve of them (82 us for 1.5 M draws).  The workgroups of a row run
+// on one XCD (consecutive ones are dealt out to the eight in turn), whose L2 then holds the row.
+constexpr int kPlaces = 6656, kPickThreads = 1024;      // 52 KB: groups of 850 000 entries
+template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick(DrawArgs a) {
+  __shared__ double place[kPlaces];        // running sums inside a chunk, as group_incl
   __shared__ double chunk_incl[kMaxChunks];
   __shared__ double wsum[kPickThreads / 64];
   __shared__ ExpTable s_exp;
@@ -807,59 +814,67 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(Dr
     for (long long d = d0 + tid; d < d1; d += kPickThreads) { a.idx[out0 + d] = -1; if (a.prob) a.prob[out0 + d] = 0.f; }
     return;
   }
-  // running sums over the row's chunks, two to a thread
-  double c0 = 2 * tid < nc ? a.chunk_sum[(long long)r * nc + 2 * tid] : 0.0;
-  double c1 = 2 * tid + 1 < nc ? a.chunk_sum[(long long)r * nc + 2 * tid + 1] : 0.0;
-  double t = c0 + c1;
+  // running sums over the row's chunks, one to a thread
+  double t = tid < nc ? a.chunk_sum[(long long)r * nc + tid] : 0.0;
   for (int o = 1; o < 64; o <<= 1) { const double x = shfl_up_d(t, o); if (lane >= o) t += x; }
-  double before = __shfl_up(t, 1);
-  if (lane == 0) before = 0.0;
   if (lane == 63) wsum[tid >> 6] = t;
+  const int n_groups = (int)(((long long)a.n_cols + kGroup - 1) / kGroup), per_chunk = a.chunk / kGroup, step = a.place_groups, per = per_chunk / step;
+  const long long g0 = (long long)r * nc * per_chunk;
+  // (what lies behind the row's last group is never looked at)
+  for (int j = tid; j < nc * per; j += kPickThreads) { const int g = (j + 1) * step - 1; place[j] = g < n_groups ? a.group_incl[g0 + g] : __builtin_inf(); }
   __syncthreads();
+  double before = 0.0;
   for (int j = 0; j < (tid >> 6); ++j) before += wsum[j];
-  chunk_incl[2 * tid] = before + c0;
-  chunk_incl[2 * tid + 1] = before + c0 + c1;
+  chunk_incl[tid] = before + t;
   __syncthreads();
   const double total = chunk_incl[kMaxChunks - 1];
-  const int per_chunk = a.chunk / kBlock, step = a.coarse_blocks, per = per_chunk / step, n_coarse = nc * per;
-  const long long blocks0 = (long long)r * nc * per_chunk;
-  const int n_blocks = (int)(((long long)a.n_cols + kBlock - 1) / kBlock);
-  int coarse_top = 1;
-  while (2 * coarse_top < n_coarse) coarse_top <<= 1;        // the search below ends at 2 coarse_top - 1, up to kCoarse - 1
-  for (int j = tid; j < 2 * coarse_top; j += kPickThreads) {
-    if (j >= n_coarse) { coarse[j] = __builtin_inf(); continue; }
-    const int ch = j / per;
-    // (the last chunk's sums end with the row's last tile: what lies behind holds the row's total)
-    const int end = (j + 1) * step - 1;
-    const double base = ch ? chunk_incl[ch - 1] : 0.0;
-    coarse[j] = (j + 1) % per == 0 || end >= n_blocks ? chunk_incl[ch] : base + a.block_incl[blocks0 + end];
-  }
-  __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const RowPar par = row_par(a, r);
   const float per_octave = (float)(par.inv_t * 1.4426950408889634);
+  const DrawGroup* const groups = a.group + g0;
   for (long long d = d0 + tid; d < d1; d += kPickThreads) {
     double u = (double)a.u[(long long)r * a.u_stride + d];
     u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
-    const double target = u * total;                 // below the total: the last place passes it
-    int lo = 0;
-    for (int k = coarse_top; k > 0; k >>= 1) { if (coarse[lo + k - 1] <= target) lo += k; }      // first place that passes the target
-    const int ch = lo / per;
+    const double target = u * total;                 // below the total: the last chunk passes it
+    int ch = 0, hi = nc - 1;
+    while (ch < hi) { const int mid = (ch + hi) >> 1; if (chunk_incl[mid] > target) hi = mid; else ch = mid + 1; }
     const double in_chunk = target - (ch ? chunk_incl[ch - 1] : 0.0);
-    const double* bi = a.block_incl + blocks0;
-    int b0 = lo * step, b1 = min(b0 + step, n_blocks) - 1;
-    while (b0 < b1) { const int mid = (b0 + b1) >> 1; if (bi[mid] > in_chunk) b1 = mid; else b0 = mid + 1; }
-    const double front = b0 % per_chunk ? bi[b0 - 1] : 0.0;
+    // the first place, group and block that pass it (the last ones, should rounding leave none)
+    const int last_group = min((ch + 1) * per_chunk, n_groups) - 1;
+    int lo = ch * per;
+    hi = min(lo + per - 1, last_group / step);
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (place[mid] > in_chunk) hi = mid; else lo = mid + 1; }
+    int g = lo * step;
+    hi = min(g + step - 1, last_group);
+    double front = lo > ch * per ? place[lo - 1] : 0.0;
+    while (g < hi) {
+      const int mid = (g + hi) >> 1;
+      const double x = a.group_incl[g0 + mid];
+      if (x > in_chunk) hi = mid; else { g = mid + 1; front = x; }
+    }
+    const DrawGroup& gr = groups[g];
+    double incl[8];
+    unsigned short bits[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) incl[j] = gr.incl[j];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits[j] = gr.kept[j];
+    int b = 0;
+    double back = incl[0];
+    unsigned kept = bits[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) if (incl[j - 1] <= in_chunk) { b = j; front = incl[j - 1]; back = incl[j]; kept = bits[j]; }
     double in_block = in_chunk - front;
-    const double mass = bi[b0] - front;
-    unsigned kept = a.block_kept[blocks0 + b0];
+    const double mass = back - front;
+    int block = g * 8 + b;
     if (!kept) {
-      // the target lies within rounding of a border between places: the first kept entry behind it, or the last before
-      while (!kept && b0 + 1 < n_blocks) kept = a.block_kept[blocks0 + ++b0];
-      while (!kept && b0 > 0) kept = a.block_kept[blocks0 + --b0];
+      // the target lies within rounding of a border: the first kept entry behind it, or the last before
+      const int last_block = (int)(((long long)a.n_cols + kBlock - 1) / kBlock) - 1;
+      while (!kept && block < last_block) { ++block; kept = groups[block >> 3].kept[block & 7]; }
+      while (!kept && block > 0) { --block; kept = groups[block >> 3].kept[block & 7]; }
       in_block = -1.0;
     }
-    const int i0 = b0 * kBlock;
+    const int i0 = block * kBlock;
     Four<DT> f[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = load_four<DT>(RowView{v.s, nullptr}, i0 + 4 * j, a.n_cols);
@@ -899,12 +914,17 @@ template <int DT> __global__ __launch_bounds__(kPickThreads) void k_draw_pick(Dr
       }
     }
     a.idx[out0 + d] = i0 + at;
-    if (a.prob) a.prob[out0 + d] = (float)(weight_of(load_score<DT>(v.s, i0 + at), st.M, par.inv_t, s_exp) / total);
+    if (a.prob) {
+      float s = f[0].s[0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) s = at == j ? f[j >> 2].s[j & 3] : s;
+      a.prob[out0 + d] = (float)(weight_of(s, st.M, par.inv_t, s_exp) / total);
+    }
   }
 }
 
 // ---------------------------------------------------------------- host side
-struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, block_incl, block_kept, part_max, part_min, bin_cnt, bin_mass, bin_excl, list_a, list_b, total; };
+struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, group, group_incl, part_max, part_min, bin_cnt, bin_mass, bin_excl, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   DrawLayout l;
   // chunks of one tile; of more where a row would have over kMaxChunks of them
@@ -917,8 +937,8 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.state = take(sizeof(DrawState) * n_rows);
   l.cut = take(sizeof(DrawCut) * n_rows);
   l.chunk_sum = take(sizeof(double) * n_rows * l.n_chunks);
-  l.block_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kBlock));
-  l.block_kept = take(sizeof(unsigned short) * n_rows * l.n_chunks * (l.chunk / kBlock));
+  l.group = take(sizeof(DrawGroup) * n_rows * l.n_chunks * (l.chunk / kGroup));
+  l.group_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kGroup));
   // Parts: up to 1 024 workgroups over all rows (four of 512 threads on each of 256 CUs: one round), but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
   // row's, which costs what reading some thousand entries does).
   const long long cols = n_cols > 0 ? n_cols : 1;
@@ -988,21 +1008,24 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.t_all = q->temperature_all; a.p_all = q->top_p_all; a.m_all = q->min_p_all; a.k_all = q->top_k_all;
   a.u = q->u; a.u_stride = q->u_stride; a.idx = q->idx; a.prob = q->prob;
   char* w = (char*)q->ws;
-  a.state = (DrawState*)(w + l.state); a.cut = (DrawCut*)(w + l.cut); a.chunk_sum = (double*)(w + l.chunk_sum); a.block_incl = (double*)(w + l.block_incl);
-  a.block_kept = (unsigned short*)(w + l.block_kept);
+  a.state = (DrawState*)(w + l.state); a.cut = (DrawCut*)(w + l.cut); a.chunk_sum = (double*)(w + l.chunk_sum); a.group = (DrawGroup*)(w + l.group);
+  a.group_incl = (double*)(w + l.group_incl);
   a.n_chunks = l.n_chunks; a.chunk = l.chunk;
   a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
   a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
   a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
   a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
-  // Draws to a workgroup: its start costs a pass over kCoarse sums, so up to eight to a thread once the card is full (six
+  // Draws to a workgroup: its start costs a pass over the row's running sums, so several to a thread once the card is full (two
   // workgroups on each of 256 CUs).
   a.pick_len = kPickThreads;
-  while (a.pick_len < 8 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len > 1536) a.pick_len *= 2;
+  while (a.pick_len < 16 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len >= 512) a.pick_len += kPickThreads;
   a.pick_wgs = (int)((a.n_draws + a.pick_len - 1) / a.pick_len);
-  // Places in LDS as close as kCoarse of them reach; few draws do not repay filling them and start from the chunks.
-  a.coarse_blocks = a.chunk / kBlock;
-  if (a.n_draws > 64) while (a.coarse_blocks % 2 == 0 && (long long)a.n_chunks * (a.chunk / kBlock) / (a.coarse_blocks / 2) <= kCoarse) a.coarse_blocks /= 2;
+  // Places in LDS: every group's end if they fit, else every second, fourth ...; few draws do not repay filling them and start
+  // from the chunks.
+  const int per_chunk = a.chunk / kGroup;
+  a.place_groups = 1;
+  while ((long long)a.n_chunks * (per_chunk / a.place_groups) > (a.n_draws > 64 ? kPlaces : a.n_chunks))
+    a.place_groups = per_chunk % (2 * a.place_groups) == 0 ? 2 * a.place_groups : per_chunk;
   hipStream_t s = (hipStream_t)stream;
   if (q->dtype == PSL_F32) launch_draw<PSL_F32>(a, s);
   else if (q->dtype == PSL_BF16) launch_draw<PSL_BF16>(a, s);
