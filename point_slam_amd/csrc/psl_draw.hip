@@ -38,12 +38,15 @@ struct DrawArgs {
 };
 struct DrawState {
   u64 thr;                     // kept: number(entry) >= thr
+  double inv_t, m;             // 1 / temperature, min-p
   float M; int any;            // largest allowed score; whether there is one
   unsigned n_a, n_b;           // fill of the two lists
 };
 
 struct DrawCut {
-  unsigned want;                   // entries of k_bin that top-k keeps
+  float M; int any;                // as in DrawState
+  double inv_t, p, width;          // 1 / temperature, top-p (1: off), a bin's width
+  float scale; unsigned want;      // bins per unit of score; entries of k_bin that top-k keeps
   int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
   unsigned n_a;                    // entries of k_bin
   unsigned key[4];                 // keys of k_bin: [0] .. [1] - 1; of [p_lo, p_hi]: [2] .. [3] - 1
@@ -107,14 +110,16 @@ __device__ __forceinline__ RowPar row_par(const DrawArgs& a, int r) {
 // into the exponent.  Beyond x = 1100 the result is 0; a NaN counts as that.
 struct ExpTable { double t[64]; };
 __device__ __forceinline__ void exp_table_init(ExpTable& e) { if (threadIdx.x < 64) e.t[threadIdx.x] = exp2(-(double)threadIdx.x / 64.0); }
+// a constant that stays in a scalar register (the compiler would write it into two vector registers for every use)
+__device__ __forceinline__ double resident(double c) { asm("" : "+s"(c)); return c; }
 __device__ __forceinline__ double exp_neg(double x, const ExpTable& e) {
   x = fmin(x, 1100.0);
-  const double n = rint(x * 92.332482616893656);        // 64 / ln2
-  double r = fma(n, -0x1.62e42fefa39efp-7, x);          // ln2 / 64, and what that number leaves of it
-  r = fma(n, -0x1.abc9e3b39803fp-62, r);
+  const double n = rint(x * resident(92.332482616893656));          // 64 / ln2
+  double r = fma(n, resident(-0x1.62e42fefa39efp-7), x);            // ln2 / 64, and what that number leaves of it
+  r = fma(n, resident(-0x1.abc9e3b39803fp-62), r);
   const int k = (int)n;
-  double p = fma(r, -1.0 / 120.0, 1.0 / 24.0);
-  p = fma(r, p, -1.0 / 6.0);
+  double p = fma(r, resident(-1.0 / 120.0), resident(1.0 / 24.0));
+  p = fma(r, p, resident(-1.0 / 6.0));
   p = fma(r, p, 0.5);
   p = fma(r, p, -1.0);
   p = fma(r, p, 1.0);
@@ -325,11 +330,15 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
   __shared__ unsigned s_want, s_na;
   const int r = blockIdx.x, j = threadIdx.x, lane = j & 63, wave = j >> 6;
   const RowPar par = row_par(a, r);
-  if (!has_cut(par)) return;
+  DrawCut* o = a.cut + r;
   if (j == 0) { s_k = kBins; s_lo = kBins; s_hi = kBins; s_last = -1; s_want = 0u; s_na = 0u; }
   const Range g = row_range(a, r);
-  if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
+  if (j == 0) { o->M = b.M; o->any = g.mx ? 1 : 0; o->inv_t = par.inv_t; o->p = par.k == 1 ? 1.0 : par.p; o->width = b.width; o->scale = b.scale; }
+  if (!g.mx || !has_cut(par)) {
+    if (j == 0) { o->k_bin = kBins; o->p_hi = -1; o->n_a = 0u; }
+    return;
+  }
   const unsigned c = a.bin_cnt[(long long)r * kBins + j];
   const double m = ldexp((double)a.bin_mass[(long long)r * kBins + j], -bin_shift(b, j));
   unsigned n_incl = c; double incl = m;
@@ -365,7 +374,6 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
   }
   __syncthreads();
   const int p_lo = cut_p ? min(s_lo, s_last) : 0, p_hi = cut_p ? min(s_hi, s_last) : -1;
-  DrawCut* o = a.cut + r;
   if (j < 4) {
     const int bin = j == 0 ? k_bin : j == 1 ? k_bin - 1 : j == 2 ? p_hi : p_lo - 1;
     o->key[j] = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
@@ -390,16 +398,13 @@ __device__ __forceinline__ void list_add(ListBuf& b, u64 x, u64* dst, unsigned* 
 template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs a) {
   __shared__ ListBuf buf_a, buf_b;
   const int r = blockIdx.y, tid = threadIdx.x;
-  const RowPar par = row_par(a, r);
-  if (!has_cut(par)) return;
-  if (tid == 0) { buf_a.n = 0u; buf_b.n = 0u; }
-  const Range g = row_range(a, r);
-  if (!g.mx) return;
   const DrawCut& c = a.cut[r];
   const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.p_hi >= 0;
   if (!do_a && !do_b) return;
   // (no such bin: an empty interval)
   const unsigned a0 = do_a ? c.key[0] : 1u, a1 = do_a ? c.key[1] : 0u, b0 = do_b ? c.key[2] : 1u, b1 = do_b ? c.key[3] : 0u;
+  if (tid == 0) { buf_a.n = 0u; buf_b.n = 0u; }
+  __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
   u64* la = a.list_a + (long long)r * a.list_cap;
@@ -599,18 +604,19 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
   __shared__ double s_wave[16], s_kept;
   __shared__ int s_bin, s_at, s_end;
   const ExpTable& s_exp = sh.exp;
-  exp_table_init(sh.exp);               // (row_range's barrier covers it)
+  exp_table_init(sh.exp);
   const int r = blockIdx.x, tid = threadIdx.x;
-  const RowPar par = row_par(a, r);
-  const Range g = row_range(a, r);
-  const float M = score_of(g.mx);
+  const DrawCut& c = a.cut[r];
+  const float M = c.M;
+  const double inv_t = c.inv_t;
+  const bool cut_k = c.k_bin < kBins, cut_p = c.p < 1.0;
   u64 thr = 1ull << 32;                             // every allowed entry
-  if (g.mx && has_cut(par)) {
+  __syncthreads();                                  // (the table)
+  if (c.any && (cut_k || cut_p)) {
     const RowView v = row_view<DT>(a, r);
     const u64* la = a.list_a + (long long)r * a.list_cap;
     const u64* lb = a.list_b + (long long)r * a.list_cap;
     const double* cum = (const double*)(a.bin_mass + (long long)r * kBins);
-    const DrawCut& c = a.cut[r];
     const unsigned n_b = a.state[r].n_b;
     const bool listed_a = c.n_a <= (unsigned)a.list_cap, listed_b = n_b <= (unsigned)a.list_cap;
     // a list that its entries do not fit into: the row itself, entry by entry
@@ -621,7 +627,6 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
       return k >= a0 && k < a1 ? number_of(k, i) : 0ull;
     };
     const int len_a = listed_a ? (int)c.n_a : a.n_cols;
-    const bool cut_k = c.k_bin < kBins, cut_p = par.p < 1.0 && par.k != 1;
     double kept = 0.0;                              // mass of what top-k keeps of its bin
     bool p_in_a = false;
     if (cut_k && len_a <= kSorted) {
@@ -630,13 +635,13 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
       if (tid == (int)c.want - 1) s_thr = x;
       double incl = 0.0;
       if (cut_p) {
-        incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp) : 0.0, s_wave);
+        incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, inv_t, s_exp) : 0.0, s_wave);
         if (tid == (int)c.want - 1) s_kept = incl;
       }
       __syncthreads();
       if (cut_p) {
         kept = s_kept;
-        const double target = par.p * (c.above_k + kept);
+        const double target = c.p * (c.above_k + kept);
         p_in_a = target > c.above_k;
         if (p_in_a) {
           note_first(&s_at, incl >= target - c.above_k);
@@ -648,35 +653,36 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
       thr = s_thr;
     } else if (cut_k) {
       const Numbers<decltype(src_a)> num(src_a, len_a);
-      const u64 thr_k = radix_select(num, false, c.want, 0.0, M, par.inv_t, sh);
+      const u64 thr_k = radix_select(num, false, c.want, 0.0, M, inv_t, sh);
       thr = thr_k;
       if (cut_p) {
         __syncthreads();
         if (tid == 0) { sh.hi = 0ull; sh.lo = 0ull; }
         __syncthreads();
         u64 hi = 0ull, lo = 0ull;
-        num.each([&](u64 x) { if (x >= thr_k) { const Fixed f = to_fixed(weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp)); hi += f.hi; lo += f.lo; } });
+        num.each([&](u64 x) { if (x >= thr_k) { const Fixed f = to_fixed(weight_of(score_of((unsigned)(x >> 32)), M, inv_t, s_exp)); hi += f.hi; lo += f.lo; } });
         for (int o = 32; o > 0; o >>= 1) { hi += __shfl_xor(hi, o); lo += __shfl_xor(lo, o); }
         if ((tid & 63) == 0) { atomicAdd(&sh.hi, hi); atomicAdd(&sh.lo, lo); }
         __syncthreads();
         kept = fixed_d(sh.hi, sh.lo);
-        const double target = par.p * (c.above_k + kept);
+        const double target = c.p * (c.above_k + kept);
         p_in_a = target > c.above_k;
         if (p_in_a) {
           auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
-          thr = radix_select(Numbers<decltype(src)>(src, len_a), true, 0u, target - c.above_k, M, par.inv_t, sh);
+          thr = radix_select(Numbers<decltype(src)>(src, len_a), true, 0u, target - c.above_k, M, inv_t, sh);
         }
       }
     }
     if (cut_p && !p_in_a && c.p_hi >= 0) {
-      const double target = par.p * (cut_k ? c.above_k + kept : c.total);
+      const double target = c.p * (cut_k ? c.above_k + kept : c.total);
       // first bin of [p_lo, p_hi] whose running sum reaches the target (empty ones hold -1; p_hi is not empty)
       if (tid == 0) s_bin = c.p_hi;
       __syncthreads();
       for (int j = c.p_lo + tid; j < c.p_hi; j += 1024) if (cum[j] >= target) atomicMin(&s_bin, j);
       __syncthreads();
       const int bin = s_bin;
-      const Binning b = make_binning(g, par.inv_t, a.n_cols);
+      Binning b;
+      b.M = M; b.scale = c.scale;
       const unsigned b0 = c.key[2], b1 = c.key[3];
       auto src = [&](int i) -> u64 {
         u64 x = 0ull;
@@ -689,7 +695,7 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
       u64 t;
       if (len_b <= kSorted) {
         const u64 x = block_sort(tid < len_b ? src(tid) : 0ull, len_b, s_sort);
-        const double incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, par.inv_t, s_exp) : 0.0, s_wave);
+        const double incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, inv_t, s_exp) : 0.0, s_wave);
         // (none reaches it, by rounding: the last one)
         if (tid == 0) { s_at = kSorted; s_end = 0; }
         __syncthreads();
@@ -699,18 +705,22 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
         if (tid == min(s_at, s_end)) s_thr = x;
         __syncthreads();
         t = s_thr;
-      } else t = radix_select(Numbers<decltype(src)>(src, len_b), true, 0u, target - before, M, par.inv_t, sh);
+      } else t = radix_select(Numbers<decltype(src)>(src, len_b), true, 0u, target - before, M, inv_t, sh);
       if (t > thr) thr = t;                         // (an empty source gives 0)
     }
   }
-  if (tid == 0) { a.state[r].thr = thr; a.state[r].M = M; a.state[r].any = g.mx ? 1 : 0; }
+  if (tid == 0) {
+    DrawState* o = a.state + r;
+    o->thr = thr; o->M = M; o->any = c.any; o->inv_t = inv_t; o->m = row_par(a, r).m;
+  }
 }
 
-// a row's threshold, largest score, and whether it has one
+// what k_draw_sums and k_draw_pick need of a row
 __device__ __forceinline__ DrawState row_state(const DrawArgs& a, int r) {
   if (a.cuts) return a.state[r];
   const Range g = row_range(a, r);
-  return DrawState{1ull << 32, score_of(g.mx), g.mx ? 1 : 0, 0u, 0u};
+  const RowPar par = row_par(a, r);
+  return DrawState{1ull << 32, par.inv_t, par.m, score_of(g.mx), g.mx ? 1 : 0, 0u, 0u};
 }
 
 // ---------------------------------------------------------------- running sums of the kept weights
@@ -733,8 +743,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
   exp_table_init(s_exp);
   const RowView v = row_view<DT>(a, r);
   const DrawState st = row_state(a, r);
-  const RowPar par = row_par(a, r);
   const Kept kp = kept_from(st.thr);
+  const double least = fmax(st.m, 0x1p-1074);       // (what weighs nothing is never drawn)
   __syncthreads();
   double carry = 0.0;
   const long long out0 = ((long long)r * a.n_chunks + blockIdx.x) * (a.chunk / kGroup);
@@ -756,8 +766,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         if (((f[j].live >> q) & 1u) && is_kept(f[j].s[q], e + q, kp)) {
-          const double x = weight_of(f[j].s[q], st.M, par.inv_t, s_exp);
-          if (x > 0.0 && x >= par.m) { w += x; bits |= 1u << q; }
+          const double x = weight_of(f[j].s[q], st.M, st.inv_t, s_exp);
+          if (x >= least) { w += x; bits |= 1u << q; }
         }
       }
       bits <<= 4 * (lane & 3);
@@ -829,8 +839,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
   __syncthreads();
   const double total = chunk_incl[kMaxChunks - 1];
   const RowView v = row_view<DT>(a, r);
-  const RowPar par = row_par(a, r);
-  const float per_octave = (float)(par.inv_t * 1.4426950408889634);
+  const float per_octave = (float)(st.inv_t * 1.4426950408889634);
   const DrawGroup* const groups = a.group + g0;
   for (long long d = d0 + tid; d < d1; d += kPickThreads) {
     double u = (double)a.u[(long long)r * a.u_stride + d];
@@ -906,7 +915,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
       at = -1;
       for (int j = 0; j < 16; ++j) {
         if ((kept >> j) & 1u) {
-          const double w = weight_of(load_score<DT>(v.s, i0 + j), st.M, par.inv_t, s_exp);
+          const double w = weight_of(load_score<DT>(v.s, i0 + j), st.M, st.inv_t, s_exp);
           at = j;
           acc += w;
           if (acc > in_block) break;
@@ -918,7 +927,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
       float s = f[0].s[0];
 #pragma unroll
       for (int j = 1; j < 16; ++j) s = at == j ? f[j >> 2].s[j & 3] : s;
-      a.prob[out0 + d] = (float)(weight_of(s, st.M, par.inv_t, s_exp) / total);
+      a.prob[out0 + d] = (float)(weight_of(s, st.M, st.inv_t, s_exp) / total);
     }
   }
 }
