@@ -238,9 +238,42 @@ __device__ __forceinline__ u64 to_integer(double x) { return (u64)__double_as_lo
 
 // An entry's scaled weight is its bin's first weight (a table) times e^-f, f < kRange / kBins = 0.047 behind the bin's begin:
 // the terms to the seventh leave 1e-15 of it.  What lies beyond kRange counts as lying at the last bin's end: 1e-21 of the
-// largest weight, a million of which do not reach the sum's rounding.  Bound: instructions (65 per entry made this 25 us for
-// twelve rows of 816 000), then the LDS atomics: entries are counted only where top-k asks and weighed only where top-p
-// does, and neighbouring lanes use different copies.
+// largest weight, a million of which do not reach the sum's rounding.
+__device__ __forceinline__ double first_weight(const Binning& b, int j) {
+  return b.M == __builtin_inff() && j ? 0.0 : ldexp(exp(-(double)j * b.width), bin_shift(b, j));
+}
+// the coefficients stay in registers (the compiler would write them anew for every entry: they are not inline constants)
+struct BinPoly { double c7, c6, c5, c4, c3; };
+__device__ __forceinline__ BinPoly make_bin_poly() {
+  BinPoly p{-1.0 / 5040.0, 1.0 / 720.0, -1.0 / 120.0, 1.0 / 24.0, -1.0 / 6.0};
+  asm("" : "+v"(p.c7), "+v"(p.c6), "+v"(p.c5), "+v"(p.c4), "+v"(p.c3));
+  return p;
+}
+template <int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f, const Binning& b, const BinPoly& c, bool count, bool weigh,
+                                                              unsigned* cnt, u64* mass, const double* first) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const float s = f.s[q];
+    if (((f.live >> q) & 1u) && s > -__builtin_inff()) {
+      const int bin = bin_of(b, s);
+      if (count) atomicAdd(&cnt[bin], 1u);
+      if (weigh) {
+        const double y = fmin(fma((double)bin, -b.width, ((double)b.M - (double)s) * b.inv_t), b.width);      // (a NaN gives the width)
+        double p = fma(y, c.c7, c.c6);
+        p = fma(y, p, c.c5);
+        p = fma(y, p, c.c4);
+        p = fma(y, p, c.c3);
+        p = fma(y, p, 0.5);
+        p = fma(y, p, -1.0);
+        p = fma(y, p, 1.0);
+        atomicAdd(&mass[bin], to_integer(first[bin] * p));
+      }
+    }
+  }
+}
+
+// Bound: instructions (65 per entry made this 25 us for twelve rows of 816 000), then the LDS atomics: entries are counted
+// only where top-k asks and weighed only where top-p does, and neighbouring lanes use different copies.
 constexpr int kCopies = 2;
 template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
   __shared__ unsigned cnt[kCopies][kBins];
@@ -253,43 +286,21 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   const Range g = row_range(a, r);
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
-  const bool inf_row = b.M == __builtin_inff();
   for (int j = tid; j < kBins; j += 512) {
 #pragma unroll
     for (int q = 0; q < kCopies; ++q) { cnt[q][j] = 0u; mass[q][j] = 0ull; }
-    if (weigh) first[j] = inf_row && j ? 0.0 : ldexp(exp(-(double)j * b.width), bin_shift(b, j));
+    if (weigh) first[j] = first_weight(b, j);
   }
   __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
   unsigned* const my_cnt = cnt[tid & (kCopies - 1)];
   u64* const my_mass = mass[tid & (kCopies - 1)];
-  const double M = (double)b.M;
-  // the coefficients stay in registers (the compiler would write them anew for every entry: they are not inline constants)
-  double c7 = -1.0 / 5040.0, c6 = 1.0 / 720.0, c5 = -1.0 / 120.0, c4 = 1.0 / 24.0, c3 = -1.0 / 6.0;
-  asm("" : "+v"(c7), "+v"(c6), "+v"(c5), "+v"(c4), "+v"(c3));
+  const BinPoly poly = make_bin_poly();
 #pragma unroll 2
   for (int i = i0 + tid * 4; i < i1; i += 2048) {
     const Four<DT> f = load_four<DT>(v, i, i1);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float s = f.s[q];
-      if (((f.live >> q) & 1u) && s > -__builtin_inff()) {
-        const int bin = bin_of(b, s);
-        if (count) atomicAdd(&my_cnt[bin], 1u);
-        if (weigh) {
-          const double y = fmin(fma((double)bin, -b.width, (M - (double)s) * b.inv_t), b.width);      // (a NaN gives the width)
-          double p = fma(y, c7, c6);
-          p = fma(y, p, c5);
-          p = fma(y, p, c4);
-          p = fma(y, p, c3);
-          p = fma(y, p, 0.5);
-          p = fma(y, p, -1.0);
-          p = fma(y, p, 1.0);
-          atomicAdd(&my_mass[bin], to_integer(first[bin] * p));
-        }
-      }
-    }
+    add_to_bins(f, b, poly, count, weigh, my_cnt, my_mass, first);
   }
   __syncthreads();
   for (int j = tid; j < kBins; j += 512) {
@@ -321,67 +332,72 @@ __device__ __forceinline__ void note_last(int* at, bool cond) {
   const u64 m = __ballot(cond);
   if (m && (threadIdx.x & 63) == 0) atomicMax(at, (int)(threadIdx.x & ~63u) + 63 - __clzll((long long)m));
 }
-// Which bins the two limits fall into: one workgroup to a row, a thread to a bin, the largest scores first.  (In every
-// workgroup of k_draw_gather instead, this cost each of them 8 us.)
-__global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
-  __shared__ unsigned s_cnt[kBins / 64];
-  __shared__ double s_mass[kBins / 64], s_above_k, s_most;
-  __shared__ int s_k, s_lo, s_hi, s_last;
-  __shared__ unsigned s_want, s_na;
-  const int r = blockIdx.x, j = threadIdx.x, lane = j & 63, wave = j >> 6;
-  const RowPar par = row_par(a, r);
-  DrawCut* o = a.cut + r;
-  if (j == 0) { s_k = kBins; s_lo = kBins; s_hi = kBins; s_last = -1; s_want = 0u; s_na = 0u; }
-  const Range g = row_range(a, r);
-  const Binning b = make_binning(g, par.inv_t, a.n_cols);
-  if (j == 0) { o->M = b.M; o->any = g.mx ? 1 : 0; o->inv_t = par.inv_t; o->p = par.k == 1 ? 1.0 : par.p; o->width = b.width; o->scale = b.scale; }
+// Which bins the two limits fall into, by a workgroup with a thread to a bin, the largest scores first: c entries, mass m.
+// cum / excl receive the running sums behind and in front of the bins (behind an empty one: -1).
+struct BinsShared { unsigned cnt[kBins / 64]; double mass[kBins / 64], above_k, most; int k, lo, hi, last; unsigned want, na; };
+__device__ __forceinline__ void find_bins(const DrawArgs& a, const RowPar& par, const Range& g, const Binning& b, unsigned c, double m,
+                                          double* cum, double* excl_out, DrawCut* o, BinsShared& sh) {
+  const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
+  if (j == 0) {
+    sh.k = kBins; sh.lo = kBins; sh.hi = kBins; sh.last = -1; sh.want = 0u; sh.na = 0u;
+    o->M = b.M; o->any = g.mx ? 1 : 0; o->inv_t = par.inv_t; o->p = par.k == 1 ? 1.0 : par.p; o->width = b.width; o->scale = b.scale;
+  }
   if (!g.mx || !has_cut(par)) {
     if (j == 0) { o->k_bin = kBins; o->p_hi = -1; o->n_a = 0u; }
     return;
   }
-  const unsigned c = a.bin_cnt[(long long)r * kBins + j];
-  const double m = ldexp((double)a.bin_mass[(long long)r * kBins + j], -bin_shift(b, j));
   unsigned n_incl = c; double incl = m;
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned cu = __shfl_up(n_incl, o); const double mu = shfl_up_d(incl, o);
-    if (lane >= o) { n_incl += cu; incl += mu; }
+  for (int i = 1; i < 64; i <<= 1) {
+    const unsigned cu = __shfl_up(n_incl, i); const double mu = shfl_up_d(incl, i);
+    if (lane >= i) { n_incl += cu; incl += mu; }
   }
-  if (lane == 63) { s_cnt[wave] = n_incl; s_mass[wave] = incl; }
+  if (lane == 63) { sh.cnt[wave] = n_incl; sh.mass[wave] = incl; }
   __syncthreads();
   unsigned n_valid = 0u, n_before = 0u; double total = 0.0, before = 0.0;
   for (int w = 0; w < kBins / 64; ++w) {
     if (w == wave) { n_before = n_valid; before = total; }
-    n_valid += s_cnt[w]; total += s_mass[w];
+    n_valid += sh.cnt[w]; total += sh.mass[w];
   }
   // running sums in front of and behind this bin; only bins that hold something are ever chosen
   const double up = __shfl_up(incl, 1), excl = lane ? before + up : before;
   n_incl += n_before; incl += before;
-  ((double*)(a.bin_mass + (long long)r * kBins))[j] = m > 0.0 ? incl : -1.0;
-  a.bin_excl[(long long)r * kBins + j] = excl;
+  cum[j] = m > 0.0 ? incl : -1.0;
+  excl_out[j] = excl;
   const bool cut_k = par.k > 0 && (unsigned)par.k < n_valid, cut_p = par.p < 1.0 && par.k != 1;
   if (cut_k && n_incl >= (unsigned)par.k && n_incl - c < (unsigned)par.k) {
-    s_k = j; s_want = (unsigned)par.k - (n_incl - c); s_na = c; s_most = incl; s_above_k = excl;
+    sh.k = j; sh.want = (unsigned)par.k - (n_incl - c); sh.na = c; sh.most = incl; sh.above_k = excl;
   }
   __syncthreads();
-  const int k_bin = s_k;
-  const double above_k = cut_k ? s_above_k : total, most = cut_k ? s_most : total;
+  const int k_bin = sh.k;
+  const double above_k = cut_k ? sh.above_k : total, most = cut_k ? sh.most : total;
   if (cut_p) {
     // top-k leaves a mass between above_k and `most`: the bins before k_bin where its share can fall (none, by rounding: the last)
     const bool held = m > 0.0 && j < k_bin;
-    note_last(&s_last, held);
-    note_first(&s_lo, held && incl >= par.p * above_k);
-    note_first(&s_hi, held && incl >= par.p * most);
+    note_last(&sh.last, held);
+    note_first(&sh.lo, held && incl >= par.p * above_k);
+    note_first(&sh.hi, held && incl >= par.p * most);
   }
   __syncthreads();
-  const int p_lo = cut_p ? min(s_lo, s_last) : 0, p_hi = cut_p ? min(s_hi, s_last) : -1;
+  const int p_lo = cut_p ? min(sh.lo, sh.last) : 0, p_hi = cut_p ? min(sh.hi, sh.last) : -1;
   if (j < 4) {
     const int bin = j == 0 ? k_bin : j == 1 ? k_bin - 1 : j == 2 ? p_hi : p_lo - 1;
     o->key[j] = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
   }
   if (j == 64) {
-    o->want = s_want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = s_na;
-    o->above_k = above_k; o->total = total;
+    o->want = sh.want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = sh.na; o->above_k = above_k; o->total = total;
   }
+}
+// One workgroup to a row.  (In every workgroup of k_draw_gather instead, this cost each of them 8 us.)
+__global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
+  __shared__ BinsShared sh;
+  const int r = blockIdx.x, j = threadIdx.x;
+  const RowPar par = row_par(a, r);
+  const Range g = row_range(a, r);
+  const Binning b = make_binning(g, par.inv_t, a.n_cols);
+  const long long at = (long long)r * kBins + j;
+  const unsigned c = a.bin_cnt[at];
+  const double m = ldexp((double)a.bin_mass[at], -bin_shift(b, j));
+  find_bins(a, par, g, b, c, m, (double*)(a.bin_mass + (long long)r * kBins), a.bin_excl + (long long)r * kBins, a.cut + r, sh);
 }
 
 // Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.  A bin
@@ -598,120 +614,120 @@ __device__ __forceinline__ double block_running(double w, double* lds16) {
   return before + w;
 }
 
-template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
-  __shared__ RadixShared sh;
-  __shared__ u64 s_sort[kSorted], s_thr;
-  __shared__ double s_wave[16], s_kept;
-  __shared__ int s_bin, s_at, s_end;
-  const ExpTable& s_exp = sh.exp;
-  exp_table_init(sh.exp);
-  const int r = blockIdx.x, tid = threadIdx.x;
-  const DrawCut& c = a.cut[r];
+// The threshold of a row with a limit, by a workgroup of 1 024: from the lists (of up to `cap` numbers) and the bins' running sums.
+struct CutShared { RadixShared sh; u64 sort[kSorted], thr; double wave[16], kept; int bin, at, end; };
+template <int DT> __device__ __forceinline__ u64 find_threshold(const RowView& v, int n_cols, const DrawCut& c, const u64* la, const u64* lb, unsigned n_b,
+                                                                unsigned cap, const double* cum, const double* excl, CutShared& S) {
+  const int tid = threadIdx.x;
   const float M = c.M;
   const double inv_t = c.inv_t;
   const bool cut_k = c.k_bin < kBins, cut_p = c.p < 1.0;
   u64 thr = 1ull << 32;                             // every allowed entry
-  __syncthreads();                                  // (the table)
-  if (c.any && (cut_k || cut_p)) {
-    const RowView v = row_view<DT>(a, r);
-    const u64* la = a.list_a + (long long)r * a.list_cap;
-    const u64* lb = a.list_b + (long long)r * a.list_cap;
-    const double* cum = (const double*)(a.bin_mass + (long long)r * kBins);
-    const unsigned n_b = a.state[r].n_b;
-    const bool listed_a = c.n_a <= (unsigned)a.list_cap, listed_b = n_b <= (unsigned)a.list_cap;
-    // a list that its entries do not fit into: the row itself, entry by entry
-    const unsigned a0 = c.key[0], a1 = c.key[1];
-    auto src_a = [&](int i) -> u64 {
-      if (listed_a) return la[i];
-      const unsigned k = entry_key<DT>(v, i);
-      return k >= a0 && k < a1 ? number_of(k, i) : 0ull;
-    };
-    const int len_a = listed_a ? (int)c.n_a : a.n_cols;
-    double kept = 0.0;                              // mass of what top-k keeps of its bin
-    bool p_in_a = false;
-    if (cut_k && len_a <= kSorted) {
-      const u64 x = block_sort(tid < len_a ? src_a(tid) : 0ull, len_a, s_sort);
-      if (tid == 0) s_at = (int)c.want - 1;
-      if (tid == (int)c.want - 1) s_thr = x;
-      double incl = 0.0;
-      if (cut_p) {
-        incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, inv_t, s_exp) : 0.0, s_wave);
-        if (tid == (int)c.want - 1) s_kept = incl;
-      }
-      __syncthreads();
-      if (cut_p) {
-        kept = s_kept;
-        const double target = c.p * (c.above_k + kept);
-        p_in_a = target > c.above_k;
-        if (p_in_a) {
-          note_first(&s_at, incl >= target - c.above_k);
-          __syncthreads();
-          if (tid == s_at) s_thr = x;
-          __syncthreads();
-        }
-      }
-      thr = s_thr;
-    } else if (cut_k) {
-      const Numbers<decltype(src_a)> num(src_a, len_a);
-      const u64 thr_k = radix_select(num, false, c.want, 0.0, M, inv_t, sh);
-      thr = thr_k;
-      if (cut_p) {
+  const bool listed_a = c.n_a <= cap, listed_b = n_b <= cap;
+  // a list that its entries do not fit into: the row itself, entry by entry
+  const unsigned a0 = c.key[0], a1 = c.key[1];
+  auto src_a = [&](int i) -> u64 {
+    if (listed_a) return la[i];
+    const unsigned k = entry_key<DT>(v, i);
+    return k >= a0 && k < a1 ? number_of(k, i) : 0ull;
+  };
+  const int len_a = listed_a ? (int)c.n_a : n_cols;
+  double kept = 0.0;                              // mass of what top-k keeps of its bin
+  bool p_in_a = false;
+  if (cut_k && len_a <= kSorted) {
+    const u64 x = block_sort(tid < len_a ? src_a(tid) : 0ull, len_a, S.sort);
+    if (tid == 0) S.at = (int)c.want - 1;
+    if (tid == (int)c.want - 1) S.thr = x;
+    double incl = 0.0;
+    if (cut_p) {
+      incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, inv_t, S.sh.exp) : 0.0, S.wave);
+      if (tid == (int)c.want - 1) S.kept = incl;
+    }
+    __syncthreads();
+    if (cut_p) {
+      kept = S.kept;
+      const double target = c.p * (c.above_k + kept);
+      p_in_a = target > c.above_k;
+      if (p_in_a) {
+        note_first(&S.at, incl >= target - c.above_k);
         __syncthreads();
-        if (tid == 0) { sh.hi = 0ull; sh.lo = 0ull; }
+        if (tid == S.at) S.thr = x;
         __syncthreads();
-        u64 hi = 0ull, lo = 0ull;
-        num.each([&](u64 x) { if (x >= thr_k) { const Fixed f = to_fixed(weight_of(score_of((unsigned)(x >> 32)), M, inv_t, s_exp)); hi += f.hi; lo += f.lo; } });
-        for (int o = 32; o > 0; o >>= 1) { hi += __shfl_xor(hi, o); lo += __shfl_xor(lo, o); }
-        if ((tid & 63) == 0) { atomicAdd(&sh.hi, hi); atomicAdd(&sh.lo, lo); }
-        __syncthreads();
-        kept = fixed_d(sh.hi, sh.lo);
-        const double target = c.p * (c.above_k + kept);
-        p_in_a = target > c.above_k;
-        if (p_in_a) {
-          auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
-          thr = radix_select(Numbers<decltype(src)>(src, len_a), true, 0u, target - c.above_k, M, inv_t, sh);
-        }
       }
     }
-    if (cut_p && !p_in_a && c.p_hi >= 0) {
-      const double target = c.p * (cut_k ? c.above_k + kept : c.total);
-      // first bin of [p_lo, p_hi] whose running sum reaches the target (empty ones hold -1; p_hi is not empty)
-      if (tid == 0) s_bin = c.p_hi;
+    thr = S.thr;
+  } else if (cut_k) {
+    const Numbers<decltype(src_a)> num(src_a, len_a);
+    const u64 thr_k = radix_select(num, false, c.want, 0.0, M, inv_t, S.sh);
+    thr = thr_k;
+    if (cut_p) {
       __syncthreads();
-      for (int j = c.p_lo + tid; j < c.p_hi; j += 1024) if (cum[j] >= target) atomicMin(&s_bin, j);
+      if (tid == 0) { S.sh.hi = 0ull; S.sh.lo = 0ull; }
       __syncthreads();
-      const int bin = s_bin;
-      Binning b;
-      b.M = M; b.scale = c.scale;
-      const unsigned b0 = c.key[2], b1 = c.key[3];
-      auto src = [&](int i) -> u64 {
-        u64 x = 0ull;
-        if (listed_b) x = lb[i];
-        else { const unsigned k = entry_key<DT>(v, i); if (k >= b0 && k < b1) x = number_of(k, i); }
-        return x && bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
-      };
-      const double before = a.bin_excl[(long long)r * kBins + bin];
-      const int len_b = listed_b ? (int)n_b : a.n_cols;
-      u64 t;
-      if (len_b <= kSorted) {
-        const u64 x = block_sort(tid < len_b ? src(tid) : 0ull, len_b, s_sort);
-        const double incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, inv_t, s_exp) : 0.0, s_wave);
-        // (none reaches it, by rounding: the last one)
-        if (tid == 0) { s_at = kSorted; s_end = 0; }
-        __syncthreads();
-        note_first(&s_at, x && incl >= target - before);
-        note_last(&s_end, x != 0ull);
-        __syncthreads();
-        if (tid == min(s_at, s_end)) s_thr = x;
-        __syncthreads();
-        t = s_thr;
-      } else t = radix_select(Numbers<decltype(src)>(src, len_b), true, 0u, target - before, M, inv_t, sh);
-      if (t > thr) thr = t;                         // (an empty source gives 0)
+      u64 hi = 0ull, lo = 0ull;
+      num.each([&](u64 x) { if (x >= thr_k) { const Fixed f = to_fixed(weight_of(score_of((unsigned)(x >> 32)), M, inv_t, S.sh.exp)); hi += f.hi; lo += f.lo; } });
+      for (int o = 32; o > 0; o >>= 1) { hi += __shfl_xor(hi, o); lo += __shfl_xor(lo, o); }
+      if ((tid & 63) == 0) { atomicAdd(&S.sh.hi, hi); atomicAdd(&S.sh.lo, lo); }
+      __syncthreads();
+      kept = fixed_d(S.sh.hi, S.sh.lo);
+      const double target = c.p * (c.above_k + kept);
+      p_in_a = target > c.above_k;
+      if (p_in_a) {
+        auto src = [&](int i) -> u64 { const u64 x = src_a(i); return x >= thr_k ? x : 0ull; };
+        thr = radix_select(Numbers<decltype(src)>(src, len_a), true, 0u, target - c.above_k, M, inv_t, S.sh);
+      }
     }
   }
-  if (tid == 0) {
+  if (cut_p && !p_in_a && c.p_hi >= 0) {
+    const double target = c.p * (cut_k ? c.above_k + kept : c.total);
+    // first bin of [p_lo, p_hi] whose running sum reaches the target (empty ones hold -1; p_hi is not empty)
+    if (tid == 0) S.bin = c.p_hi;
+    __syncthreads();
+    for (int j = c.p_lo + tid; j < c.p_hi; j += 1024) if (cum[j] >= target) atomicMin(&S.bin, j);
+    __syncthreads();
+    const int bin = S.bin;
+    Binning b;
+    b.M = M; b.scale = c.scale;
+    const unsigned b0 = c.key[2], b1 = c.key[3];
+    auto src = [&](int i) -> u64 {
+      u64 x = 0ull;
+      if (listed_b) x = lb[i];
+      else { const unsigned k = entry_key<DT>(v, i); if (k >= b0 && k < b1) x = number_of(k, i); }
+      return x && bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
+    };
+    const double before = excl[bin];
+    const int len_b = listed_b ? (int)n_b : n_cols;
+    u64 t;
+    if (len_b <= kSorted) {
+      const u64 x = block_sort(tid < len_b ? src(tid) : 0ull, len_b, S.sort);
+      const double incl = block_running(x ? weight_of(score_of((unsigned)(x >> 32)), M, inv_t, S.sh.exp) : 0.0, S.wave);
+      // (none reaches it, by rounding: the last one)
+      if (tid == 0) { S.at = kSorted; S.end = 0; }
+      __syncthreads();
+      note_first(&S.at, x && incl >= target - before);
+      note_last(&S.end, x != 0ull);
+      __syncthreads();
+      if (tid == min(S.at, S.end)) S.thr = x;
+      __syncthreads();
+      t = S.thr;
+    } else t = radix_select(Numbers<decltype(src)>(src, len_b), true, 0u, target - before, M, inv_t, S.sh);
+    if (t > thr) thr = t;                         // (an empty source gives 0)
+  }
+  return thr;
+}
+template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
+  __shared__ CutShared S;
+  exp_table_init(S.sh.exp);
+  const int r = blockIdx.x;
+  const DrawCut& c = a.cut[r];
+  __syncthreads();
+  u64 thr = 1ull << 32;
+  if (c.any && (c.k_bin < kBins || c.p < 1.0))
+    thr = find_threshold<DT>(row_view<DT>(a, r), a.n_cols, c, a.list_a + (long long)r * a.list_cap, a.list_b + (long long)r * a.list_cap, a.state[r].n_b,
+                             (unsigned)a.list_cap, (const double*)(a.bin_mass + (long long)r * kBins), a.bin_excl + (long long)r * kBins, S);
+  if (threadIdx.x == 0) {
     DrawState* o = a.state + r;
-    o->thr = thr; o->M = M; o->any = c.any; o->inv_t = inv_t; o->m = row_par(a, r).m;
+    o->thr = thr; o->M = c.M; o->any = c.any; o->inv_t = c.inv_t; o->m = row_par(a, r).m;
   }
 }
 
@@ -932,6 +948,142 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
   }
 }
 
+// ---------------------------------------------------------------- short rows: everything by one workgroup
+// The same steps with the row in registers (up to 16 entries to a thread), all else in LDS: one launch instead of seven,
+// whose starts and first loads are what a short row costs (1 x 2 048: 32 us in seven, 13 us in one).
+constexpr int kRowCols = 16384, kRowList = 1024;
+struct RowShared {
+  union { unsigned cnt[kBins]; double running[kBins]; };          // bin counts, later the blocks' running sums (kRowCols / kBlock = kBins)
+  union { u64 mass[kBins]; double cum[kBins]; };
+  union { double first[kBins]; double excl[kBins]; };
+  u64 la[kRowList], lb[kRowList];
+  unsigned short kept[kBins];
+  CutShared cut;
+  BinsShared bins;
+  DrawCut c;
+  unsigned n_a, n_b;
+};
+static_assert(sizeof(RowShared) <= 65536, "LDS");
+template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a) {
+  __shared__ RowShared S;
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const RowView v = row_view<DT>(a, r);
+  const RowPar par = row_par(a, r);
+  exp_table_init(S.cut.sh.exp);
+  Four<DT> f[4];
+  unsigned mx = 0u, mn = 0xffffffffu;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[j].live = 0u;
+    const int i = j * 4096 + tid * 4;
+    if (i < a.n_cols) f[j] = load_four<DT>(v, i, a.n_cols);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) { const unsigned k = four_key(f[j], q); mx = max(mx, k); mn = min(mn, k ? k : 0xffffffffu); }
+  }
+  for (int o = 32; o > 0; o >>= 1) { mx = max(mx, (unsigned)__shfl_xor((int)mx, o)); mn = min(mn, (unsigned)__shfl_xor((int)mn, o)); }
+  if (lane == 0) { S.cut.sh.mx[tid >> 6] = mx; S.cut.sh.mn[tid >> 6] = mn; }
+  S.cnt[tid] = 0u; S.mass[tid] = 0ull;
+  if (tid == 0) { S.n_a = 0u; S.n_b = 0u; }
+  __syncthreads();
+  for (int j = 0; j < 16; ++j) { mx = max(mx, (unsigned)S.cut.sh.mx[j]); mn = min(mn, (unsigned)S.cut.sh.mn[j]); }
+  const long long out0 = (long long)r * a.n_draws;
+  if (!mx) {
+    for (int d = tid; d < a.n_draws; d += 1024) { a.idx[out0 + d] = -1; if (a.prob) a.prob[out0 + d] = 0.f; }
+    return;
+  }
+  const float M = score_of(mx);
+  u64 thr = 1ull << 32;
+  if (has_cut(par)) {
+    const Range g{mx, mn};
+    const Binning b = make_binning(g, par.inv_t, a.n_cols);
+    const bool weigh = par.p < 1.0, count = par.k > 0;
+    if (weigh) S.first[tid] = first_weight(b, tid);
+    __syncthreads();
+    const BinPoly poly = make_bin_poly();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) add_to_bins(f[j], b, poly, count, weigh, S.cnt, S.mass, S.first);
+    __syncthreads();
+    const unsigned c = S.cnt[tid];
+    const double m = ldexp((double)S.mass[tid], -bin_shift(b, tid));
+    __syncthreads();
+    find_bins(a, par, g, b, c, m, S.cum, S.excl, &S.c, S.bins);
+    __syncthreads();
+    const DrawCut& cut = S.c;
+    if (cut.k_bin < kBins || cut.p < 1.0) {
+      const bool do_a = cut.k_bin < kBins && cut.n_a <= kRowList, do_b = cut.p_hi >= 0;
+      const unsigned a0 = do_a ? cut.key[0] : 1u, a1 = do_a ? cut.key[1] : 0u, b0 = do_b ? cut.key[2] : 1u, b1 = do_b ? cut.key[3] : 0u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const unsigned k = four_key(f[j], q);
+          const int i = j * 4096 + tid * 4 + q;
+          if (k >= a0 && k < a1) { const unsigned at = atomicAdd(&S.n_a, 1u); if (at < kRowList) S.la[at] = number_of(k, i); }
+          if (k >= b0 && k < b1) { const unsigned at = atomicAdd(&S.n_b, 1u); if (at < kRowList) S.lb[at] = number_of(k, i); }
+        }
+      __syncthreads();
+      thr = find_threshold<DT>(v, a.n_cols, cut, S.la, S.lb, S.n_b, kRowList, S.cum, S.excl, S.cut);
+    }
+    __syncthreads();
+  }
+  // Running sums at the end of each block of 16 entries, and which of them are kept.  The row is read once more: its
+  // registers held through the search above would spill.
+  const Kept kp = kept_from(thr);
+  const double least = fmax(par.m, 0x1p-1074);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    f[j].live = 0u;
+    if (j * 4096 + tid * 4 < a.n_cols) f[j] = load_four<DT>(v, j * 4096 + tid * 4, a.n_cols);
+    double w = 0.0;
+    unsigned bits = 0u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (((f[j].live >> q) & 1u) && is_kept(f[j].s[q], j * 4096 + tid * 4 + q, kp)) {
+        const double x = weight_of(f[j].s[q], M, par.inv_t, S.cut.sh.exp);
+        if (x >= least) { w += x; bits |= 1u << q; }
+      }
+    bits <<= 4 * (lane & 3);
+    w += __shfl_xor(w, 1);
+    w += __shfl_xor(w, 2);
+    bits |= (unsigned)__shfl_xor((int)bits, 1);
+    bits |= (unsigned)__shfl_xor((int)bits, 2);
+    if ((tid & 3) == 0) { S.running[j * 256 + (tid >> 2)] = w; S.kept[j * 256 + (tid >> 2)] = (unsigned short)bits; }
+  }
+  __syncthreads();
+  const double incl = block_running(S.running[tid], S.cut.wave);
+  S.running[tid] = incl;
+  __syncthreads();
+  const double total = S.running[kBins - 1];
+  const int last_block = (a.n_cols + kBlock - 1) / kBlock - 1;
+  for (int d = tid; d < a.n_draws; d += 1024) {
+    double u = (double)a.u[(long long)r * a.u_stride + d];
+    u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
+    const double target = u * total;
+    int lo = 0, hi = last_block;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (S.running[mid] > target) hi = mid; else lo = mid + 1; }
+    double in_block = target - (lo ? S.running[lo - 1] : 0.0);
+    unsigned kept = S.kept[lo];
+    if (!kept) {
+      // the target lies within rounding of a border: the first kept entry behind it, or the last before
+      while (!kept && lo < last_block) kept = S.kept[++lo];
+      while (!kept && lo > 0) kept = S.kept[--lo];
+      in_block = -1.0;
+    }
+    double acc = 0.0, w_at = 0.0;
+    int at = -1;
+    while (kept) {
+      const int j = __ffs((int)kept) - 1;
+      kept &= kept - 1u;
+      w_at = weight_of(load_score<DT>(v.s, lo * kBlock + j), M, par.inv_t, S.cut.sh.exp);
+      at = lo * kBlock + j;
+      acc += w_at;
+      if (acc > in_block) break;
+    }
+    a.idx[out0 + d] = at;
+    if (a.prob) a.prob[out0 + d] = (float)(w_at / total);
+  }
+}
+
 // ---------------------------------------------------------------- host side
 struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, group, group_incl, part_max, part_min, bin_cnt, bin_mass, bin_excl, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
@@ -970,6 +1122,11 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   return l;
 }
 template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
+  // short rows in one launch; many draws want more than one workgroup
+  if (a.n_cols <= kRowCols && a.n_draws <= 4096) {
+    hipLaunchKernelGGL(k_draw_row<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
+    return;
+  }
   hipLaunchKernelGGL(k_draw_range<DT>, dim3(a.n_parts, a.n_rows), dim3(256), 0, s, a);
   if (a.cuts) {
     hipLaunchKernelGGL(k_draw_hist<DT>, dim3(a.n_parts, a.n_rows), dim3(512), 0, s, a);
