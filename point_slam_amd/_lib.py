@@ -235,3 +235,16 @@ def ptr(t):
 def stream_ptr():
     import torch
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def call_on(device, entry: str, args):
+    """entry(args, the current stream of `device`) with that device current: tensors may live on another device than the
+    current one.  The raw stream is asked for directly; a torch.cuda.Stream object per call costs as much as a launch."""
+    import torch
+    fn = getattr(lib(), entry)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if device.index is None or device.index == torch.cuda.current_device():
+        stream = raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream
+        return check(fn(C.byref(args), stream), entry)
+    with torch.cuda.device(device):
+        return check(fn(C.byref(args), torch.cuda.current_stream().cuda_stream), entry)

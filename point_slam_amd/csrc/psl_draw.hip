@@ -49,7 +49,6 @@ struct DrawCut {
   float scale; unsigned want;      // bins per unit of score; entries of k_bin that top-k keeps
   int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
   unsigned n_a;                    // entries of k_bin
-  unsigned key[4];                 // keys of k_bin: [0] .. [1] - 1; of [p_lo, p_hi]: [2] .. [3] - 1
   double above_k, total;           // mass of the bins before k_bin; of all
 };
 
@@ -312,16 +311,6 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   }
 }
 
-// smallest key of the row whose bin is at most `bin` (bins fall as keys rise; the row's largest key is in bin 0)
-__device__ __forceinline__ unsigned first_key(const Binning& b, const Range& g, int bin) {
-  unsigned lo = g.mn, hi = g.mx;
-  while (lo < hi) {
-    const unsigned mid = lo + ((hi - lo) >> 1);
-    if (bin_of(b, score_of(mid)) <= bin) hi = mid; else lo = mid + 1;
-  }
-  return lo;
-}
-
 // smallest / largest thread of the workgroup for which a condition holds: a ballot per wavefront, then one LDS atomic each
 // (an atomic per thread to one address is run lane by lane)
 __device__ __forceinline__ void note_first(int* at, bool cond) {
@@ -379,10 +368,6 @@ __device__ __forceinline__ void find_bins(const DrawArgs& a, const RowPar& par, 
   }
   __syncthreads();
   const int p_lo = cut_p ? min(sh.lo, sh.last) : 0, p_hi = cut_p ? min(sh.hi, sh.last) : -1;
-  if (j < 4) {
-    const int bin = j == 0 ? k_bin : j == 1 ? k_bin - 1 : j == 2 ? p_hi : p_lo - 1;
-    o->key[j] = bin < 0 ? g.mx + 1u : first_key(b, g, bin);
-  }
   if (j == 64) {
     o->want = sh.want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = sh.na; o->above_k = above_k; o->total = total;
   }
@@ -400,9 +385,8 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
   find_bins(a, par, g, b, c, m, (double*)(a.bin_mass + (long long)r * kBins), a.bin_excl + (long long)r * kBins, a.cut + r, sh);
 }
 
-// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.  A bin
-// is an interval of keys: an entry costs integer comparisons only.  A workgroup collects in LDS and asks once for its
-// places in the row's list (a global atomic for every wavefront that found something made this 112 us for twelve rows of
+// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.  A
+// workgroup collects in LDS and asks once for its places in the row's list (a global atomic for every wavefront that found something made this 112 us for twelve rows of
 // 816 000); what does not fit there goes to the list by itself.
 constexpr int kListBuf = 1024;
 struct ListBuf { u64 e[kListBuf]; unsigned n, at; };
@@ -417,8 +401,9 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
   const DrawCut& c = a.cut[r];
   const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.p_hi >= 0;
   if (!do_a && !do_b) return;
-  // (no such bin: an empty interval)
-  const unsigned a0 = do_a ? c.key[0] : 1u, a1 = do_a ? c.key[1] : 0u, b0 = do_b ? c.key[2] : 1u, b1 = do_b ? c.key[3] : 0u;
+  Binning b;
+  b.M = c.M; b.scale = c.scale;
+  const int ka = do_a ? c.k_bin : -1, p0 = do_b ? c.p_lo : 0, p1 = do_b ? c.p_hi : -1;      // (no such bin: an empty interval)
   if (tid == 0) { buf_a.n = 0u; buf_b.n = 0u; }
   __syncthreads();
   const RowView v = row_view<DT>(a, r);
@@ -431,9 +416,12 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
     const Four<DT> f = load_four<DT>(v, i, i1);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const unsigned k = four_key(f, q);
-      if (k >= a0 && k < a1) list_add(buf_a, number_of(k, i + q), la, &a.state[r].n_a, cap);
-      if (k >= b0 && k < b1) list_add(buf_b, number_of(k, i + q), lb, &a.state[r].n_b, cap);
+      const float x = f.s[q];
+      if (((f.live >> q) & 1u) && x > -__builtin_inff()) {
+        const int bin = bin_of(b, x);
+        if (bin == ka) list_add(buf_a, number_of(key_of(x), i + q), la, &a.state[r].n_a, cap);
+        if (bin >= p0 && bin <= p1) list_add(buf_b, number_of(key_of(x), i + q), lb, &a.state[r].n_b, cap);
+      }
     }
   }
   __syncthreads();
@@ -625,12 +613,13 @@ template <int DT> __device__ __forceinline__ u64 find_threshold(const RowView& v
   u64 thr = 1ull << 32;                             // every allowed entry
   const bool listed_a = c.n_a <= cap, listed_b = n_b <= cap;
   // a list that its entries do not fit into: the row itself, entry by entry
-  const unsigned a0 = c.key[0], a1 = c.key[1];
-  auto src_a = [&](int i) -> u64 {
-    if (listed_a) return la[i];
+  Binning b;
+  b.M = M; b.scale = c.scale;
+  auto from_row = [&](int i, int bin) -> u64 {
     const unsigned k = entry_key<DT>(v, i);
-    return k >= a0 && k < a1 ? number_of(k, i) : 0ull;
+    return k && bin_of(b, score_of(k)) == bin ? number_of(k, i) : 0ull;
   };
+  auto src_a = [&](int i) -> u64 { return listed_a ? la[i] : from_row(i, c.k_bin); };
   const int len_a = listed_a ? (int)c.n_a : n_cols;
   double kept = 0.0;                              // mass of what top-k keeps of its bin
   bool p_in_a = false;
@@ -686,14 +675,10 @@ template <int DT> __device__ __forceinline__ u64 find_threshold(const RowView& v
     for (int j = c.p_lo + tid; j < c.p_hi; j += 1024) if (cum[j] >= target) atomicMin(&S.bin, j);
     __syncthreads();
     const int bin = S.bin;
-    Binning b;
-    b.M = M; b.scale = c.scale;
-    const unsigned b0 = c.key[2], b1 = c.key[3];
     auto src = [&](int i) -> u64 {
-      u64 x = 0ull;
-      if (listed_b) x = lb[i];
-      else { const unsigned k = entry_key<DT>(v, i); if (k >= b0 && k < b1) x = number_of(k, i); }
-      return x && bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
+      if (!listed_b) return from_row(i, bin);
+      const u64 x = lb[i];
+      return bin_of(b, score_of((unsigned)(x >> 32))) == bin ? x : 0ull;
     };
     const double before = excl[bin];
     const int len_b = listed_b ? (int)n_b : n_cols;
@@ -1011,15 +996,15 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a)
     const DrawCut& cut = S.c;
     if (cut.k_bin < kBins || cut.p < 1.0) {
       const bool do_a = cut.k_bin < kBins && cut.n_a <= kRowList, do_b = cut.p_hi >= 0;
-      const unsigned a0 = do_a ? cut.key[0] : 1u, a1 = do_a ? cut.key[1] : 0u, b0 = do_b ? cut.key[2] : 1u, b1 = do_b ? cut.key[3] : 0u;
+      const int ka = do_a ? cut.k_bin : -1, p0 = do_b ? cut.p_lo : 0, p1 = do_b ? cut.p_hi : -1;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const unsigned k = four_key(f[j], q);
-          const int i = j * 4096 + tid * 4 + q;
-          if (k >= a0 && k < a1) { const unsigned at = atomicAdd(&S.n_a, 1u); if (at < kRowList) S.la[at] = number_of(k, i); }
-          if (k >= b0 && k < b1) { const unsigned at = atomicAdd(&S.n_b, 1u); if (at < kRowList) S.lb[at] = number_of(k, i); }
+          const int i = j * 4096 + tid * 4 + q, bin = k ? bin_of(b, score_of(k)) : -2;
+          if (bin == ka) { const unsigned at = atomicAdd(&S.n_a, 1u); if (at < kRowList) S.la[at] = number_of(k, i); }
+          if (bin >= p0 && bin <= p1) { const unsigned at = atomicAdd(&S.n_b, 1u); if (at < kRowList) S.lb[at] = number_of(k, i); }
         }
       __syncthreads();
       thr = find_threshold<DT>(v, a.n_cols, cut, S.la, S.lb, S.n_b, kRowList, S.cum, S.excl, S.cut);

@@ -78,7 +78,6 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     if u.dim() != 2 or u.dtype != torch.float32 or u.shape[0] != R or u.device != dev:
         raise ValueError(f"u: float32 [{R}, draws] on {dev}, got {tuple(u.shape)} {u.dtype} on {u.device}")
     n = u.shape[1]
-    scores, u = scores.detach(), u.detach()
     if V > 1 and scores.stride(1) != 1:
         scores = scores.contiguous()
     if n > 1 and u.stride(1) != 1:
@@ -88,7 +87,6 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     if mask is not None:
         if mask.dtype not in (torch.bool, torch.uint8) or mask.device != dev or tuple(mask.shape) not in ((R, V), (V,)):
             raise ValueError(f"mask: bool or uint8 [{R}, {V}] or [{V}] on {dev}, got {tuple(mask.shape)} {mask.dtype} on {mask.device}")
-        mask = mask.detach()
         mask = mask.expand(R, V)
         if V > 1 and mask.stride(1) != 1:
             mask = mask.contiguous()
@@ -99,7 +97,7 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
         if torch.is_tensor(x):
             if tuple(x.shape) != (R,) or x.device != dev or x.dtype != dt:
                 raise ValueError(f"{name}: a number or {dt} [{R}] on {dev}, got {tuple(x.shape)} {x.dtype} on {x.device}")
-            x = x.detach().contiguous()
+            x = x.contiguous()
             keep.append(x)
             setattr(a, name, x.data_ptr())
         elif name == "top_k":
@@ -113,12 +111,10 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     idx = torch.empty(R, n, dtype=torch.int32, device=dev)
     prob = torch.empty(R, n, dtype=torch.float32, device=dev) if with_prob else None
     if R and n:
-        L = _lib.lib()
-        with torch.cuda.device(dev):
-            a.ws_bytes = _lib.check(L.psl_draw_ws_bytes(R, V), "psl_draw_ws_bytes")
-            ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
-            a.idx, a.prob, a.ws = idx.data_ptr(), prob.data_ptr() if with_prob else None, ws.data_ptr()
-            _lib.check(L.psl_draw_indices(C.byref(a), _lib.stream_ptr()), "psl_draw_indices")
+        a.ws_bytes = _lib.check(_lib.lib().psl_draw_ws_bytes(R, V), "psl_draw_ws_bytes")
+        ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
+        a.idx, a.prob, a.ws = idx.data_ptr(), prob.data_ptr() if with_prob else None, ws.data_ptr()
+        _lib.call_on(dev, "psl_draw_indices", a)
     if one:
         idx, prob = idx[0], prob[0] if with_prob else None
     return (idx, prob) if with_prob else idx

@@ -14,7 +14,6 @@ There is no torch fallback.
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import Optional
 
 import torch
@@ -45,8 +44,7 @@ def _call(entry, values, rows, first, n, fmt, group, capacity, codes, codes_row_
                            value_row_stride=values.stride(0), value_head_stride=values.stride(1), codes=codes.data_ptr(),
                            codes_row_stride=codes_row_stride, scales=scales.data_ptr(), scales_row_stride=scales_row_stride,
                            owner=None if owner is None else owner.data_ptr())
-    with torch.cuda.device(values.device):       # the launch belongs to the tensors' device and its current stream
-        _lib.check(getattr(_lib.lib(), entry)(C.byref(a), _lib.stream_ptr()), entry)
+    _lib.call_on(values.device, entry, a)
 
 
 def record_floats(heads: int, dim: int, fmt: str, group: Optional[int] = None) -> tuple:
@@ -129,8 +127,7 @@ class QuantizedRows:
         if values.device != self.device:
             raise ValueError(f"values on {values.device}, the store on {self.device}")
         n = values.shape[0]
-        values = values.detach()
-        if values.stride(2) != 1 or min(values.stride()) < 0:
+        if values.stride(2) != 1:
             values = values.contiguous()
         owner = None
         if rows is None:
