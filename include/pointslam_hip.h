@@ -361,7 +361,8 @@ int psl_keyframe_overlap_sync(const float* rays_o, const float* rays_d, const fl
  *                    (padding: -1).  The same id more than once: with `owner` ([capacity] int32 scratch, any contents) the
  *                    largest i wins; with owner NULL the caller vouches that the ids are distinct.
  *   psl_rows_read  : the values of row rows[i] -> values[i], rounded once to dtype; ids outside [0, capacity) give zeros.
- * Rows that are not named stay as they were.  heads, dim <= 4096; group <= 1024 divides dim (even for int4). */
+ * Rows that are not named stay as they were.  heads, dim <= 4096; group <= 1024 divides dim (even for int4);
+ * n, capacity < 2^31; strides up to 2^29.  The codes of a group with scale NaN mean nothing. */
 enum psl_dtype { PSL_F32 = 0, PSL_BF16 = 1, PSL_F16 = 2 };
 enum psl_row_format { PSL_ROWS_INT8 = 0, PSL_ROWS_E4M3 = 1, PSL_ROWS_INT4 = 2 };
 typedef struct psl_rows_args {

@@ -3,9 +3,10 @@
 // A row is heads x dim values, cut into groups of G; a group shares one fp32 scale s = max|x| / Q (Q = 127 int8, 7 int4,
 // 448 e4m3) and every code is the NEAREST representable value to x / s, ties to even.  fp32's x / s cannot decide that by
 // itself: it rounds quotients beside the middle between two codes onto it (with bf16 inputs x = a / 2 that happens in
-// every few rows).  The quotient is therefore rounded to ODD: truncated, its last bit set when the residual
-// x - q s is not zero (one fma gives the residual's exact sign).  Rounding that 24-bit value once more to 8 bits or fewer is
-// then the rounding of the exact quotient.
+// every few rows).  What decides is the residual x - n s, which one fma gives exactly:
+//   integers: n = rint(x / s), and x - n s against s / 2 says whether n is the nearest (it nearly always is);
+//   e4m3: the quotient rounded to ODD -- truncated, its last bit set when the residual is not zero.  Rounding that 24-bit value
+//   once more, to four bits, is the rounding of the exact quotient.
 //
 // Bound: memory.  A thread owns VEC consecutive values; the L lanes of a group find its maximum with L-lane shuffles, so a
 // value is read once and lives in registers until its code is stored.
@@ -32,12 +33,13 @@ __device__ __forceinline__ unsigned fast_div(unsigned x, const FastDiv& f) { ret
 struct RowsArgs {
   const void* rows;        // destination / source row ids, or NULL: first + i
   long long first, capacity, i0;      // i0: first row of this launch (launches cover < 2^31 groups each)
-  char* values; long long vrow, vhead;          // bytes
-  unsigned char* codes; long long crow;         // bytes per row; a head holds dim * bits / 8
-  float* scales; long long srow;                // floats per row
+  char* values; unsigned vrow, vhead;           // bytes
+  unsigned char* codes; unsigned crow;          // bytes per row; a head holds dim * bits / 8
+  float* scales; unsigned srow;                 // floats per row
   const int* owner;        // write: row -> last i that writes it (NULL: the rows are distinct)
   unsigned n;              // rows of this launch
-  int heads, dim, group, chunks;                // chunks = group / VEC
+  unsigned group, chunks;                       // values of a group; chunks = group / VEC
+  bool heads_apart;                             // the heads of a row of values do not follow one another
   int lanes_log2;          // lanes that share a group
   FastDiv groups_per_row, groups_per_head;
   int rows_bits;           // 32 | 64
@@ -130,16 +132,51 @@ template <int FMT> struct Code {
   static constexpr float top = FMT == PSL_ROWS_INT8 ? 127.f : FMT == PSL_ROWS_INT4 ? 7.f : 448.f;
 };
 
-// x / s rounded to odd, sign carried; s > 0, xs = x * f and ss = s * f with the power of two f that keeps the residual normal
-__device__ __forceinline__ float quotient_odd(float xs, float ss, float inv) {
-  const float ax = fabsf(xs);
+// x / s rounded to odd, sign carried (s > 0, inv = 1 / s to a few units of the last place, the residual not denormal)
+__device__ __forceinline__ float quotient_odd(float x, float s, float inv) {
+  const float ax = fabsf(x);
   const float q0 = ax * inv;
-  const float q = fmaf(fmaf(-q0, ss, ax), inv, q0);      // within one unit of the last place of the exact quotient
-  const float e = fmaf(-q, ss, ax);                      // its exact remainder's sign
+  const float q = fmaf(fmaf(-q0, s, ax), inv, q0);       // within one unit of the last place of the exact quotient
+  const float e = fmaf(-q, s, ax);                       // its exact remainder's sign
   unsigned b = __float_as_uint(q);
   b -= (e < 0.f) ? 1u : 0u;
   b |= (e != 0.f) ? 1u : 0u;
-  return copysignf(__uint_as_float(b), xs);
+  return copysignf(__uint_as_float(b), x);
+}
+
+// codes of VEC values, as the numbers they are (integers; e4m3: rounded to odd, the conversion does the rest)
+template <int FMT, int VEC> __device__ __forceinline__ void quotients(const float (&x)[VEC], float s, float inv, float (&q)[VEC]) {
+  if constexpr (FMT == PSL_ROWS_E4M3) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) q[k] = quotient_odd(x[k], s, inv);
+  } else {
+    float far = -1.f;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      q[k] = rintf(x[k] * inv);
+      const float r = fmaf(-q[k], s, x[k]);              // exact: a multiple of the smaller last place, below s
+      far = fmaxf(far, fmaf(2.f, fabsf(r), -s));         // above 0: a neighbour is nearer; 0: a tie
+    }
+    if (far >= 0.f) {
+      asm volatile("");            // (a branch: rarely taken)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const float r = fmaf(-q[k], s, x[k]), h = fmaf(2.f, fabsf(r), -s);
+        if (h > 0.f || (h == 0.f && ((int)q[k] & 1))) q[k] += copysignf(1.f, r);
+      }
+    }
+  }
+}
+// the same where the largest value is below 2^-60: scaled by 2^80, so that residuals are not denormal; a scale in the
+// denormals is coarse, and the quotient may pass the largest code
+template <int FMT, int VEC> __device__ __forceinline__ void quotients_tiny(const float (&x)[VEC], float s, float (&q)[VEC]) {
+  constexpr float f = 0x1p80f;
+  const float ss = s * f, inv = 1.f / ss;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const float y = fminf(fmaxf(quotient_odd(x[k] * f, ss, inv), -Code<FMT>::top), Code<FMT>::top);
+    q[k] = s > 0.f ? (FMT == PSL_ROWS_E4M3 ? y : rintf(y)) : 0.f;
+  }
 }
 
 template <int FMT, int VEC> __device__ __forceinline__ void encode(const float (&q)[VEC], unsigned char* dst) {
@@ -161,7 +198,7 @@ template <int FMT, int VEC> __device__ __forceinline__ void encode(const float (
     for (int k = 0; k < VEC / PER; ++k) {
       unsigned w = 0;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) w |= ((unsigned)(int)rintf(q[k * PER + j]) & ((1u << B) - 1u)) << (B * j);
+      for (int j = 0; j < PER; ++j) w |= ((unsigned)(int)q[k * PER + j] & ((1u << B) - 1u)) << (B * j);
       r.w[k] = w;
     }
   }
@@ -189,18 +226,26 @@ template <int FMT, int VEC> __device__ __forceinline__ void decode(const unsigne
   }
 }
 
-// the group's place: row i, its row id, head, offset of the group inside the head
-struct Place { long long i, row; int head, g; };
+// the place of group `unit`: row i of the call (inside this launch), row of the store (-1: none), group u of the row.  Codes and
+// scales of a row's groups lie one behind the other; 32 x 32 -> 64 bit products reach every address.
+struct Place { unsigned i, u; int row; };
 __device__ __forceinline__ Place place_of(const RowsArgs& a, unsigned unit) {
   Place p;
-  const unsigned i = fast_div(unit, a.groups_per_row);
-  const unsigned u = unit - i * a.groups_per_row.d;
-  p.head = (int)fast_div(u, a.groups_per_head);
-  p.g = (int)(u - (unsigned)p.head * a.groups_per_head.d);
-  p.i = a.i0 + i;
-  p.row = row_of(a, p.i);
+  p.i = fast_div(unit, a.groups_per_row);
+  p.u = unit - p.i * a.groups_per_row.d;
+  p.row = (int)row_of(a, a.i0 + p.i);
   return p;
 }
+__device__ __forceinline__ char* values_at(const RowsArgs& a, const Place& p, unsigned es) {
+  char* v = a.values + (unsigned long long)p.i * a.vrow;
+  if (!a.heads_apart) return v + p.u * a.group * es;
+  const unsigned head = fast_div(p.u, a.groups_per_head);
+  return v + (unsigned long long)head * a.vhead + (p.u - head * a.groups_per_head.d) * a.group * es;
+}
+template <int BITS> __device__ __forceinline__ unsigned char* codes_at(const RowsArgs& a, const Place& p) {
+  return a.codes + (unsigned long long)(unsigned)p.row * a.crow + (p.u * a.group * BITS >> 3);
+}
+__device__ __forceinline__ float* scale_at(const RowsArgs& a, const Place& p) { return a.scales + (unsigned long long)(unsigned)p.row * a.srow + p.u; }
 
 // The last of several i with the same row wins: clear the rows' entries, then keep the largest i (two launches: a maximum
 // does not depend on the order of the atomics).
@@ -218,59 +263,57 @@ __global__ __launch_bounds__(256) void k_rows_owner_claim(RowsArgs a, int* __res
 }
 
 // ITERS chunks of a group per lane (lane, lane + L, ...), held in registers between the maximum and the codes
+template <int CTRL> __device__ __forceinline__ unsigned max_dpp(unsigned x) {
+  return max(x, (unsigned)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true));
+}
+// maximum over the 2^k lanes of a group (aligned to them)
+__device__ __forceinline__ unsigned group_max(unsigned x, int k) {
+  if (k > 0) x = max_dpp<0xb1>(x);        // quad_perm 1 0 3 2
+  if (k > 1) x = max_dpp<0x4e>(x);        // quad_perm 2 3 0 1
+  if (k > 2) x = max_dpp<0x141>(x);       // row_half_mirror: the other four of eight, which agree by now
+  if (k > 3) x = max_dpp<0x140>(x);       // row_mirror: the other eight of sixteen
+  if (k > 4) x = max(x, (unsigned)__shfl_xor((int)x, 16));
+  if (k > 5) x = max(x, (unsigned)__shfl_xor((int)x, 32));
+  return x;
+}
+
 template <int FMT, int DT, int VEC, int ITERS>
 __global__ __launch_bounds__(256) void k_rows_write(RowsArgs a) {
-  const unsigned long long t = (unsigned long long)blockIdx.x * 256 + threadIdx.x;
-  const unsigned long long unit64 = t >> a.lanes_log2;
-  // whole wavefronts stay for the shuffles; a group's lanes are in range together
-  const bool in = unit64 < (unsigned long long)a.n * a.groups_per_row.d;
-  const Place p = in ? place_of(a, (unsigned)unit64) : Place{0, -1, 0, 0};
-  const int L = 1 << a.lanes_log2, lane = (int)(t & (unsigned)(L - 1));
-  const bool live = p.row >= 0 && !(a.owner && a.owner[p.row] != (int)p.i);
+  const unsigned t = blockIdx.x * 256u + threadIdx.x;
+  const unsigned unit = t >> a.lanes_log2;
+  // Whole wavefronts stay for the maximum; a group's lanes are in range together.  Lanes without a group read the first
+  // one's values, lanes without a chunk their group's last: what they add to a maximum is in it already or not used.
+  const bool in = unit < a.n * a.groups_per_row.d;
+  const Place p = place_of(a, in ? unit : 0u);
+  const unsigned L = 1u << a.lanes_log2, lane = t & (L - 1u);
   float x[ITERS][VEC];
-  float top = 0.f;
-  bool bad = false;
-  if (live) {
-    const char* v = a.values + p.i * a.vrow + p.head * a.vhead + (long long)p.g * a.group * Elem<DT>::bytes;
-#pragma unroll
-    for (int it = 0; it < ITERS; ++it) {
-      const int c = lane + it * L;
-      if (c < a.chunks) {
-        load_values<DT, VEC>(v + (long long)c * VEC * Elem<DT>::bytes, x[it]);
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          const float m = fabsf(x[it][k]);
-          bad |= !(m < __builtin_inff());
-          top = fmaxf(top, m);
-        }
-      }
-    }
-  }
-  // an infinite or NaN value makes the whole group NaN: it is not hidden, and nothing finite is made of it
-  if (bad) top = __builtin_inff();
-  for (int o = L >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (!live) return;
-  const bool finite = top < __builtin_inff();
-  const float s = finite ? top / Code<FMT>::top : __builtin_nanf("");
-  const float f = top < 8.6736174e-19f /* 2^-60 */ ? 1.2089258e24f /* 2^80 */ : 1.f;
-  const float ss = s * f, inv = 1.f / ss;
-  const long long row = p.row;
-  unsigned char* cd = a.codes + row * a.crow + ((long long)p.head * a.dim + (long long)p.g * a.group) * Code<FMT>::bits / 8;
+  unsigned top_bits = 0u;         // |x| as bits: ordered like the magnitudes, infinities and NaN above them
+  const char* v = values_at(a, p, Elem<DT>::bytes);
 #pragma unroll
   for (int it = 0; it < ITERS; ++it) {
-    const int c = lane + it * L;
+    load_values<DT, VEC>(v + min(lane + it * L, a.chunks - 1u) * (unsigned)(VEC * Elem<DT>::bytes), x[it]);
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) top_bits = max(top_bits, __float_as_uint(x[it][k]) & 0x7fffffffu);
+  }
+  top_bits = group_max(top_bits, a.lanes_log2);
+  if (!in || p.row < 0 || (a.owner && a.owner[p.row] != (int)(a.i0 + p.i))) return;
+  // an infinite or NaN value makes the whole group NaN: it is not hidden, and nothing finite is made of it
+  const float top = __uint_as_float(top_bits);
+  const float s = top_bits < 0x7f800000u ? top / Code<FMT>::top : __builtin_nanf("");
+  const bool tiny = top < 0x1p-60f && s > 0.f;
+  const float inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
+  unsigned char* cd = codes_at<Code<FMT>::bits>(a, p);
+#pragma unroll
+  for (int it = 0; it < ITERS; ++it) {
+    const unsigned c = lane + it * L;
     if (c < a.chunks) {
       float q[VEC];
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) {
-        // a scale in the denormals is coarse: the quotient may pass the largest code
-        const float y = fminf(fmaxf(quotient_odd(x[it][k] * f, ss, inv), -Code<FMT>::top), Code<FMT>::top);
-        q[k] = s > 0.f ? y : 0.f;
-      }
-      encode<FMT, VEC>(q, cd + (long long)c * VEC * Code<FMT>::bits / 8);
+      quotients<FMT, VEC>(x[it], s, inv, q);
+      if (tiny) { asm volatile(""); quotients_tiny<FMT, VEC>(x[it], s, q); }      // (the asm keeps this a branch: it is never taken)
+      encode<FMT, VEC>(q, cd + (c * (unsigned)VEC * Code<FMT>::bits >> 3));
     }
   }
-  if (lane == 0) a.scales[row * a.srow + (long long)p.head * a.groups_per_head.d + p.g] = s;
+  if (lane == 0) *scale_at(a, p) = s;
 }
 
 // one chunk of VEC codes per thread
@@ -283,27 +326,27 @@ __global__ __launch_bounds__(256) void k_rows_read(RowsArgs a, FastDiv chunks, u
   const Place p = place_of(a, unit);
   float y[VEC];
   if (p.row >= 0) {
-    const float s = a.scales[p.row * a.srow + (long long)p.head * a.groups_per_head.d + p.g];
-    decode<FMT, VEC>(a.codes + p.row * a.crow + ((long long)p.head * a.dim + (long long)p.g * a.group + (long long)c * VEC) * Code<FMT>::bits / 8, y);
+    const float s = *scale_at(a, p);
+    decode<FMT, VEC>(codes_at<Code<FMT>::bits>(a, p) + (c * (unsigned)VEC * Code<FMT>::bits >> 3), y);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) y[k] *= s;
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) y[k] = 0.f;
   }
-  store_values<DT, VEC>(a.values + p.i * a.vrow + p.head * a.vhead + ((long long)p.g * a.group + (long long)c * VEC) * Elem<DT>::bytes, y);
+  store_values<DT, VEC>(values_at(a, p, Elem<DT>::bytes) + c * (unsigned)(VEC * Elem<DT>::bytes), y);
 }
 
 // chunks of a group that one lane holds at most: 64 lanes x 8 x VEC >= 1024 from pairs on, single elements need 16
 constexpr int max_iters(int vec) { return vec == 1 ? 16 : 8; }
 template <int FMT, int DT, int VEC> static void launch_write(const RowsArgs& a, unsigned grid, hipStream_t s) {
-  const int iters = (a.chunks + (1 << a.lanes_log2) - 1) >> a.lanes_log2;
+  const unsigned iters = (a.chunks + (1u << a.lanes_log2) - 1u) >> a.lanes_log2;
   if (iters == 1) hipLaunchKernelGGL((k_rows_write<FMT, DT, VEC, 1>), dim3(grid), dim3(256), 0, s, a);
   else hipLaunchKernelGGL((k_rows_write<FMT, DT, VEC, max_iters(VEC)>), dim3(grid), dim3(256), 0, s, a);
 }
 template <int FMT, int DT, int VEC> static void launch_read(const RowsArgs& a, hipStream_t s) {
-  const unsigned total = a.n * a.groups_per_row.d * (unsigned)a.chunks;
-  hipLaunchKernelGGL((k_rows_read<FMT, DT, VEC>), dim3((total + 255) / 256), dim3(256), 0, s, a, make_fastdiv((unsigned)a.chunks), total);
+  const unsigned total = a.n * a.groups_per_row.d * a.chunks;
+  hipLaunchKernelGGL((k_rows_read<FMT, DT, VEC>), dim3((total + 255) / 256), dim3(256), 0, s, a, make_fastdiv(a.chunks), total);
 }
 template <int FMT, int DT> static void dispatch(const RowsArgs& a, int vec, bool write, unsigned grid, hipStream_t s) {
 #define PSL_ROWS_CASE(V) if (vec == V) { if (write) launch_write<FMT, DT, V>(a, grid, s); else launch_read<FMT, DT, V>(a, s); return; }
@@ -326,13 +369,13 @@ static int run_rows(const char* who, const psl_rows_args* q, bool write, hipStre
     PSL_BAD("%s: heads %d, dim %d, group %d (heads and dim up to 4096, group up to 1024 and a divisor of dim)", who, q->heads, q->dim, q->group);
   const int bits = q->format == PSL_ROWS_INT4 ? 4 : 8, es = q->dtype == PSL_F32 ? 4 : 2;
   if (bits == 4 && (q->group & 1)) PSL_BAD("%s: two int4 codes share a byte: group %d must be even", who, q->group);
-  if (q->n < 0 || q->n > (1ll << 40) || q->capacity < 0 || q->capacity > (1ll << 40)) PSL_BAD("%s: n %lld, capacity %lld", who, (long long)q->n, (long long)q->capacity);
+  if (q->n < 0 || q->n > 0x7fffffffll || q->capacity < 0 || q->capacity > 0x7fffffffll) PSL_BAD("%s: n %lld, capacity %lld", who, (long long)q->n, (long long)q->capacity);
   if (q->n == 0) return PSL_OK;
   if (!q->values || !q->codes || !q->scales) PSL_BAD("%s: missing pointer", who);
   if (q->rows ? (q->rows_bits != 32 && q->rows_bits != 64) : (q->first < 0 || q->first > q->capacity || q->n > q->capacity - q->first))
     PSL_BAD("%s: rows [%lld, +%lld) of %lld (rows_bits %d)", who, (long long)q->first, (long long)q->n, (long long)q->capacity, q->rows_bits);
   const long long hd = (long long)q->heads * q->dim;
-  const long long big = 1ll << 40;
+  const long long big = 1ll << 29;          // strides in bytes stay below 2^31
   if (q->value_row_stride < 0 || q->value_head_stride < 0 || q->value_row_stride > big || q->value_head_stride > big || q->codes_row_stride > big || q->scales_row_stride > big ||
       q->codes_row_stride < hd * bits / 8 || q->scales_row_stride < hd / q->group)
     PSL_BAD("%s: bad stride", who);
@@ -340,7 +383,6 @@ static int run_rows(const char* who, const psl_rows_args* q, bool write, hipStre
     PSL_BAD("%s: rows of the output overlap", who);
   const uintptr_t pv = (uintptr_t)q->values, pc = (uintptr_t)q->codes, ps = (uintptr_t)q->scales;
   if (pv % es || ps % 4 || (q->rows && (uintptr_t)q->rows % (q->rows_bits / 8))) PSL_BAD("%s: misaligned pointer", who);
-  if (write && q->rows && q->owner && q->n > 0x7fffffffll) PSL_BAD("%s: %lld rows in one call with an owner table (2^31 - 1 at most)", who, (long long)q->n);
   // VEC: the widest piece that divides a group and that every address keeps aligned (16-byte loads of values, code words of
   // VEC * bits / 8 bytes).  fp32 rows of 32: 8 beats 1 by 6x (54 000 rows).
   int vec = 8;
@@ -353,19 +395,20 @@ static int run_rows(const char* who, const psl_rows_args* q, bool write, hipStre
   }
   RowsArgs a;
   a.rows = q->rows; a.rows_bits = q->rows_bits; a.first = q->first; a.capacity = q->capacity;
-  a.values = (char*)q->values; a.vrow = q->value_row_stride * es; a.vhead = q->value_head_stride * es;
-  a.codes = (unsigned char*)q->codes; a.crow = q->codes_row_stride; a.scales = q->scales; a.srow = q->scales_row_stride;
+  a.vrow = (unsigned)(q->value_row_stride * es); a.vhead = (unsigned)(q->value_head_stride * es);
+  a.codes = (unsigned char*)q->codes; a.crow = (unsigned)q->codes_row_stride; a.scales = q->scales; a.srow = (unsigned)q->scales_row_stride;
+  a.heads_apart = q->heads > 1 && q->value_head_stride != q->dim;
   a.owner = write && q->rows ? q->owner : nullptr;
-  a.heads = q->heads; a.dim = q->dim; a.group = q->group; a.chunks = q->group / vec;
+  a.group = (unsigned)q->group; a.chunks = (unsigned)(q->group / vec);
   a.groups_per_row = make_fastdiv((unsigned)(hd / q->group)); a.groups_per_head = make_fastdiv((unsigned)(q->dim / q->group));
   // Lanes of a group: the largest power of two that divides its chunks leaves no lane idle (a group of 80 = ten chunks on
   // two lanes); where that would leave more than eight chunks to a lane, the next power of two above, some lanes idle.
   int l = 0;
   while (l < 6 && (a.chunks >> l) % 2 == 0) ++l;
-  if ((a.chunks >> l) > 8) { l = 0; while (l < 6 && (1 << l) < a.chunks) ++l; }
+  if ((a.chunks >> l) > 8) { l = 0; while (l < 6 && (1u << l) < a.chunks) ++l; }
   a.lanes_log2 = l;
   if (a.owner) {
-    a.i0 = 0; a.n = (unsigned)q->n;
+    a.i0 = 0; a.n = (unsigned)q->n; a.values = (char*)q->values;
     const unsigned grid = (unsigned)((q->n + 255) / 256);
     hipLaunchKernelGGL(k_rows_owner_clear, dim3(grid), dim3(256), 0, s, a, q->owner);
     hipLaunchKernelGGL(k_rows_owner_claim, dim3(grid), dim3(256), 0, s, a, q->owner);
@@ -375,6 +418,7 @@ static int run_rows(const char* who, const psl_rows_args* q, bool write, hipStre
   const long long step = (1ll << 30) / per_row;
   for (long long i0 = 0; i0 < q->n; i0 += step) {
     a.i0 = i0; a.n = (unsigned)(q->n - i0 < step ? q->n - i0 : step);
+    a.values = (char*)q->values + i0 * q->value_row_stride * es;
     const unsigned grid = (unsigned)((((long long)a.n * a.groups_per_row.d << l) + 255) / 256);
     if (q->format == PSL_ROWS_INT8) dispatch<PSL_ROWS_INT8>(a, q->dtype, vec, write, grid, s);
     else if (q->format == PSL_ROWS_E4M3) dispatch<PSL_ROWS_E4M3>(a, q->dtype, vec, write, grid, s);
