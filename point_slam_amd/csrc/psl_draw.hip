@@ -212,16 +212,19 @@ __device__ __forceinline__ bool has_cut(const RowPar& p) { return p.k > 0 || p.p
 // bin: a difference, a product and a truncation never fall as the score falls, so a bin is an interval of scores, and that is
 // all it has to be.  A bin's mass is a sum of integers, weights scaled by 2^(q + the bin's own exponent): it has no order, and its
 // rounding is 2^-q of the bin's own weights.
-struct Binning { float M, scale; double inv_t, width, oct; int q; };
+struct Binning { float M, scale; double inv_t, width, oct; int q; bool plain; };      // plain: no entry lies behind its bin
 __device__ __forceinline__ Binning make_binning(const Range& g, double inv_t, int n_cols) {
   Binning b;
   b.M = score_of(g.mx); b.inv_t = inv_t;
   double range = ((double)b.M - (double)score_of(g.mn)) * inv_t;
-  if (!(range < kRange)) range = kRange;
-  // An infinite largest score: it in the first bin, everything else in the last, which weighs nothing (k_draw_hist).
-  const bool inf_row = b.M == __builtin_inff();
-  b.width = inf_row ? 0.0 : range / (double)kBins;              // in temperatures
-  b.scale = inf_row ? 1.f : (float)(inv_t / b.width);           // bins per unit of score (inf: no other score than M)
+  b.plain = range < kRange;
+  if (!b.plain) range = kRange;
+  // bins per unit of score, a number whatever the row is (equal scores, denormal ones, infinite ones, no temperature), and the
+  // width that this number means, in temperatures
+  const double sc = (double)kBins * inv_t / range;
+  b.plain = b.plain && sc > 1e-36 && sc < 3e38;
+  b.scale = sc > 0.0 ? (float)fmin(fmax(sc, 1e-36), 3e38) : 1.f;
+  b.width = inv_t / (double)b.scale;
   b.oct = b.width * 1.4426950408889634;             // binary orders per bin
   b.q = min(62 - (32 - __clz(n_cols)), 51);         // the row's sum below 2^63, an entry's below to_integer's limit
   return b;
@@ -230,17 +233,14 @@ __device__ __forceinline__ int bin_of(const Binning& b, float s) {
   // (NaN, from inf - inf or 0 * inf, converts to 0: the largest score's bin)
   return (int)min(__float2uint_rz((b.M - s) * b.scale), (unsigned)(kBins - 1));
 }
-__device__ __forceinline__ int bin_shift(const Binning& b, int bin) { return b.q + (int)((double)bin * b.oct); }
+__device__ __forceinline__ int bin_shift(const Binning& b, int bin) { return b.q + (int)fmin((double)bin * b.oct, 1000.0); }
 
 // 0 <= x < 2^52 to the nearest integer: 2^52 + x has it in its low bits
 __device__ __forceinline__ u64 to_integer(double x) { return (u64)__double_as_longlong(x + 0x1p52) & 0xfffffffffffffull; }
 
 // An entry's scaled weight is its bin's first weight (a table) times e^-f, f < kRange / kBins = 0.047 behind the bin's begin:
-// the terms to the seventh leave 1e-15 of it.  What lies beyond kRange counts as lying at the last bin's end: 1e-21 of the
-// largest weight, a million of which do not reach the sum's rounding.
-__device__ __forceinline__ double first_weight(const Binning& b, int j) {
-  return b.M == __builtin_inff() && j ? 0.0 : ldexp(exp(-(double)j * b.width), bin_shift(b, j));
-}
+// the terms to the seventh leave 1e-15 of it.  What lies beyond kRange, in the last bin, takes the exponential.
+__device__ __forceinline__ double first_weight(const Binning& b, int j) { return ldexp(exp(-(double)j * b.width), bin_shift(b, j)); }
 // the coefficients stay in registers (the compiler would write them anew for every entry: they are not inline constants)
 struct BinPoly { double c7, c6, c5, c4, c3; };
 __device__ __forceinline__ BinPoly make_bin_poly() {
@@ -248,7 +248,7 @@ __device__ __forceinline__ BinPoly make_bin_poly() {
   asm("" : "+v"(p.c7), "+v"(p.c6), "+v"(p.c5), "+v"(p.c4), "+v"(p.c3));
   return p;
 }
-template <int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f, const Binning& b, const BinPoly& c, bool count, bool weigh,
+template <bool PLAIN, int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f, const Binning& b, const BinPoly& c, bool count, bool weigh,
                                                               unsigned* cnt, u64* mass, const double* first) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
@@ -257,7 +257,7 @@ template <int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f,
       const int bin = bin_of(b, s);
       if (count) atomicAdd(&cnt[bin], 1u);
       if (weigh) {
-        const double y = fmin(fma((double)bin, -b.width, ((double)b.M - (double)s) * b.inv_t), b.width);      // (a NaN gives the width)
+        const double y = fma((double)bin, -b.width, ((double)b.M - (double)s) * b.inv_t);
         double p = fma(y, c.c7, c.c6);
         p = fma(y, p, c.c5);
         p = fma(y, p, c.c4);
@@ -265,6 +265,9 @@ template <int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f,
         p = fma(y, p, 0.5);
         p = fma(y, p, -1.0);
         p = fma(y, p, 1.0);
+        if (!PLAIN && !(fabs(y) <= 0.06)) {        // far scores, odd rows
+          p = b.M == __builtin_inff() ? (s == b.M ? 1.0 : 0.0) : exp(-fmin(fmax(y, 0.0), 1100.0));
+        }
         atomicAdd(&mass[bin], to_integer(first[bin] * p));
       }
     }
@@ -296,10 +299,11 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   unsigned* const my_cnt = cnt[tid & (kCopies - 1)];
   u64* const my_mass = mass[tid & (kCopies - 1)];
   const BinPoly poly = make_bin_poly();
+  if (b.plain) {
 #pragma unroll 2
-  for (int i = i0 + tid * 4; i < i1; i += 2048) {
-    const Four<DT> f = load_four<DT>(v, i, i1);
-    add_to_bins(f, b, poly, count, weigh, my_cnt, my_mass, first);
+    for (int i = i0 + tid * 4; i < i1; i += 2048) add_to_bins<true>(load_four<DT>(v, i, i1), b, poly, count, weigh, my_cnt, my_mass, first);
+  } else {
+    for (int i = i0 + tid * 4; i < i1; i += 2048) add_to_bins<false>(load_four<DT>(v, i, i1), b, poly, count, weigh, my_cnt, my_mass, first);
   }
   __syncthreads();
   for (int j = tid; j < kBins; j += 512) {
@@ -386,8 +390,8 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
 }
 
 // Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.  A
-// workgroup collects in LDS and asks once for its places in the row's list (a global atomic for every wavefront that found something made this 112 us for twelve rows of
-// 816 000); what does not fit there goes to the list by itself.
+// workgroup collects in LDS and asks once for its places in the row's list (a global atomic for every wavefront that found
+// something made this 112 us for twelve rows of 816 000); what does not fit there goes to the list by itself.
 constexpr int kListBuf = 1024;
 struct ListBuf { u64 e[kListBuf]; unsigned n, at; };
 __device__ __forceinline__ void list_add(ListBuf& b, u64 x, u64* dst, unsigned* fill, unsigned cap) {
@@ -986,7 +990,7 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a)
     __syncthreads();
     const BinPoly poly = make_bin_poly();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) add_to_bins(f[j], b, poly, count, weigh, S.cnt, S.mass, S.first);
+    for (int j = 0; j < 4; ++j) add_to_bins<false>(f[j], b, poly, count, weigh, S.cnt, S.mass, S.first);
     __syncthreads();
     const unsigned c = S.cnt[tid];
     const double m = ldexp((double)S.mass[tid], -bin_shift(b, tid));

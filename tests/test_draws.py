@@ -351,3 +351,10 @@ def test_wide_and_narrow_ranges():
               torch.where(base > 2.5, base, torch.full_like(base, torch.finfo(torch.float32).min))):
         for cut in (dict(top_k=1000), dict(top_p=0.9), dict(top_k=20000, top_p=0.99), dict(top_p=0.5, temperature=1e-3), dict(top_k=5000, temperature=1e4), dict(top_p=1 - 1e-9), dict(top_k=V - 1)):
             _check(s, u, where=str(cut), **cut)
+    for scale, t in ((1e-37, 1e-37), (1e-40, 1e-41), (1e-38, 1e-30), (1e30, 1e35), (1e-30, 1e-320), (1e37, 1e-300)):
+        for cut in (dict(top_p=0.9), dict(top_k=700, top_p=0.5), dict(top_k=25000)):
+            _check(base * scale, u, where=f"{scale} {t} {cut}", temperature=t, **cut)
+    s = base.clone(); s[0, ::1000] = float("inf")
+    for t in (1.0, float("inf"), 1e-300, 1e300):
+        for cut in (dict(top_p=0.5), dict(top_k=7), dict(top_k=3000, top_p=0.9)):
+            _check(s, u, where=f"inf {t} {cut}", temperature=t, **cut)
