@@ -866,18 +866,21 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
       const double x = a.group_incl[g0 + mid];
       if (x > in_chunk) hi = mid; else { g = mid + 1; front = x; }
     }
-    const DrawGroup& gr = groups[g];
     double incl[8];
-    unsigned short bits[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) incl[j] = gr.incl[j];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) bits[j] = gr.kept[j];
+    uint4 bits;
+    __builtin_memcpy(incl, groups[g].incl, 64);
+    __builtin_memcpy(&bits, groups[g].kept, 16);
     int b = 0;
     double back = incl[0];
-    unsigned kept = bits[0];
 #pragma unroll
-    for (int j = 1; j < 8; ++j) if (incl[j - 1] <= in_chunk) { b = j; front = incl[j - 1]; back = incl[j]; kept = bits[j]; }
+    for (int j = 1; j < 8; ++j) {
+      const bool behind = incl[j - 1] <= in_chunk;
+      b += behind ? 1 : 0;
+      front = behind ? incl[j - 1] : front;
+      back = behind ? incl[j] : back;
+    }
+    const unsigned half = b & 4 ? (b & 2 ? bits.w : bits.z) : (b & 2 ? bits.y : bits.x);
+    unsigned kept = b & 1 ? half >> 16 : half & 0xffffu;
     double in_block = in_chunk - front;
     const double mass = back - front;
     int block = g * 8 + b;
