@@ -27,6 +27,8 @@ struct DrawArgs {
   struct DrawState* state;     // [n_rows]
   struct DrawCut* cut;         // [n_rows]
   unsigned* part_max; unsigned* part_min;       // [n_rows][n_parts] keys
+  unsigned* tops; int top_lanes, n_tops;       // [n_rows][n_tops] keys: the largest of every top_lanes lanes of a part's workgroup
+  int listed_draws;            // whether k_draw_cut may draw from a row's list
   unsigned* bin_cnt; unsigned long long* bin_mass;       // [n_rows][kBins]
   double* bin_excl;            // [n_rows][kBins]: running sums in front of the bins; those behind them replace bin_mass
   unsigned long long* list_a; unsigned long long* list_b; int list_cap;      // [n_rows][list_cap] numbers of candidate entries
@@ -41,14 +43,16 @@ struct DrawState {
   double inv_t, m;             // 1 / temperature, min-p
   float M; int any;            // largest allowed score; whether there is one
   unsigned n_a, n_b;           // fill of the two lists
+  int drawn;                   // k_draw_cut has drawn for this row
 };
 
 struct DrawCut {
   float M; int any;                // as in DrawState
-  double inv_t, p, width;          // 1 / temperature, top-p (1: off), a bin's width
+  double inv_t, p;                 // 1 / temperature, top-p (1: off)
   float scale; unsigned want;      // bins per unit of score; entries of k_bin that top-k keeps
   int k_bin, p_lo, p_hi;           // k_bin = kBins: top-k keeps all; top-p's bin lies in [p_lo, p_hi], or is k_bin
   unsigned n_a;                    // entries of k_bin
+  unsigned n_all;                  // entries up to the last bin that a limit can fall into, if they are all drawn from one list (else 0)
   double above_k, total;           // mass of the bins before k_bin; of all
 };
 
@@ -63,6 +67,7 @@ constexpr int kMaxChunks = 1024;
 constexpr int kMaxParts = 256;
 constexpr int kBins = 1024;
 constexpr double kRange = 48.0;
+constexpr int kSorted = 1024;  // numbers that a workgroup sorts, one to a thread
 
 // ---- an entry's order: excluded entries (masked, NaN, -inf) are 0, everything else grows with the score; -0 == +0
 __device__ __forceinline__ unsigned key_of(float s) {
@@ -179,8 +184,14 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_range(DrawArgs a
 #pragma unroll
     for (int q = 0; q < 4; ++q) { const unsigned k = four_key(f, q); mx = max(mx, k); mn = min(mn, k ? k : 0xffffffffu); }
   }
-  for (int o = 32; o > 0; o >>= 1) { mx = max(mx, (unsigned)__shfl_xor((int)mx, o)); mn = min(mn, (unsigned)__shfl_xor((int)mn, o)); }
-  if (lane == 0) { s_mx[tid >> 6] = mx; s_mn[tid >> 6] = mn; }
+  for (int o = 1; o < 64; o <<= 1) {
+    if (o == a.top_lanes && a.cuts && (tid & (o - 1)) == 0) a.tops[(long long)r * a.n_tops + blockIdx.x * (256 / o) + tid / o] = mx;
+    mx = max(mx, (unsigned)__shfl_xor((int)mx, o)); mn = min(mn, (unsigned)__shfl_xor((int)mn, o));
+  }
+  if (lane == 0) {
+    s_mx[tid >> 6] = mx; s_mn[tid >> 6] = mn;
+    if (a.top_lanes == 64 && a.cuts) a.tops[(long long)r * a.n_tops + blockIdx.x * 4 + (tid >> 6)] = mx;
+  }
   __syncthreads();
   if (tid == 0) {
     a.part_max[(long long)r * a.n_parts + blockIdx.x] = max(max(s_mx[0], s_mx[1]), max(s_mx[2], s_mx[3]));
@@ -189,7 +200,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_range(DrawArgs a
   // what the next launches add to
   if (a.cuts && blockIdx.x == 0) {
     for (int j = tid; j < kBins; j += 256) { a.bin_cnt[(long long)r * kBins + j] = 0u; a.bin_mass[(long long)r * kBins + j] = 0ull; }
-    if (tid == 0) { a.state[r].n_a = 0u; a.state[r].n_b = 0u; }
+    if (tid == 0) { a.state[r].n_a = 0u; a.state[r].n_b = 0u; a.state[r].drawn = 0; }
   }
 }
 // the same of the whole row, to every thread of a workgroup (n_parts <= kMaxParts)
@@ -248,13 +259,14 @@ __device__ __forceinline__ BinPoly make_bin_poly() {
   asm("" : "+v"(p.c7), "+v"(p.c6), "+v"(p.c5), "+v"(p.c4), "+v"(p.c3));
   return p;
 }
-template <bool PLAIN, int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f, const Binning& b, const BinPoly& c, bool count, bool weigh,
+template <bool PLAIN, int DT> __device__ __forceinline__ void add_to_bins(const Four<DT>& f, const Binning& b, const BinPoly& c, bool count, bool weigh, int last,
                                                               unsigned* cnt, u64* mass, const double* first) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const float s = f.s[q];
     if (((f.live >> q) & 1u) && s > -__builtin_inff()) {
       const int bin = bin_of(b, s);
+      if (bin > last) continue;
       if (count) atomicAdd(&cnt[bin], 1u);
       if (weigh) {
         const double y = fma((double)bin, -b.width, ((double)b.M - (double)s) * b.inv_t);
@@ -274,8 +286,33 @@ template <bool PLAIN, int DT> __device__ __forceinline__ void add_to_bins(const 
   }
 }
 
+// The last bin that matters to a row with top-k: of n_tops maxima of disjoint parts of the row the k-th largest is no larger
+// than the row's k-th score, and top-p weighs what top-k leaves.  What lies behind is neither counted nor weighed.  A workgroup of 512, cnt zero before and after.
+constexpr int kTops = 1024;
+__device__ __forceinline__ int last_bin(const DrawArgs& a, int r, int k, const Binning& b, unsigned* cnt) {
+  __shared__ unsigned s_n[8];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) s_last = kBins - 1;
+  for (int j = tid; j < a.n_tops; j += 512) {
+    const unsigned key = a.tops[(long long)r * a.n_tops + j];
+    if (key) atomicAdd(&cnt[bin_of(b, score_of(key))], 1u);
+  }
+  __syncthreads();
+  const unsigned c0 = cnt[2 * tid], c1 = cnt[2 * tid + 1];
+  cnt[2 * tid] = 0u; cnt[2 * tid + 1] = 0u;
+  unsigned incl = c0 + c1;
+  for (int o = 1; o < 64; o <<= 1) { const unsigned x = __shfl_up(incl, o); if (lane >= o) incl += x; }
+  if (lane == 63) s_n[tid >> 6] = incl;
+  __syncthreads();
+  for (int w = 0; w < (tid >> 6); ++w) incl += s_n[w];
+  if (incl >= (unsigned)k && incl - c0 - c1 < (unsigned)k) s_last = incl - c1 >= (unsigned)k ? 2 * tid : 2 * tid + 1;
+  __syncthreads();
+  return s_last;
+}
+
 // Bound: instructions (65 per entry made this 25 us for twelve rows of 816 000), then the LDS atomics: entries are counted
-// only where top-k asks and weighed only where top-p does, and neighbouring lanes use different copies.
+// only where that is used and weighed only where top-p does, and neighbouring lanes use different copies.
 constexpr int kCopies = 2;
 template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
   __shared__ unsigned cnt[kCopies][kBins];
@@ -284,15 +321,17 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   const int r = blockIdx.y, tid = threadIdx.x;
   const RowPar par = row_par(a, r);
   if (!has_cut(par)) return;
-  const bool weigh = par.p < 1.0, count = par.k > 0;
+  const bool weigh = par.p < 1.0 && par.k != 1, count = par.k > 0 || a.listed_draws;
   const Range g = row_range(a, r);
   if (!g.mx) return;
   const Binning b = make_binning(g, par.inv_t, a.n_cols);
   for (int j = tid; j < kBins; j += 512) {
 #pragma unroll
     for (int q = 0; q < kCopies; ++q) { cnt[q][j] = 0u; mass[q][j] = 0ull; }
-    if (weigh) first[j] = first_weight(b, j);
   }
+  __syncthreads();
+  const int last = par.k > 0 && par.k <= a.n_tops ? last_bin(a, r, par.k, b, cnt[0]) : kBins - 1;
+  if (weigh) for (int j = tid; j <= last; j += 512) first[j] = first_weight(b, j);
   __syncthreads();
   const RowView v = row_view<DT>(a, r);
   const int i0 = blockIdx.x * a.part_len, i1 = min(i0 + a.part_len, a.n_cols);
@@ -301,12 +340,12 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a)
   const BinPoly poly = make_bin_poly();
   if (b.plain) {
 #pragma unroll 2
-    for (int i = i0 + tid * 4; i < i1; i += 2048) add_to_bins<true>(load_four<DT>(v, i, i1), b, poly, count, weigh, my_cnt, my_mass, first);
+    for (int i = i0 + tid * 4; i < i1; i += 2048) add_to_bins<true>(load_four<DT>(v, i, i1), b, poly, count, weigh, last, my_cnt, my_mass, first);
   } else {
-    for (int i = i0 + tid * 4; i < i1; i += 2048) add_to_bins<false>(load_four<DT>(v, i, i1), b, poly, count, weigh, my_cnt, my_mass, first);
+    for (int i = i0 + tid * 4; i < i1; i += 2048) add_to_bins<false>(load_four<DT>(v, i, i1), b, poly, count, weigh, last, my_cnt, my_mass, first);
   }
   __syncthreads();
-  for (int j = tid; j < kBins; j += 512) {
+  for (int j = tid; j <= last; j += 512) {
     unsigned c = 0u; u64 m = 0ull;
 #pragma unroll
     for (int q = 0; q < kCopies; ++q) { c += cnt[q][j]; m += mass[q][j]; }
@@ -333,10 +372,10 @@ __device__ __forceinline__ void find_bins(const DrawArgs& a, const RowPar& par, 
   const int j = threadIdx.x, lane = j & 63, wave = j >> 6;
   if (j == 0) {
     sh.k = kBins; sh.lo = kBins; sh.hi = kBins; sh.last = -1; sh.want = 0u; sh.na = 0u;
-    o->M = b.M; o->any = g.mx ? 1 : 0; o->inv_t = par.inv_t; o->p = par.k == 1 ? 1.0 : par.p; o->width = b.width; o->scale = b.scale;
+    o->M = b.M; o->any = g.mx ? 1 : 0; o->inv_t = par.inv_t; o->p = par.k == 1 ? 1.0 : par.p; o->scale = b.scale;
   }
   if (!g.mx || !has_cut(par)) {
-    if (j == 0) { o->k_bin = kBins; o->p_hi = -1; o->n_a = 0u; }
+    if (j == 0) { o->k_bin = kBins; o->p_hi = -1; o->n_a = 0u; o->n_all = 0u; }
     return;
   }
   unsigned n_incl = c; double incl = m;
@@ -356,7 +395,8 @@ __device__ __forceinline__ void find_bins(const DrawArgs& a, const RowPar& par, 
   n_incl += n_before; incl += before;
   cum[j] = m > 0.0 ? incl : -1.0;
   excl_out[j] = excl;
-  const bool cut_k = par.k > 0 && (unsigned)par.k < n_valid, cut_p = par.p < 1.0 && par.k != 1;
+  // (as many as there are: they may be only what was counted, and the limit keeps all of them)
+  const bool cut_k = par.k > 0 && (unsigned)par.k <= n_valid, cut_p = par.p < 1.0 && par.k != 1;
   if (cut_k && n_incl >= (unsigned)par.k && n_incl - c < (unsigned)par.k) {
     sh.k = j; sh.want = (unsigned)par.k - (n_incl - c); sh.na = c; sh.most = incl; sh.above_k = excl;
   }
@@ -372,6 +412,9 @@ __device__ __forceinline__ void find_bins(const DrawArgs& a, const RowPar& par, 
   }
   __syncthreads();
   const int p_lo = cut_p ? min(sh.lo, sh.last) : 0, p_hi = cut_p ? min(sh.hi, sh.last) : -1;
+  // the last bin that a limit can fall into, and whether all entries up to it are few
+  const int end = cut_k ? k_bin : p_hi;
+  if (j == max(end, 0)) o->n_all = a.listed_draws && end >= 0 && n_incl <= (unsigned)kSorted ? n_incl : 0u;
   if (j == 64) {
     o->want = sh.want; o->k_bin = k_bin; o->p_lo = p_lo; o->p_hi = p_hi; o->n_a = sh.na; o->above_k = above_k; o->total = total;
   }
@@ -389,7 +432,8 @@ __global__ __launch_bounds__(kBins) void k_draw_bins(DrawArgs a) {
   find_bins(a, par, g, b, c, m, (double*)(a.bin_mass + (long long)r * kBins), a.bin_excl + (long long)r * kBins, a.cut + r, sh);
 }
 
-// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other.  A
+// Entries of those bins, as their 64-bit numbers, in any order: top-k's bin into one list, top-p's into the other, or all that
+// a row can keep into the first.  A
 // workgroup collects in LDS and asks once for its places in the row's list (a global atomic for every wavefront that found
 // something made this 112 us for twelve rows of 816 000); what does not fit there goes to the list by itself.
 constexpr int kListBuf = 1024;
@@ -403,11 +447,13 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
   __shared__ ListBuf buf_a, buf_b;
   const int r = blockIdx.y, tid = threadIdx.x;
   const DrawCut& c = a.cut[r];
-  const bool do_a = c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap, do_b = c.p_hi >= 0;
+  const bool all = c.n_all > 0u, do_a = all || (c.k_bin < kBins && c.n_a <= (unsigned)a.list_cap), do_b = !all && c.p_hi >= 0;
   if (!do_a && !do_b) return;
   Binning b;
   b.M = c.M; b.scale = c.scale;
-  const int ka = do_a ? c.k_bin : -1, p0 = do_b ? c.p_lo : 0, p1 = do_b ? c.p_hi : -1;      // (no such bin: an empty interval)
+  // (no such bin: an empty interval)
+  const int k_bin = c.k_bin < kBins ? c.k_bin : c.p_hi;
+  const int a0 = all ? 0 : k_bin, a1 = do_a ? k_bin : -1, p0 = c.p_lo, p1 = do_b ? c.p_hi : -1;
   if (tid == 0) { buf_a.n = 0u; buf_b.n = 0u; }
   __syncthreads();
   const RowView v = row_view<DT>(a, r);
@@ -423,7 +469,7 @@ template <int DT> __global__ __launch_bounds__(512) void k_draw_gather(DrawArgs 
       const float x = f.s[q];
       if (((f.live >> q) & 1u) && x > -__builtin_inff()) {
         const int bin = bin_of(b, x);
-        if (bin == ka) list_add(buf_a, number_of(key_of(x), i + q), la, &a.state[r].n_a, cap);
+        if (bin >= a0 && bin <= a1) list_add(buf_a, number_of(key_of(x), i + q), la, &a.state[r].n_a, cap);
         if (bin >= p0 && bin <= p1) list_add(buf_b, number_of(key_of(x), i + q), lb, &a.state[r].n_b, cap);
       }
     }
@@ -576,7 +622,6 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
 
 // Up to 1 024 numbers, one to a thread, in descending order (zeros behind them): exchanges inside a wavefront through
 // shuffles, between wavefronts through LDS.
-constexpr int kSorted = 1024;
 __device__ __forceinline__ u64 block_sort(u64 x, int n, u64* lds) {
   const int tid = threadIdx.x;
   for (int k = 2; k < 2 * n && k <= kSorted; k <<= 1) {
@@ -704,12 +749,58 @@ template <int DT> __device__ __forceinline__ u64 find_threshold(const RowView& v
   }
   return thr;
 }
+// The draws of a row whose n entries up to the last bin of its limits are all in one list: sorted by score they give the
+// threshold, sorted by index the running sums.  What k_draw_sums and k_draw_pick do for it otherwise is two passes over the row
+// (TIME).
+__device__ __forceinline__ void draw_from_list(const DrawArgs& a, int r, const DrawCut& c, const RowPar& par, CutShared& S, double* run) {
+  const int tid = threadIdx.x, n = (int)c.n_all;
+  const bool cut_k = c.k_bin < kBins, cut_p = c.p < 1.0;
+  u64 x = block_sort(tid < n ? a.list_a[(long long)r * a.list_cap + tid] : 0ull, n, S.sort);
+  const double w = x ? weight_of(score_of((unsigned)(x >> 32)), c.M, c.inv_t, S.sh.exp) : 0.0;
+  int end = cut_k ? par.k : n;
+  if (cut_p) {
+    const double incl = block_running(w, S.wave);
+    if (tid == end - 1) { S.kept = incl; S.at = end - 1; }
+    __syncthreads();
+    note_first(&S.at, x && incl >= c.p * (cut_k ? S.kept : c.total));
+    __syncthreads();
+    end = S.at + 1;
+  }
+  x = tid < end && w >= fmax(par.m, 0x1p-1074) ? x << 32 | x >> 32 : 0ull;
+  x = block_sort(x, end, S.sort);
+  const double incl = block_running(x ? weight_of(score_of((unsigned)x), c.M, c.inv_t, S.sh.exp) : 0.0, S.wave);
+  if (tid == 0) S.at = kSorted;
+  __syncthreads();                                  // (and the sort's last exchange is over)
+  run[tid] = incl;
+  S.sort[tid] = x;
+  note_first(&S.at, !x);
+  __syncthreads();
+  const int last = S.at - 1;
+  const double total = run[kSorted - 1];
+  const long long out0 = (long long)r * a.n_draws;
+  for (int d = tid; d < a.n_draws; d += 1024) {
+    double u = (double)a.u[(long long)r * a.u_stride + d];
+    u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
+    const double target = u * total;
+    int lo = 0, hi = last;
+    while (lo < hi) { const int mid = (lo + hi) >> 1; if (run[mid] > target) hi = mid; else lo = mid + 1; }
+    const u64 e = S.sort[lo];
+    a.idx[out0 + d] = (int)~(unsigned)(e >> 32);
+    if (a.prob) a.prob[out0 + d] = (float)(weight_of(score_of((unsigned)e), c.M, c.inv_t, S.sh.exp) / total);
+  }
+}
 template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a) {
   __shared__ CutShared S;
+  __shared__ double run[kSorted];
   exp_table_init(S.sh.exp);
   const int r = blockIdx.x;
   const DrawCut& c = a.cut[r];
   __syncthreads();
+  if (c.n_all) {
+    if (threadIdx.x == 0) a.state[r].drawn = 1;
+    draw_from_list(a, r, c, row_par(a, r), S, run);
+    return;
+  }
   u64 thr = 1ull << 32;
   if (c.any && (c.k_bin < kBins || c.p < 1.0))
     thr = find_threshold<DT>(row_view<DT>(a, r), a.n_cols, c, a.list_a + (long long)r * a.list_cap, a.list_b + (long long)r * a.list_cap, a.state[r].n_b,
@@ -725,7 +816,7 @@ __device__ __forceinline__ DrawState row_state(const DrawArgs& a, int r) {
   if (a.cuts) return a.state[r];
   const Range g = row_range(a, r);
   const RowPar par = row_par(a, r);
-  return DrawState{1ull << 32, par.inv_t, par.m, score_of(g.mx), g.mx ? 1 : 0, 0u, 0u};
+  return DrawState{1ull << 32, par.inv_t, par.m, score_of(g.mx), g.mx ? 1 : 0, 0u, 0u, 0};
 }
 
 // ---------------------------------------------------------------- running sums of the kept weights
@@ -745,6 +836,7 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
   __shared__ double wsum[4];
   __shared__ ExpTable s_exp;
   const int r = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  if (a.listed_draws && a.state[r].drawn) return;
   exp_table_init(s_exp);
   const RowView v = row_view<DT>(a, r);
   const DrawState st = row_state(a, r);
@@ -822,6 +914,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
   const long long d0 = (long long)(work - (unsigned)r * (unsigned)a.pick_wgs) * a.pick_len;
   const long long d1 = d0 + a.pick_len < a.n_draws ? d0 + a.pick_len : a.n_draws;
   const long long out0 = (long long)r * a.n_draws;
+  if (a.listed_draws && a.state[r].drawn) return;
   exp_table_init(s_exp);
   const DrawState st = row_state(a, r);
   const int nc = a.n_chunks;
@@ -943,7 +1036,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
 // ---------------------------------------------------------------- short rows: everything by one workgroup
 // The same steps with the row in registers (up to 16 entries to a thread), all else in LDS: one launch instead of seven,
 // whose starts and first loads are what a short row costs (1 x 2 048: 32 us in seven, 13 us in one).
-constexpr int kRowCols = 16384, kRowList = 1024;
+constexpr int kRowCols = 16384, kRowList = 1024, kRowDraws = 4096;
 struct RowShared {
   union { unsigned cnt[kBins]; double running[kBins]; };          // bin counts, later the blocks' running sums (kRowCols / kBlock = kBins)
   union { u64 mass[kBins]; double cum[kBins]; };
@@ -955,6 +1048,7 @@ struct RowShared {
   DrawCut c;
   unsigned n_a, n_b;
 };
+static_assert(kMaxParts * 256 / 64 <= kTops, "tops");
 static_assert(sizeof(RowShared) <= 65536, "LDS");
 template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a) {
   __shared__ RowShared S;
@@ -988,12 +1082,12 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a)
   if (has_cut(par)) {
     const Range g{mx, mn};
     const Binning b = make_binning(g, par.inv_t, a.n_cols);
-    const bool weigh = par.p < 1.0, count = par.k > 0;
+    const bool weigh = par.p < 1.0 && par.k != 1, count = par.k > 0;
     if (weigh) S.first[tid] = first_weight(b, tid);
     __syncthreads();
     const BinPoly poly = make_bin_poly();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) add_to_bins<false>(f[j], b, poly, count, weigh, S.cnt, S.mass, S.first);
+    for (int j = 0; j < 4; ++j) add_to_bins<false>(f[j], b, poly, count, weigh, kBins - 1, S.cnt, S.mass, S.first);
     __syncthreads();
     const unsigned c = S.cnt[tid];
     const double m = ldexp((double)S.mass[tid], -bin_shift(b, tid));
@@ -1077,7 +1171,7 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a)
 }
 
 // ---------------------------------------------------------------- host side
-struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap; size_t state, cut, chunk_sum, group, group_incl, part_max, part_min, bin_cnt, bin_mass, bin_excl, list_a, list_b, total; };
+struct DrawLayout { int chunk, n_chunks, n_parts, part_len, list_cap, top_lanes, n_tops; size_t state, cut, chunk_sum, group, group_incl, part_max, part_min, tops, bin_cnt, bin_mass, bin_excl, list_a, list_b, total; };
 static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   DrawLayout l;
   // chunks of one tile; of more where a row would have over kMaxChunks of them
@@ -1105,6 +1199,11 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.list_cap = (int)(cols / 4 > 4096 ? cols / 4 : 4096);
   l.part_max = take(sizeof(unsigned) * n_rows * l.n_parts);
   l.part_min = take(sizeof(unsigned) * n_rows * l.n_parts);
+  // maxima for last_bin: up to kTops of a row (kMaxParts * 256 / 64), of four lanes or more
+  l.top_lanes = 4;
+  while (l.n_parts * (256 / l.top_lanes) > kTops) l.top_lanes *= 2;
+  l.n_tops = l.n_parts * (256 / l.top_lanes);
+  l.tops = take(sizeof(unsigned) * n_rows * l.n_tops);
   l.bin_cnt = take(sizeof(unsigned) * n_rows * kBins);
   l.bin_mass = take(sizeof(u64) * n_rows * kBins);
   l.bin_excl = take(sizeof(double) * n_rows * kBins);
@@ -1115,7 +1214,7 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
 }
 template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
   // short rows in one launch; many draws want more than one workgroup
-  if (a.n_cols <= kRowCols && a.n_draws <= 4096) {
+  if (a.n_cols <= kRowCols && a.n_draws <= kRowDraws) {
     hipLaunchKernelGGL(k_draw_row<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
     return;
   }
@@ -1170,9 +1269,11 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.group_incl = (double*)(w + l.group_incl);
   a.n_chunks = l.n_chunks; a.chunk = l.chunk;
   a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
+  a.tops = (unsigned*)(w + l.tops); a.top_lanes = l.top_lanes; a.n_tops = l.n_tops;
   a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
   a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
   a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
+  a.listed_draws = a.cuts && a.n_cols > kRowCols && a.n_draws <= kRowDraws;
   // Draws to a workgroup: its start costs a pass over the row's running sums, so several to a thread once the card is full (two
   // workgroups on each of 256 CUs).
   a.pick_len = kPickThreads;

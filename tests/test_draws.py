@@ -120,7 +120,8 @@ def _check(scores, u, mask=None, where="", dev="cuda", **par):
         want, p = DO.draws(scores[r].double().numpy(), u[r].numpy(), mask=m, **cut)
         bad = np.flatnonzero(idx[r] != want)
         assert bad.size == 0, (where, r, bad[:5], idx[r][bad[:5]], want[bad[:5]], u[r][bad[:5]], cut)
-        assert np.all(np.abs(prob[r] - p) <= 1.001 * 2.0 ** -24 * p), (where, r)
+        # half a step is 2^-24 of the value down to 2^-126; below, where fp32's steps are 2^-149 wide, it is 2^-150
+        assert np.all(np.abs(prob[r] - p) <= 1.001 * np.maximum(2.0 ** -24 * p, 2.0 ** -150)), (where, r)
     return idx
 
 
@@ -358,3 +359,31 @@ def test_wide_and_narrow_ranges():
     for t in (1.0, float("inf"), 1e-300, 1e300):
         for cut in (dict(top_p=0.5), dict(top_k=7), dict(top_k=3000, top_p=0.9)):
             _check(s, u, where=f"inf {t} {cut}", temperature=t, **cut)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_few_entries_kept_of_long_rows(dtype):
+    """Rows of which up to 1 024 entries are in question, and just over that: a limit on the count, on the mass of a sharp row, both,
+    a floor, no temperature; with masks; ties that straddle the limit; few draws and very many."""
+    R, V = 9, 30011
+    s = _scores(R, V, dtype, seed=5, spread=3.0)
+    s[7] = torch.randint(0, 40, (V,), generator=torch.Generator().manual_seed(6)).to(s.dtype)       # some 750 entries to a score
+    s[8, :] = -4.0
+    s[8, 17::101] = 2.0                                                                             # 297 equal ones above the rest
+    mask = torch.rand(R, V, generator=torch.Generator().manual_seed(7)) < 0.5
+    mask[3] = False
+    mask[4] = False
+    mask[4, 29999] = True
+    u = torch.rand(R, 33, generator=torch.Generator().manual_seed(8))
+    u[:, 0], u[:, 1] = 0.0, 1.0 - 2.0 ** -24
+    k = torch.tensor([1, 2, 200, 1024, 1025, 900, 0, 760, 300], dtype=torch.int32)
+    p = torch.tensor([0.9, 0.5, 0.95, 1.0, 1.0, 0.999, 0.6, 0.97, 0.5])
+    t = torch.tensor([1.0, 0.7, 0.9, 1.3, 0.8, 2.0, 0.2, 0.9, 1.0])
+    m = torch.tensor([0.0, 0.1, 0.02, 0.0, 0.0, 1e-4, 0.0, 0.0, 0.0])
+    for kw in (dict(top_k=k, temperature=t), dict(top_k=k, top_p=p, temperature=t, min_p=m), dict(top_p=p, temperature=0.15), dict(top_k=297), dict(top_k=298),
+               dict(top_k=V, top_p=p), dict(temperature=0.0), dict(top_k=5000, top_p=0.9)):
+        few = _check(s, u, where=str(kw), **kw)
+        _check(s, u, mask=mask, where="masked " + str(kw), **kw)
+        many, _ = frame_ops.draw_indices(s.cuda(), u.repeat(1, 150).cuda(), with_prob=True, **{a: b.cuda() if torch.is_tensor(b) else b for a, b in kw.items()})
+        assert np.array_equal(many[:, -33:].cpu().numpy(), few), kw
