@@ -314,7 +314,7 @@ __device__ __forceinline__ int last_bin(const DrawArgs& a, int r, int k, const B
 // Bound: instructions (65 per entry made this 25 us for twelve rows of 816 000), then the LDS atomics: entries are counted
 // only where that is used and weighed only where top-p does, and neighbouring lanes use different copies.
 constexpr int kCopies = 2;
-template <int DT> __global__ __launch_bounds__(512) void k_draw_hist(DrawArgs a) {
+template <int DT> __global__ __launch_bounds__(512, 8) void k_draw_hist(DrawArgs a) {
   __shared__ unsigned cnt[kCopies][kBins];
   __shared__ u64 mass[kCopies][kBins];
   __shared__ double first[kBins];
@@ -620,22 +620,47 @@ template <class Src> __device__ u64 radix_select(const Numbers<Src>& num, bool b
   return mn;
 }
 
-// Up to 1 024 numbers, one to a thread, in descending order (zeros behind them): exchanges inside a wavefront through
-// shuffles, between wavefronts through LDS.
+// A wavefront's values at the lane whose number differs in bit J: by moves between lanes of a row of 16, by swaps of rows and
+// halves beyond (a shuffle goes through the LDS unit and takes several times as long; the sorts below are chains of these).
+template <int J> __device__ __forceinline__ unsigned xor_lane(unsigned x) {
+  if constexpr (J == 1) return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true);           // quad_perm 1 0 3 2
+  else if constexpr (J == 2) return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true);      // quad_perm 2 3 0 1
+  else if constexpr (J == 4) {
+    const int y = __builtin_amdgcn_mov_dpp((int)x, 0x1b, 0xf, 0xf, true);                                   // quad_perm 3 2 1 0: lane ^ 3
+    return (unsigned)__builtin_amdgcn_mov_dpp(y, 0x141, 0xf, 0xf, true);                                    // row_half_mirror: lane ^ 7
+  } else if constexpr (J == 8) return (unsigned)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xf, 0xf, true);   // row_ror 8
+  else if constexpr (J == 16) {
+    const auto p = __builtin_amdgcn_permlane16_swap(x, x, false, false);                                    // rows 0 0 2 2 and 1 1 3 3
+    return threadIdx.x & 16 ? p[0] : p[1];
+  } else {
+    const auto p = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? p[0] : p[1];
+  }
+}
+template <int J> __device__ __forceinline__ u64 sort_step(u64 x, int k) {
+  const u64 y = (u64)xor_lane<J>((unsigned)(x >> 32)) << 32 | xor_lane<J>((unsigned)x);
+  const bool larger = ((threadIdx.x & J) == 0) == ((threadIdx.x & k) == 0);
+  return (x > y) == larger ? x : y;
+}
+// Up to 1 024 numbers, one to a thread, in descending order (zeros behind them), by a bitonic network: exchanges between
+// wavefronts through LDS.
 __device__ __forceinline__ u64 block_sort(u64 x, int n, u64* lds) {
   const int tid = threadIdx.x;
   for (int k = 2; k < 2 * n && k <= kSorted; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      u64 y;
-      if (j >= 64) {
-        __syncthreads();
-        lds[tid] = x;
-        __syncthreads();
-        y = lds[tid ^ j];
-      } else y = __shfl_xor(x, j);
+    for (int j = k >> 1; j >= 64; j >>= 1) {
+      __syncthreads();
+      lds[tid] = x;
+      __syncthreads();
+      const u64 y = lds[tid ^ j];
       const bool larger = ((tid & j) == 0) == ((tid & k) == 0);
       x = (x > y) == larger ? x : y;
     }
+    if (k >= 64) x = sort_step<32>(x, k);
+    if (k >= 32) x = sort_step<16>(x, k);
+    if (k >= 16) x = sort_step<8>(x, k);
+    if (k >= 8) x = sort_step<4>(x, k);
+    if (k >= 4) x = sort_step<2>(x, k);
+    x = sort_step<1>(x, k);
   }
   return x;
 }
