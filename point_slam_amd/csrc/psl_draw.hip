@@ -311,8 +311,9 @@ __device__ __forceinline__ int last_bin(const DrawArgs& a, int r, int k, const B
   return s_last;
 }
 
-// Bound: instructions (65 per entry made this 25 us for twelve rows of 816 000), then the LDS atomics: entries are counted
-// only where that is used and weighed only where top-p does, and neighbouring lanes use different copies.
+// Bound: instructions (65 per entry made this 25 us for twelve rows of 816 000, now 18), then the LDS atomics: entries are counted
+// only where that is used and weighed only where top-p does, and neighbouring lanes use different copies.  64 registers, some
+// of them spilled before the loop, let a CU hold all four of its workgroups (68: 20.8 us).
 constexpr int kCopies = 2;
 template <int DT> __global__ __launch_bounds__(512, 8) void k_draw_hist(DrawArgs a) {
   __shared__ unsigned cnt[kCopies][kBins];
@@ -775,8 +776,8 @@ template <int DT> __device__ __forceinline__ u64 find_threshold(const RowView& v
   return thr;
 }
 // The draws of a row whose n entries up to the last bin of its limits are all in one list: sorted by score they give the
-// threshold, sorted by index the running sums.  What k_draw_sums and k_draw_pick do for it otherwise is two passes over the row
-// (TIME).
+// threshold, sorted by index the running sums.  (64 x 131 072 bf16, a draw of each row: this makes k_draw_cut 3 us longer and takes
+// 14 us out of k_draw_sums and k_draw_pick, which have nothing left to do for the row.)
 __device__ __forceinline__ void draw_from_list(const DrawArgs& a, int r, const DrawCut& c, const RowPar& par, CutShared& S, double* run) {
   const int tid = threadIdx.x, n = (int)c.n_all;
   const bool cut_k = c.k_bin < kBins, cut_p = c.p < 1.0;
@@ -923,7 +924,8 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
 // ---------------------------------------------------------------- the draws
 // A workgroup holds its row's running sums in LDS, at the end of every group if they fit, so that a draw searches there and
 // then reads two lines: its group's, and the scores of one block.  Bound: these scattered lines -- about one request per
-// clock and L2 channel; a search in global memory made twelve of them (82 us for 1.5 M draws).  The workgroups of a row run
+// clock and L2 channel: 1.5 M draws from twelve rows of 816 000 take 53 us, 5.4 TB/s of group records and
+// blocks of scores (a search in global memory made twelve requests of them, 82 us).  The workgroups of a row run
 // on one XCD (consecutive ones are dealt out to the eight in turn), whose L2 then holds the row.
 constexpr int kPlaces = 6656, kPickThreads = 1024;      // 52 KB: groups of 850 000 entries
 template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick(DrawArgs a) {
@@ -1060,8 +1062,8 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
 
 // ---------------------------------------------------------------- short rows: everything by one workgroup
 // The same steps with the row in registers (up to 16 entries to a thread), all else in LDS: one launch instead of seven,
-// whose starts and first loads are what a short row costs (1 x 2 048: 32 us in seven, 13 us in one).
-constexpr int kRowCols = 16384, kRowList = 1024, kRowDraws = 4096;
+// whose starts and first loads are what a short row costs.
+constexpr int kRowCols = 16384, kRowList = 1024;
 struct RowShared {
   union { unsigned cnt[kBins]; double running[kBins]; };          // bin counts, later the blocks' running sums (kRowCols / kBlock = kBins)
   union { u64 mass[kBins]; double cum[kBins]; };
@@ -1211,13 +1213,17 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.chunk_sum = take(sizeof(double) * n_rows * l.n_chunks);
   l.group = take(sizeof(DrawGroup) * n_rows * l.n_chunks * (l.chunk / kGroup));
   l.group_incl = take(sizeof(double) * n_rows * l.n_chunks * (l.chunk / kGroup));
-  // Parts: up to 1 024 workgroups over all rows (four of 512 threads on each of 256 CUs: one round), but no part below 8 192 entries (a workgroup adds up to 1 024 bins to the
-  // row's, which costs what reading some thousand entries does).
+  // Parts: up to 1 024 workgroups over all rows (four of 512 threads on each of 256 CUs: one round; 5 000 draws with
+  // top-p from each of twelve rows of 816 000: 94 us, with 512 or 2 048 workgroups 100).  No part below 2 048 entries, and no
+  // more than 96 parts below 8 192: a workgroup adds up to 1 024 bins to its row's.  (One row of 131 072, top-k and top-p: 28 us in
+  // parts of 2 048, 29 of 4 096, 34 of 8 192; four of 307 200, top-p: 52, 48, 48.)
   const long long cols = n_cols > 0 ? n_cols : 1;
+  long long most = (cols + 8191) / 8192 > 96 ? (cols + 8191) / 8192 : 96;
+  if (most > (cols + 2047) / 2048) most = (cols + 2047) / 2048;
+  if (most > kMaxParts) most = kMaxParts;
   long long parts = 1024 / (n_rows > 0 ? n_rows : 1);
   if (parts < 1) parts = 1;
-  if (parts > (cols + 8191) / 8192) parts = (cols + 8191) / 8192;
-  if (parts > kMaxParts) parts = kMaxParts;
+  if (parts > most) parts = most;
   l.part_len = (int)(((cols + parts - 1) / parts + 2047) / 2048 * 2048);
   l.n_parts = (int)((cols + l.part_len - 1) / l.part_len);
   // Lists hold a quarter of a row: more entries in one bin mean that many equal scores, and then the row itself is read.
@@ -1238,8 +1244,10 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   return l;
 }
 template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
-  // short rows in one launch; many draws want more than one workgroup
-  if (a.n_cols <= kRowCols && a.n_draws <= kRowDraws) {
+  // Short rows in one launch (1 x 2 048, top-k and top-p: 18 us, in seven 27; 256 x 16 384: 26 and 39).  A row's draws are then
+  // one workgroup's: without limits, where three launches would do, up to 1 024 of them (1 x 16 384: 18 and 21 us; for 2 048 24 and
+  // 21), with limits up to 4 096 (1 x 16 384, both: 30 and 35 us; for 16 384 46 and 42).
+  if (a.n_cols <= kRowCols && a.n_draws <= (a.cuts ? 4096 : 1024)) {
     hipLaunchKernelGGL(k_draw_row<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
     return;
   }
@@ -1298,17 +1306,19 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
   a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
   a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
-  a.listed_draws = a.cuts && a.n_cols > kRowCols && a.n_draws <= kRowDraws;
+  // A row's workgroup draws from its list: 64 x 131 072 with top-k and top-p, one draw of each: 42 us, by sums and k_draw_pick 59; for
+  // 16 384 draws 52 and 84; of a single row 43 and 43, and more draws want more workgroups.
+  a.listed_draws = a.cuts && a.n_draws <= 16384;
   // Draws to a workgroup: its start costs a pass over the row's running sums, so several to a thread once the card is full (two
-  // workgroups on each of 256 CUs).
+  // workgroups on each of 256 CUs): twelve rows of 816 000, 124 800 draws of each: 83 us, with one to a thread 91.
   a.pick_len = kPickThreads;
   while (a.pick_len < 16 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len >= 512) a.pick_len += kPickThreads;
   a.pick_wgs = (int)((a.n_draws + a.pick_len - 1) / a.pick_len);
-  // Places in LDS: every group's end if they fit, else every second, fourth ...; few draws do not repay filling them and start
-  // from the chunks.
+  // Places in LDS: every group's end if they fit, else every second, fourth ...  Fewer draws than twice the groups do not repay
+  // filling them and start from the chunks (twelve rows of 816 000: 48 and 47 us for 1 024 draws of each, 69 and 76 for 65 536).
   const int per_chunk = a.chunk / kGroup;
   a.place_groups = 1;
-  while ((long long)a.n_chunks * (per_chunk / a.place_groups) > (a.n_draws > 64 ? kPlaces : a.n_chunks))
+  while ((long long)a.n_chunks * (per_chunk / a.place_groups) > (a.n_draws / 2 > a.n_cols / kGroup ? kPlaces : a.n_chunks))
     a.place_groups = per_chunk % (2 * a.place_groups) == 0 ? 2 * a.place_groups : per_chunk;
   hipStream_t s = (hipStream_t)stream;
   if (q->dtype == PSL_F32) launch_draw<PSL_F32>(a, s);

@@ -385,5 +385,14 @@ def test_few_entries_kept_of_long_rows(dtype):
                dict(top_k=V, top_p=p), dict(temperature=0.0), dict(top_k=5000, top_p=0.9)):
         few = _check(s, u, where=str(kw), **kw)
         _check(s, u, mask=mask, where="masked " + str(kw), **kw)
-        many, _ = frame_ops.draw_indices(s.cuda(), u.repeat(1, 150).cuda(), with_prob=True, **{a: b.cuda() if torch.is_tensor(b) else b for a, b in kw.items()})
-        assert np.array_equal(many[:, -33:].cpu().numpy(), few), kw
+        for times in (150, 600):                     # from the list still, and by sums over the row
+            many, _ = frame_ops.draw_indices(s.cuda(), u.repeat(1, times).cuda(), with_prob=True, **{a: b.cuda() if torch.is_tensor(b) else b for a, b in kw.items()})
+            assert np.array_equal(many[:, -33:].cpu().numpy(), few) and np.array_equal(many[:, :33].cpu().numpy(), few), kw
+
+
+@gpu
+@pytest.mark.parametrize("V,n", [(2048, 1024), (2048, 1025), (16384, 4096), (16384, 4097), (16385, 1), (40000, 622), (40000, 626), (40000, 16384), (40000, 16385)])
+def test_both_sides_of_each_limit_between_forms(V, n):
+    s, u = _scores(2, V, "f32", seed=V), torch.rand(2, n, generator=torch.Generator().manual_seed(n))
+    for cut in (dict(), dict(top_k=90), dict(top_p=0.9), dict(top_k=2000, top_p=0.99, min_p=1e-4)):
+        _check(s, u, where=str(cut), **cut)
