@@ -78,6 +78,8 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     if u.dim() != 2 or u.dtype != torch.float32 or u.shape[0] != R or u.device != dev:
         raise ValueError(f"u: float32 [{R}, draws] on {dev}, got {tuple(u.shape)} {u.dtype} on {u.device}")
     n = u.shape[1]
+    if R > 65535 or V > 0x7f000000 or n > 0x7fffffff:
+        raise ValueError(f"{R} rows of {V} entries, {n} draws: up to 65535 rows of {0x7f000000} entries, {0x7fffffff} draws")
     if V > 1 and scores.stride(1) != 1:
         scores = scores.contiguous()
     if n > 1 and u.stride(1) != 1:

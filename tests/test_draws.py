@@ -82,6 +82,9 @@ def test_python_refusals():
         a.update(kw)
         with pytest.raises(ValueError):
             frame_ops.draw_indices(**a)
+    for S, U in (((1, 2 ** 32 + 5), (1, 3)), ((1, 5), (1, 2 ** 32 + 5)), ((65536, 5), (65536, 1))):      # sizes that a 32-bit field would wrap
+        with pytest.raises(ValueError, match="up to 65535 rows"):
+            frame_ops.draw_indices(torch.zeros(1, 1).expand(S), torch.zeros(1, 1).expand(U))
     with pytest.raises(_lib.PslError):
         frame_ops.draw_indices(s, u)                                  # no host fallback
 
