@@ -964,7 +964,9 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
   __syncthreads();
   const double total = chunk_incl[kMaxChunks - 1];
   const RowView v = row_view<DT>(a, r);
-  const float per_octave = (float)(st.inv_t * 1.4426950408889634);
+  const double per_total = 1.0 / total;             // (a probability is off by this one's rounding and the product's, 2^-52, and by fp32's)
+  const float per_score = (float)(st.inv_t * 1.4426950408889634);
+  const float per_octave = per_score >= 1e-37f ? per_score : __builtin_nanf("");      // (above 0, so that what is not kept is infinitely far; else fp64 decides)
   const DrawGroup* const groups = a.group + g0;
   for (long long d = d0 + tid; d < d1; d += kPickThreads) {
     double u = (double)a.u[(long long)r * a.u_stride + d];
@@ -1016,28 +1018,21 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
 #pragma unroll
     for (int j = 0; j < 4; ++j) f[j] = load_four<DT>(RowView{v.s, nullptr}, i0 + 4 * j, a.n_cols);
     // In fp32 first, weights relative to the block's largest: 16 exponentials of at most one unit of the last place and 15 sums
-    // are within 35 * 2^-24 of the block's mass (x 2^-x <= 0.53 bounds what the rounded exponent does), so a border that
-    // is 2^-18 of it away is on the side it seems to be on.  One draw in ten thousand is not that clear.
-    float top = -__builtin_inff();
+    // are within 35 * 2^-24 of the block's mass (x 2^-x <= 0.53 bounds what the rounded exponent does), the target's share
+    // of it within 6 * 2^-24, so a border that is 2^-18 of it away is on the side it seems to be on.  One draw in ten thousand
+    // is not that clear.
+    float x[16], top = -__builtin_inff();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) if ((kept >> j) & 1u) top = fmaxf(top, f[j >> 2].s[j & 3]);
-    float run[16], sum = 0.f;
+    for (int j = 0; j < 16; ++j) { x[j] = (kept >> j) & 1u ? f[j >> 2].s[j & 3] : -__builtin_inff(); top = fmaxf(top, x[j]); }
+    float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float w = __builtin_amdgcn_exp2f((f[j >> 2].s[j & 3] - top) * per_octave);
-      sum += (kept >> j) & 1u ? w : 0.f;
-      run[j] = sum;
-    }
-    const float share = (float)(in_block / mass) * sum, room = sum * 0x1p-18f;
-    unsigned passed = 0u, near = 0u;
+    for (int j = 0; j < 16; ++j) { sum += __builtin_amdgcn_exp2f((x[j] - top) * per_octave); x[j] = sum; }
+    const float share = (float)in_block * __builtin_amdgcn_rcpf((float)mass) * sum, room = sum * 0x1p-18f;
+    // (the sums never fall: as many borders as lie in front of the target's)
+    int at = 0, far = 0;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      passed |= (run[j] > share ? 1u : 0u) << j;
-      near |= (fabsf(run[j] - share) <= room ? 1u : 0u) << j;
-    }
-    passed &= kept;
-    int at = __ffs((int)passed) - 1;
-    if (at < 0 || near || !(sum < 1e30f)) {
+    for (int j = 0; j < 16; ++j) { at += x[j] < share - room ? 1 : 0; far += x[j] <= share + room ? 1 : 0; }
+    if (at != far || at > 15 || !(sum < 1e30f)) {
       // in fp64, entry by entry
       double acc = 0.0;
       at = -1;
@@ -1052,10 +1047,11 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
     }
     a.idx[out0 + d] = i0 + at;
     if (a.prob) {
-      float s = f[0].s[0];
+      float s4[4];
 #pragma unroll
-      for (int j = 1; j < 16; ++j) s = at == j ? f[j >> 2].s[j & 3] : s;
-      a.prob[out0 + d] = (float)(weight_of(s, st.M, st.inv_t, s_exp) / total);
+      for (int j = 0; j < 4; ++j) s4[j] = at & 2 ? (at & 1 ? f[j].s[3] : f[j].s[2]) : (at & 1 ? f[j].s[1] : f[j].s[0]);
+      const float s = at & 8 ? (at & 4 ? s4[3] : s4[2]) : (at & 4 ? s4[1] : s4[0]);
+      a.prob[out0 + d] = (float)(weight_of(s, st.M, st.inv_t, s_exp) * per_total);
     }
   }
 }
