@@ -921,12 +921,42 @@ template <int DT> __global__ __launch_bounds__(256) void k_draw_sums(DrawArgs a)
   if (tid == 0) a.chunk_sum[(long long)r * a.n_chunks + blockIdx.x] = carry;
 }
 
+// Records of 16 N bytes, one to a lane, at p.  A load reads whole records, the four lanes of a quad to one, so that a wavefront
+// asks for 16 of them at a time and not for a piece of each of 64; an exchange inside the quad then hands every lane the
+// pieces of its own.  (1.5 M draws from twelve rows of 816 000: 43 us, with every lane loading its own records 51.  Whole quads
+// must be there.)
+template <int CTRL> __device__ __forceinline__ unsigned quad_move(unsigned x) { return (unsigned)__builtin_amdgcn_mov_dpp((int)x, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ const char* quad_move(const char* p) {
+  const u64 b = (u64)(uintptr_t)p;
+  return (const char*)(uintptr_t)((u64)quad_move<CTRL>((unsigned)(b >> 32)) << 32 | quad_move<CTRL>((unsigned)b));
+}
+template <int N> __device__ __forceinline__ void swap_pieces(unsigned (&a)[N], unsigned (&b)[N], bool upper, bool by_two) {
+#pragma unroll
+  for (int w = 0; w < N; ++w) {
+    const unsigned x = a[w], y = b[w];
+    const unsigned ys = by_two ? quad_move<0x4e>(y) : quad_move<0xb1>(y), xs = by_two ? quad_move<0x4e>(x) : quad_move<0xb1>(x);
+    a[w] = upper ? ys : x;
+    b[w] = upper ? y : xs;
+  }
+}
+template <int N> __device__ __forceinline__ void load_records(const char* p, unsigned (&x)[4][N]) {
+  const int q = threadIdx.x & 3;
+  __builtin_memcpy(x[0], quad_move<0x00>(p) + 4 * N * q, 4 * N);
+  __builtin_memcpy(x[1], quad_move<0x55>(p) + 4 * N * q, 4 * N);
+  __builtin_memcpy(x[2], quad_move<0xaa>(p) + 4 * N * q, 4 * N);
+  __builtin_memcpy(x[3], quad_move<0xff>(p) + 4 * N * q, 4 * N);
+  swap_pieces<N>(x[0], x[1], q & 1, false);
+  swap_pieces<N>(x[2], x[3], q & 1, false);
+  swap_pieces<N>(x[0], x[2], q & 2, true);
+  swap_pieces<N>(x[1], x[3], q & 2, true);
+}
+
 // ---------------------------------------------------------------- the draws
 // A workgroup holds its row's running sums in LDS, at the end of every group if they fit, so that a draw searches there and
-// then reads two lines: its group's, and the scores of one block.  Bound: these scattered lines -- about one request per
-// clock and L2 channel: 1.5 M draws from twelve rows of 816 000 take 53 us, 5.4 TB/s of group records and
-// blocks of scores (a search in global memory made twelve requests of them, 82 us).  The workgroups of a row run
-// on one XCD (consecutive ones are dealt out to the eight in turn), whose L2 then holds the row.
+// then reads two lines: its group's, and the scores of one block.  Bound: instructions (700 a wavefront of draws, 28 us of
+// issue for 1.5 M draws from twelve rows of 816 000, which take 43) and these scattered lines (a search in global memory made
+// twelve of them, 82 us).  The workgroups of a row run on one XCD (consecutive ones are dealt out to the eight in turn), whose
+// L2 then holds most of the row.
 constexpr int kPlaces = 6656, kPickThreads = 1024;      // 52 KB: groups of 850 000 entries
 template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick(DrawArgs a) {
   __shared__ double place[kPlaces];        // running sums inside a chunk, as group_incl
@@ -968,8 +998,10 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
   const float per_score = (float)(st.inv_t * 1.4426950408889634);
   const float per_octave = per_score >= 1e-37f ? per_score : __builtin_nanf("");      // (above 0, so that what is not kept is infinitely far; else fp64 decides)
   const DrawGroup* const groups = a.group + g0;
-  for (long long d = d0 + tid; d < d1; d += kPickThreads) {
-    double u = (double)a.u[(long long)r * a.u_stride + d];
+  // (whole wavefronts stay: lanes load for one another.  A lane without a draw of its own finds the one of u = 0.)
+  for (long long first = d0 + (tid & ~63); first < d1; first += kPickThreads) {
+    const long long d = first + lane;
+    double u = d < d1 ? (double)a.u[(long long)r * a.u_stride + d] : 0.0;
     u = u > 0.0 ? (u < 1.0 ? u : 1.0 - 0x1p-24) : 0.0;
     const double target = u * total;                 // below the total: the last chunk passes it
     int ch = 0, hi = nc - 1;
@@ -990,7 +1022,11 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
     }
     double incl[8];
     uint4 bits;
-    __builtin_memcpy(incl, groups[g].incl, 64);
+    {
+      unsigned x[4][4];
+      load_records<4>((const char*)(groups + g), x);
+      __builtin_memcpy(incl, x, 64);
+    }
     __builtin_memcpy(&bits, groups[g].kept, 16);
     int b = 0;
     double back = incl[0];
@@ -1015,8 +1051,22 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
     }
     const int i0 = block * kBlock;
     Four<DT> f[4];
+    constexpr int es = DT == PSL_F32 ? 4 : 2;
+    unsigned raw[4][es];                              // (two bytes to an entry: pieces of eight bytes)
+    if (__any(i0 + kBlock > a.n_cols)) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = load_four<DT>(RowView{v.s, nullptr}, i0 + 4 * j, a.n_cols);
+      for (int j = 0; j < 4; ++j) f[j] = load_four<DT>(RowView{v.s, nullptr}, i0 + 4 * j, a.n_cols);
+    } else {
+      load_records<es>((const char*)v.s + (long long)i0 * es, raw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (DT == PSL_F32) f[j].s[k] = __uint_as_float(raw[j][k]);
+          else if constexpr (DT == PSL_BF16) f[j].s[k] = __uint_as_float(k & 1 ? raw[j][k >> 1] & 0xffff0000u : raw[j][k >> 1] << 16);
+          else { const unsigned short h = (unsigned short)(raw[j][k >> 1] >> (16 * (k & 1))); _Float16 x; __builtin_memcpy(&x, &h, 2); f[j].s[k] = (float)x; }
+        }
+    }
     // In fp32 first, weights relative to the block's largest: 16 exponentials of at most one unit of the last place and 15 sums
     // are within 35 * 2^-24 of the block's mass (x 2^-x <= 0.53 bounds what the rounded exponent does), the target's share
     // of it within 6 * 2^-24, so a border that is 2^-18 of it away is on the side it seems to be on.  One draw in ten thousand
@@ -1045,8 +1095,8 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
         }
       }
     }
-    a.idx[out0 + d] = i0 + at;
-    if (a.prob) {
+    if (d < d1) a.idx[out0 + d] = i0 + at;
+    if (d < d1 && a.prob) {
       float s4[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) s4[j] = at & 2 ? (at & 1 ? f[j].s[3] : f[j].s[2]) : (at & 1 ? f[j].s[1] : f[j].s[0]);
@@ -1306,7 +1356,7 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   // 16 384 draws 52 and 84; of a single row 43 and 43, and more draws want more workgroups.
   a.listed_draws = a.cuts && a.n_draws <= 16384;
   // Draws to a workgroup: its start costs a pass over the row's running sums, so several to a thread once the card is full (two
-  // workgroups on each of 256 CUs): twelve rows of 816 000, 124 800 draws of each: 83 us, with one to a thread 91.
+  // workgroups on each of 256 CUs): twelve rows of 816 000, 124 800 draws of each, nothing cut: 83 us, with one to a thread 91.
   a.pick_len = kPickThreads;
   while (a.pick_len < 16 * kPickThreads && (long long)a.n_rows * a.n_draws / a.pick_len >= 512) a.pick_len += kPickThreads;
   a.pick_wgs = (int)((a.n_draws + a.pick_len - 1) / a.pick_len);
