@@ -360,7 +360,8 @@ int psl_keyframe_overlap_sync(const float* rays_o, const float* rays_d, const fl
  *   psl_rows_write : values[i] -> row rows[i] (or first + i when rows is NULL).  Ids outside [0, capacity) write nothing
  *                    (padding: -1).  The same id more than once: with `owner` ([capacity] int32 scratch, any contents) the
  *                    largest i wins; with owner NULL the caller vouches that the ids are distinct.
- *   psl_rows_read  : the values of row rows[i] -> values[i], rounded once to dtype; ids outside [0, capacity) give zeros.
+ *   psl_rows_read  : the values of row rows[i] -> values[i], fp32 products converted to dtype; ids outside
+ *                    [0, capacity) give zeros.
  * Rows that are not named stay as they were.  heads, dim <= 4096; group <= 1024 divides dim (even for int4);
  * n, capacity < 2^31; strides up to 2^29.  The codes of a group with scale NaN mean nothing. */
 enum psl_dtype { PSL_F32 = 0, PSL_BF16 = 1, PSL_F16 = 2 };

@@ -330,7 +330,12 @@ __global__ __launch_bounds__(256) void k_rows_read(RowsArgs a, FastDiv chunks, u
     const float s = *scale_at(a, p);
     decode<FMT, VEC>(codes_at<Code<FMT>::bits>(a, p) + (c * (unsigned)VEC * Code<FMT>::bits >> 3), y);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) y[k] *= s;
+    for (int k = 0; k < VEC; ++k) {
+      y[k] *= s;
+      // an fp32 number, then converted: one instruction for both (the compiler's choice for fp16, element by element) rounds the
+      // exact product instead, and a value would depend on the width of the pieces
+      asm("" : "+v"(y[k]));
+    }
   } else {
 #pragma unroll
     for (int k = 0; k < VEC; ++k) y[k] = 0.f;
