@@ -778,10 +778,10 @@ template <int DT> __device__ __forceinline__ u64 find_threshold(const RowView& v
 // The draws of a row whose n entries up to the last bin of its limits are all in one list: sorted by score they give the
 // threshold, sorted by index the running sums.  (64 x 131 072 bf16, a draw of each row: this makes k_draw_cut 3 us longer and takes
 // 14 us out of k_draw_sums and k_draw_pick, which have nothing left to do for the row.)
-__device__ __forceinline__ void draw_from_list(const DrawArgs& a, int r, const DrawCut& c, const RowPar& par, CutShared& S, double* run) {
+__device__ __forceinline__ void draw_from_list(const DrawArgs& a, int r, const u64* list, const DrawCut& c, const RowPar& par, CutShared& S, double* run) {
   const int tid = threadIdx.x, n = (int)c.n_all;
   const bool cut_k = c.k_bin < kBins, cut_p = c.p < 1.0;
-  u64 x = block_sort(tid < n ? a.list_a[(long long)r * a.list_cap + tid] : 0ull, n, S.sort);
+  u64 x = block_sort(tid < n ? list[tid] : 0ull, n, S.sort);
   const double w = x ? weight_of(score_of((unsigned)(x >> 32)), c.M, c.inv_t, S.sh.exp) : 0.0;
   int end = cut_k ? par.k : n;
   if (cut_p) {
@@ -824,7 +824,7 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_cut(DrawArgs a)
   __syncthreads();
   if (c.n_all) {
     if (threadIdx.x == 0) a.state[r].drawn = 1;
-    draw_from_list(a, r, c, row_par(a, r), S, run);
+    draw_from_list(a, r, a.list_a + (long long)r * a.list_cap, c, row_par(a, r), S, run);
     return;
   }
   u64 thr = 1ull << 32;
@@ -1155,15 +1155,42 @@ template <int DT> __global__ __launch_bounds__(1024) void k_draw_row(DrawArgs a)
   if (has_cut(par)) {
     const Range g{mx, mn};
     const Binning b = make_binning(g, par.inv_t, a.n_cols);
-    const bool weigh = par.p < 1.0 && par.k != 1, count = par.k > 0;
-    if (weigh) S.first[tid] = first_weight(b, tid);
-    __syncthreads();
+    const bool weigh = par.p < 1.0 && par.k != 1;
     const BinPoly poly = make_bin_poly();
+    unsigned c = 0u;
+    if (par.k > 0) {
+      // Top-k by itself first: where it leaves few entries, a list of them is all that the rest needs, and no mass is.  (1 x 2 048, top-k
+      // and top-p: 50 entries 14.8 us, 20.6 by masses, bins and sums; 800 entries 21.3 and 21.9.  Top-k alone, which weighs nothing
+      // on the way: 100 entries 14.5 and 15.8, 400 18.4 and 16.1.)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) add_to_bins<false>(f[j], b, poly, count, weigh, kBins - 1, S.cnt, S.mass, S.first);
-    __syncthreads();
-    const unsigned c = S.cnt[tid];
-    const double m = ldexp((double)S.mass[tid], -bin_shift(b, tid));
+      for (int j = 0; j < 4; ++j) add_to_bins<false>(f[j], b, poly, true, false, kBins - 1, S.cnt, S.mass, S.first);
+      __syncthreads();
+      c = S.cnt[tid];
+      find_bins(a, par, g, b, c, 0.0, S.cum, S.excl, &S.c, S.bins);
+      __syncthreads();
+      if (S.c.k_bin < kBins && S.c.n_all && (weigh || S.c.n_all <= 128u)) {
+        const int k_bin = S.c.k_bin;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const unsigned k = four_key(f[j], q);
+            if (k && bin_of(b, score_of(k)) <= k_bin) S.la[atomicAdd(&S.n_a, 1u)] = number_of(k, j * 4096 + tid * 4 + q);
+          }
+        __syncthreads();
+        draw_from_list(a, r, S.la, S.c, par, S.cut, S.running);
+        return;
+      }
+      S.mass[tid] = 0ull;
+    }
+    if (weigh) {
+      S.first[tid] = first_weight(b, tid);
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) add_to_bins<false>(f[j], b, poly, false, true, kBins - 1, S.cnt, S.mass, S.first);
+      __syncthreads();
+    }
+    const double m = weigh ? ldexp((double)S.mass[tid], -bin_shift(b, tid)) : 0.0;
     __syncthreads();
     find_bins(a, par, g, b, c, m, S.cum, S.excl, &S.c, S.bins);
     __syncthreads();
@@ -1290,7 +1317,7 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   return l;
 }
 template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
-  // Short rows in one launch (1 x 2 048, top-k and top-p: 18 us, in seven 27; 256 x 16 384: 26 and 39).  A row's draws are then
+  // Short rows in one launch (1 x 2 048, top-k and top-p: 15 us, in seven 27; 256 x 16 384: 26 and 39).  A row's draws are then
   // one workgroup's: without limits, where three launches would do, up to 1 024 of them (1 x 16 384: 18 and 21 us; for 2 048 24 and
   // 21), with limits up to 4 096 (1 x 16 384, both: 30 and 35 us; for 16 384 46 and 42).
   if (a.n_cols <= kRowCols && a.n_draws <= (a.cuts ? 4096 : 1024)) {
