@@ -994,7 +994,7 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
   __syncthreads();
   const double total = chunk_incl[kMaxChunks - 1];
   const RowView v = row_view<DT>(a, r);
-  const double per_total = 1.0 / total;             // (a probability is off by this one's rounding and the product's, 2^-52, and by fp32's)
+  const double per_total = 1.0 / total;
   const float per_score = (float)(st.inv_t * 1.4426950408889634);
   const float per_octave = per_score >= 1e-37f ? per_score : __builtin_nanf("");      // (above 0, so that what is not kept is infinitely far; else fp64 decides)
   const DrawGroup* const groups = a.group + g0;
@@ -1101,7 +1101,8 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
 #pragma unroll
       for (int j = 0; j < 4; ++j) s4[j] = at & 2 ? (at & 1 ? f[j].s[3] : f[j].s[2]) : (at & 1 ? f[j].s[1] : f[j].s[0]);
       const float s = at & 8 ? (at & 4 ? s4[3] : s4[2]) : (at & 4 ? s4[1] : s4[0]);
-      a.prob[out0 + d] = (float)(weight_of(s, st.M, st.inv_t, s_exp) * per_total);
+      const double w = weight_of(s, st.M, st.inv_t, s_exp), p = w * per_total;
+      a.prob[out0 + d] = (float)fma(fma(-p, total, w), per_total, p);      // the quotient, by its remainder
     }
   }
 }
