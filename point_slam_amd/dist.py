@@ -45,7 +45,8 @@ rank-invariant; bench.py --merge reports the render loss after the exchange unde
 Feature rows on the wire (`wire=`): None sends fp32 as above; "int8", "e4m3" or "int4" sends the feature rows of new points and
 the changes of touched rows as codes with one fp32 scale to a row (row_store.write_records: int8 88 B instead of 272 B per
 point, 76 B instead of 260 B per row).  Every rank, the sender included, goes on with what the codes stand for, so replicas
-stay identical; positions, radii, row ids and the decoder stay fp32.
+stay identical; positions, radii, row ids and the decoder stay fp32.  Like `merge`, it has to be the same on every rank: it sets
+the width of the records.
 """
 from __future__ import annotations
 
