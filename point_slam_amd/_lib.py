@@ -242,9 +242,10 @@ def call_on(device, entry: str, args):
     current one.  The raw stream is asked for directly; a torch.cuda.Stream object per call costs as much as a launch."""
     import torch
     fn = getattr(lib(), entry)
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    if device.index is None or device.index == torch.cuda.current_device():
-        stream = raw(torch.cuda.current_device()) if raw is not None else torch.cuda.current_stream().cuda_stream
+    here = torch.cuda.current_device()
+    if device.index is None or device.index == here:
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        stream = raw(here) if raw is not None else torch.cuda.current_stream().cuda_stream
         return check(fn(C.byref(args), stream), entry)
     with torch.cuda.device(device):
         return check(fn(C.byref(args), torch.cuda.current_stream().cuda_stream), entry)

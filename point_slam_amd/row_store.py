@@ -36,15 +36,15 @@ def _check_layout(heads, dim, fmt, group):
 
 def _call(entry, values, rows, first, n, fmt, group, capacity, codes, codes_row_stride, scales, scales_row_stride, owner=None):
     """One psl_rows_* call.  values [n, heads, dim], rows ids or None; codes / scales: tensors whose data_ptr is row 0."""
-    if values.device.type != "cuda":
-        raise _lib.PslError(f"{entry}: tensors on {values.device}; the kernels run on the GPU and have no host fallback")
-    a = _lib.psl_rows_args(format=FORMATS[fmt], dtype=_DTYPES[values.dtype], heads=values.shape[1], dim=values.shape[2],
-                           group=group, rows_bits=0 if rows is None else rows.element_size() * 8, n=n, capacity=capacity,
-                           first=first, rows=None if rows is None else rows.data_ptr(), values=values.data_ptr(),
-                           value_row_stride=values.stride(0), value_head_stride=values.stride(1), codes=codes.data_ptr(),
-                           codes_row_stride=codes_row_stride, scales=scales.data_ptr(), scales_row_stride=scales_row_stride,
-                           owner=None if owner is None else owner.data_ptr())
-    _lib.call_on(values.device, entry, a)
+    dev = values.device
+    if dev.type != "cuda":
+        raise _lib.PslError(f"{entry}: tensors on {dev}; the kernels run on the GPU and have no host fallback")
+    _, heads, dim = values.shape
+    row, head, _ = values.stride()
+    _lib.call_on(dev, entry, _lib.psl_rows_args(         # in the order of the struct's fields
+        FORMATS[fmt], _DTYPES[values.dtype], heads, dim, group, 0 if rows is None else rows.element_size() * 8, n, capacity, first,
+        None if rows is None else rows.data_ptr(), values.data_ptr(), row, head, codes.data_ptr(), codes_row_stride,
+        scales.data_ptr(), scales_row_stride, None if owner is None else owner.data_ptr()))
 
 
 def record_floats(heads: int, dim: int, fmt: str, group: Optional[int] = None) -> tuple:
@@ -122,7 +122,7 @@ class QuantizedRows:
         """values [n, heads, dim] (fp32, bf16 or fp16) into rows `rows` [n], or into [first, first + n) when rows is None.
         Ids outside the store (padding: -1) are skipped.  When an id comes more than once the last one wins;
         `distinct=True` vouches that none does and saves that bookkeeping (two launches)."""
-        if values.dtype not in _DTYPES or values.dim() != 3 or tuple(values.shape[1:]) != (self.heads, self.dim):
+        if values.dtype not in _DTYPES or values.dim() != 3 or values.shape[1] != self.heads or values.shape[2] != self.dim:
             raise ValueError(f"values: [n, {self.heads}, {self.dim}] in float32, bfloat16 or float16, got {tuple(values.shape)} {values.dtype}")
         if values.device != self.device:
             raise ValueError(f"values on {values.device}, the store on {self.device}")
