@@ -396,10 +396,12 @@ __device__ __forceinline__ void find_bins(const DrawArgs& a, const RowPar& par, 
   n_incl += n_before; incl += before;
   cum[j] = m > 0.0 ? incl : -1.0;
   excl_out[j] = excl;
-  // (as many as there are: they may be only what was counted, and the limit keeps all of them)
-  const bool cut_k = par.k > 0 && (unsigned)par.k <= n_valid, cut_p = par.p < 1.0 && par.k != 1;
-  if (cut_k && n_incl >= (unsigned)par.k && n_incl - c < (unsigned)par.k) {
-    sh.k = j; sh.want = (unsigned)par.k - (n_incl - c); sh.na = c; sh.most = incl; sh.above_k = excl;
+  // As many as there are, or more: the limit keeps all of them.  It is looked for all the same where they may be only what was
+  // counted, and where they are few enough for one list.
+  const unsigned k = (unsigned)par.k > n_valid && n_valid <= (unsigned)kSorted ? n_valid : (unsigned)par.k;
+  const bool cut_k = par.k > 0 && k <= n_valid, cut_p = par.p < 1.0 && par.k != 1;
+  if (cut_k && n_incl >= k && n_incl - c < k) {
+    sh.k = j; sh.want = k - (n_incl - c); sh.na = c; sh.most = incl; sh.above_k = excl;
   }
   __syncthreads();
   const int k_bin = sh.k;
@@ -783,7 +785,7 @@ __device__ __forceinline__ void draw_from_list(const DrawArgs& a, int r, const u
   const bool cut_k = c.k_bin < kBins, cut_p = c.p < 1.0;
   u64 x = block_sort(tid < n ? list[tid] : 0ull, n, S.sort);
   const double w = x ? weight_of(score_of((unsigned)(x >> 32)), c.M, c.inv_t, S.sh.exp) : 0.0;
-  int end = cut_k ? par.k : n;
+  int end = cut_k ? min(par.k, n) : n;
   if (cut_p) {
     const double incl = block_running(w, S.wave);
     if (tid == end - 1) { S.kept = incl; S.at = end - 1; }
