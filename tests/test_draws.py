@@ -304,6 +304,31 @@ def test_another_stream_and_captured_graphs():
 
 
 @gpu
+def test_captured_draws_from_long_rows_follow_their_inputs():
+    """Scores and limits change between the replays, and with them the way a row takes: from a list, by sums over the row, empty."""
+    R, V, n = 4, 40000, 50
+    s, u, mask = _scores(R, V, "f32").cuda(), torch.rand(R, n).cuda(), torch.ones(R, V, dtype=torch.bool, device="cuda")
+    k, p = torch.zeros(R, dtype=torch.int32, device="cuda"), torch.ones(R, device="cuda")
+    kw = dict(top_k=k, top_p=p, temperature=0.9, mask=mask, with_prob=True)
+    frame_ops.draw_indices(s, u, **kw)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        idx, prob = frame_ops.draw_indices(s, u, **kw)
+    limits = [([50, 0, 20000, 1], [0.9, 0.5, 1.0, 1.0]), ([0, 0, 0, 0], [1.0, 1.0, 1.0, 1.0]), ([30000, 700, 5, 0], [0.99, 1.0, 0.3, 0.999]),
+              ([1024, 1025, 2000, 1], [1.0, 0.9, 0.9, 0.0])]
+    for j, (kk, pp) in enumerate(limits + limits[:2]):
+        s.copy_(_scores(R, V, "f32", seed=30 + j)); u.uniform_()
+        k.copy_(torch.tensor(kk, dtype=torch.int32)); p.copy_(torch.tensor(pp))
+        mask.fill_(True)
+        mask[j % R] = False if j % 2 else True
+        g.replay()
+        want = frame_ops.draw_indices(s, u, **kw)
+        torch.cuda.synchronize()
+        assert torch.equal(idx, want[0]) and torch.equal(prob, want[1]), j
+        _check(s.cpu(), u.cpu(), mask=mask.cpu(), where=str(j), top_k=k.cpu(), top_p=p.cpu(), temperature=0.9)
+
+
+@gpu
 def test_rows_longer_than_a_thousand_tiles_and_offsets_past_32_bits():
     V = 5_000_001
     s, u = _scores(2, V, "f32"), torch.rand(2, 300)
