@@ -194,13 +194,22 @@ template <int FMT, int VEC> __device__ __forceinline__ void encode(const float (
       }
     }
   } else {
+    // 16 bits of codes at a time as ONE number, q0 + 2^B q1 + ..., made in fp32 with every code raised by half its range: it is below
+    // 2^16, so every product and sum is exact; half a range more is the sign bit turned over.
     constexpr int B = Code<FMT>::bits, PER = (BYTES >= 4 ? 32 : BYTES * 8) / B;      // codes per stored word
+    constexpr int RUN = PER * B > 16 ? 16 / B : PER;
+    constexpr unsigned HALF = B == 4 ? 0x88888888u : 0x80808080u;
 #pragma unroll
     for (int k = 0; k < VEC / PER; ++k) {
       unsigned w = 0;
 #pragma unroll
-      for (int j = 0; j < PER; ++j) w |= ((unsigned)(int)q[k * PER + j] & ((1u << B) - 1u)) << (B * j);
-      r.w[k] = w;
+      for (int h = 0; h < PER / RUN; ++h) {
+        float t = q[k * PER + h * RUN] + (float)(HALF & ((1u << (RUN * B)) - 1u));
+#pragma unroll
+        for (int j = 1; j < RUN; ++j) t = fmaf(q[k * PER + h * RUN + j], (float)(1u << (B * j)), t);
+        w |= (unsigned)t << (16 * h);
+      }
+      r.w[k] = w ^ (PER * B == 32 ? HALF : HALF & ((1u << (PER * B)) - 1u));
     }
   }
   store_raw(dst, r);
