@@ -162,8 +162,11 @@ template <int FMT, int VEC> __device__ __forceinline__ void quotients(const floa
       asm volatile("");            // (a branch: rarely taken)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
+        // above the middle, or on it with an odd code: at least 0 for an odd one, the smallest number above 0 for an even one
+        // (no branch: groups of bf16 reach the middle often enough that half the wavefronts come here)
         const float r = fmaf(-q[k], s, x[k]), h = fmaf(2.f, fabsf(r), -s);
-        if (h > 0.f || (h == 0.f && ((int)q[k] & 1))) q[k] += copysignf(1.f, r);
+        const float least = __uint_as_float(((unsigned)(int)q[k] & 1u) ^ 1u);
+        q[k] += h >= least ? copysignf(1.f, r) : 0.f;
       }
     }
   }
@@ -239,10 +242,15 @@ template <int FMT, int VEC> __device__ __forceinline__ void decode(const unsigne
 // the place of group `unit`: row i of the call (inside this launch), row of the store (-1: none), group u of the row.  Codes and
 // scales of a row's groups lie one behind the other; 32 x 32 -> 64 bit products reach every address.
 struct Place { unsigned i, u; int row; };
-__device__ __forceinline__ Place place_of(const RowsArgs& a, unsigned unit) {
+__device__ __forceinline__ Place place_in_call(const RowsArgs& a, unsigned unit) {
   Place p;
   p.i = fast_div(unit, a.groups_per_row);
   p.u = unit - p.i * a.groups_per_row.d;
+  p.row = -1;
+  return p;
+}
+__device__ __forceinline__ Place place_of(const RowsArgs& a, unsigned unit) {
+  Place p = place_in_call(a, unit);
   p.row = (int)row_of(a, a.i0 + p.i);
   return p;
 }
@@ -294,14 +302,16 @@ __global__ __launch_bounds__(256) void k_rows_write(RowsArgs a) {
   // Whole wavefronts stay for the maximum; a group's lanes are in range together.  Lanes without a group read the first
   // one's values, lanes without a chunk their group's last: what they add to a maximum is in it already or not used.
   const bool in = unit < a.n * a.groups_per_row.d;
-  const Place p = place_of(a, in ? unit : 0u);
+  Place p = place_in_call(a, in ? unit : 0u);
   const unsigned L = 1u << a.lanes_log2, lane = t & (L - 1u);
   float x[ITERS][VEC];
   unsigned top_bits = 0u;         // |x| as bits: ordered like the magnitudes, infinities and NaN above them
   const char* v = values_at(a, p, Elem<DT>::bytes);
 #pragma unroll
+  for (int it = 0; it < ITERS; ++it) load_values<DT, VEC>(v + min(lane + it * L, a.chunks - 1u) * (unsigned)(VEC * Elem<DT>::bytes), x[it]);
+  p.row = (int)row_of(a, a.i0 + p.i);       // (its load behind those of the values: none waits for the other)
+#pragma unroll
   for (int it = 0; it < ITERS; ++it) {
-    load_values<DT, VEC>(v + min(lane + it * L, a.chunks - 1u) * (unsigned)(VEC * Elem<DT>::bytes), x[it]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) top_bits = max(top_bits, __float_as_uint(x[it][k]) & 0x7fffffffu);
   }
