@@ -9,8 +9,8 @@
 //   once more, to four bits, is the rounding of the exact quotient.
 //
 // Bound: memory.  A thread owns VEC consecutive values; the lanes of a group find its maximum by moves between lanes, so a value
-// is read once and lives in registers until its code is stored.  2.5 M rows of 2 x 32 fp32 to 8 bits and back: 140 and 142 us, the
-// 820 MB that they read and write at 5.8 TB/s, where a copy of 256 MiB reaches 5.4.
+// is read once and lives in registers until its code is stored.  2.5 M rows of 2 x 32 fp32 to 8 bits and back: 140 and 142 us
+// each by itself, 164 and 150 in turn -- the 820 MB that each reads and writes at 5.8 and 5.2 TB/s, where a copy of 256 MiB reaches 5.4.
 #include "psl_common.h"
 
 namespace psl {
