@@ -424,3 +424,64 @@ def test_both_sides_of_each_limit_between_forms(V, n):
     s, u = _scores(2, V, "f32", seed=V), torch.rand(2, n, generator=torch.Generator().manual_seed(n))
     for cut in (dict(), dict(top_k=90), dict(top_p=0.9), dict(top_k=2000, top_p=0.99, min_p=1e-4)):
         _check(s, u, where=str(cut), **cut)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("V", [16385, 300000])
+def test_the_smallest_u_where_the_first_entries_weigh_next_to_nothing(V, dtype):
+    """Leading entries 100 and 700 temperatures below the rest -- 4e-44 and 1e-304 of its weight, below what fp32 holds -- and in
+    front of them entries that are not to be drawn: u = 0 (and what is turned into it) takes the first that is."""
+    u = torch.tensor([[0.0, -1.0, float("nan"), 1e-45, 2.0 ** -24, 0.5, 1 - 2.0 ** -24]] * 5)
+    for below in (100.0, 700.0):
+        for lead in (16, 40, 2000):
+            s = _scores(5, V, dtype, seed=V + lead, spread=0.5)
+            s[:, :lead] = -below
+            mask = torch.ones(5, V, dtype=torch.bool)
+            mask[0, 0] = False
+            s[1, :3] = -float("inf")
+            s[2, :17] = float("nan")
+            mask[3, ::16] = False
+            s[4, 0] = float("inf")
+            mask[4, :lead - 1] = False                      # one light entry in its block
+            for cut in (dict(), dict(top_k=V - 5), dict(min_p=1e-306)):
+                first = _check(s, u, mask=mask, where=f"{below} {lead} {cut}", **cut)[:, 0]
+                if cut != dict(top_k=V - 5):
+                    assert first.tolist() == [1, 3, 17, 1, lead - 1], (below, lead, cut)
+            many = frame_ops.draw_indices(s.cuda(), torch.zeros(5, 20000, device="cuda"), mask=mask.cuda())      # places of every group
+            assert (many.cpu() == torch.tensor([1, 3, 17, 1, lead - 1])[:, None]).all()
+
+
+@gpu
+def test_u_on_the_border_of_a_chunk_that_begins_with_light_entries():
+    """Three fifths of a row are equal weights whose sums are exact; u = 1/8 is their sum in front of the second 4 096 entries, where 15
+    entries of e^-100 or e^-700 follow one that is masked."""
+    for below in (100.0, 700.0):
+        s = torch.zeros(1, 5 * 8192)
+        mask = torch.ones(1, 5 * 8192, dtype=torch.bool)
+        s[0, 4096:4112], mask[0, 4096] = -below, False
+        mask[0, 4112 + 28672:] = False                      # 32 768 entries of weight 1
+        idx, prob = frame_ops.draw_indices(s.cuda(), torch.tensor([[0.125]], device="cuda"), mask=mask.cuda(), with_prob=True)
+        # any entry that lies within rounding of the border, and none that is masked
+        assert 4095 <= int(idx) <= 4112 and bool(mask[0, int(idx)]), (below, int(idx))
+        w = 1.0 if int(idx) in (4095, 4112) else np.exp(-below)
+        assert abs(float(prob) - w / 32768) <= 1.001 * max(2.0 ** -24 * w / 32768, 2.0 ** -150)
+
+
+@gpu
+@pytest.mark.parametrize("how", ["masked", "-inf", "nan"])
+def test_u_on_a_border_with_nothing_to_draw_behind_it(how):
+    """Rows of two equal halves with 56 empty blocks between them, the first entry of every block excluded: u = 0.5 lies within
+    rounding of the border, and the running sums of empty blocks are off by a last place in one row of eight.  The draw is the last entry
+    in front or the first behind."""
+    R, V = 400, 20000
+    g = torch.Generator().manual_seed(12)
+    half = torch.randn(R, 1600, generator=g)
+    s, ok = torch.zeros(R, V), torch.zeros(R, V, dtype=torch.bool)
+    for at in (0, 2496):
+        s[:, at:at + 1600], ok[:, at:at + 1600] = half, True
+    ok[:, ::16] = False
+    s[~ok] = {"masked": 3.0, "-inf": -float("inf"), "nan": float("nan")}[how]
+    u = torch.full((R, 3), 0.5)
+    idx = frame_ops.draw_indices(s.cuda(), u.cuda(), mask=ok.cuda() if how == "masked" else None).cpu()
+    assert bool(((idx == 1599) | (idx == 2497)).all()), idx[(idx != 1599) & (idx != 2497)].unique()
