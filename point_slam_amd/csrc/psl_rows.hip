@@ -158,7 +158,7 @@ template <int FMT, int VEC> __device__ __forceinline__ void quotients(const floa
       const float r = fmaf(-q[k], s, x[k]);              // exact: a multiple of the smaller last place, below s
       far = fmaxf(far, fmaf(2.f, fabsf(r), -s));         // above 0: a neighbour is nearer; 0: a tie
     }
-    if (far >= 0.f) {
+    if (far >= 0.f && s > 0.f) {   // (a scale that underflowed to 0: all codes are 0)
       asm volatile("");            // (a branch: rarely taken)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {

@@ -368,3 +368,25 @@ def test_tensors_of_another_device():
     assert _same(st.read().cpu(), _expect(v, "int8", 32, torch.float32)[2])
     with pytest.raises(ValueError):
         st.write(v.to("cuda:0"))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "int4"])
+def test_groups_of_the_smallest_numbers(fmt, dtype):
+    """Groups whose largest value is 0 to 600 times the smallest denormal: where the scale underflows to 0 every code is 0, and what is
+    read is 0 and not -0 in the integer formats; from there on codes are nearest to the quotient by a scale of few bits."""
+    tops = torch.arange(0, 601, dtype=torch.int32)
+    bits = tops[:, None] * torch.tensor([4, 3, 2, 1], dtype=torch.int32) // 4
+    v = (bits.view(torch.float32) if dtype == "f32" else bits.to(torch.int16).view(torch.bfloat16))
+    v = (v * torch.tensor([1, -1, 1, -1], dtype=v.dtype))[:, None, :]
+    assert int((v.float().abs().amax(-1) > 0).sum()) == 600
+    st = QuantizedRows(601, 1, 4, fmt).write(v.cuda())
+    q, s, want = _expect(v, fmt, 4, DT[dtype])
+    assert _same(st.scales.cpu(), s) and (dtype == "bf16" or (s[1:4] == 0).all())
+    assert _same(_decode_codes(st.codes, fmt), q)
+    out = st.read(dtype=DT[dtype]).cpu()
+    assert _same(out.float(), want.float())
+    if fmt != "e4m3":
+        assert (st.codes.cpu()[torch.from_numpy(s[..., 0] == 0)] == 0).all()
+        assert not torch.signbit(out[out == 0]).any()
