@@ -354,7 +354,8 @@ int psl_keyframe_overlap_sync(const float* rays_o, const float* rays_d, const fl
 
 /* ---- feature rows held in 8 or 4 bits (no reference counterpart: the reference keeps every feature in fp32) ----------
  * A row is heads x dim values in groups of `group`; a group stands for code * scale with one fp32 scale = max|x| / Q,
- * Q = 127 (int8), 7 (int4, two codes to a byte, the even one low), 448 (e4m3, OCP); a code is the representable value
+ * Q = 127 (int8), 7 (int4, two codes to a byte, the even one low), 448 (e4m3, OCP), rounded to nearest, or down where Q times
+ * it would not be finite (int8, max|x| = fp32's largest number); a code is the representable value
  * NEAREST to the exact x / scale, ties to even.  A group of zeros has scale 0; a group with an infinite or NaN value has
  * scale NaN and reads back as NaN.  ABI v8.
  *   psl_rows_write : values[i] -> row rows[i] (or first + i when rows is NULL).  Ids outside [0, capacity) write nothing

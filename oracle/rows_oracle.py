@@ -1,10 +1,17 @@
 """Feature rows in 8 or 4 bits restated in float64 numpy from their definition (include/pointslam_hip.h, psl_rows_*): scale =
-fp32(max|x| / Q) per group, code = the representable value nearest to x / scale, ties to even.  The float64 quotient of two
-24-bit numbers is never on a tie that the exact one is not on (they differ by at least 2^-27 of their size), so the codes
-here are THE codes.  Test infrastructure only."""
+fp32(max|x| / Q) per group (rounded down where Q times it would not be finite), code = the representable value nearest to x / scale,
+ties to even.  The float64 quotient of two 24-bit numbers is never on a tie that the exact one is not on (they differ by at
+least 2^-27 of their size), so the codes here are THE codes.  Test infrastructure only."""
 import numpy as np
 
 TOP = {"int8": 127.0, "int4": 7.0, "e4m3": 448.0}
+
+
+def largest_scale(fmt):
+    s = np.finfo(np.float32).max / np.float32(TOP[fmt])
+    while float(s) * TOP[fmt] >= 2.0 ** 128 - 2.0 ** 103:       # what fp32 rounds to infinity
+        s = np.nextafter(s, np.float32(0))
+    return s
 
 
 def nearest_e4m3(q):
@@ -21,7 +28,8 @@ def quantize(x, fmt, group):
     g = x.reshape(n, h, d // group, group)
     top = np.abs(g).max(-1)                                     # NaN stays NaN
     with np.errstate(all="ignore"):
-        s = np.where(np.isfinite(top), (top.astype(np.float32) / np.float32(TOP[fmt])).astype(np.float32), np.float32(np.nan))
+        s = np.minimum((top.astype(np.float32) / np.float32(TOP[fmt])).astype(np.float32), largest_scale(fmt))
+        s = np.where(np.isfinite(top), s, np.float32(np.nan))
         q = g / s.astype(np.float64)[..., None]
         q = np.where((s > 0)[..., None], q, 0.0)
         q = nearest_e4m3(q) if fmt == "e4m3" else np.round(q)

@@ -1,7 +1,7 @@
 // Feature rows held in 8 or 4 bits: quantised as they are written, expanded as they are read.
 //
 // A row is heads x dim values, cut into groups of G; a group shares one fp32 scale s = max|x| / Q (Q = 127 int8, 7 int4,
-// 448 e4m3) and every code is the NEAREST representable value to x / s, ties to even.  fp32's x / s cannot decide that by
+// 448 e4m3; rounded to nearest, down where Q s would not be finite) and every code is the NEAREST representable value to x / s, ties to even.  fp32's x / s cannot decide that by
 // itself: it rounds quotients beside the middle between two codes onto it (with bf16 inputs x = a / 2 that happens in
 // every few rows).  What decides is the residual x - n s, which one fma gives exactly:
 //   integers: n = rint(x / s), and x - n s against s / 2 says whether n is the nearest (it nearly always is);
@@ -131,6 +131,8 @@ template <int DT, int VEC> __device__ __forceinline__ void store_values(char* p,
 template <int FMT> struct Code {
   static constexpr int bits = FMT == PSL_ROWS_INT4 ? 4 : 8;
   static constexpr float top = FMT == PSL_ROWS_INT8 ? 127.f : FMT == PSL_ROWS_INT4 ? 7.f : 448.f;
+  // the largest scale whose product with the largest code is finite: below fl32(largest number / top) for 127, that number for 7 and 448
+  static constexpr float most = FMT == PSL_ROWS_INT8 ? 0x1.020406p+121f : __builtin_inff();
 };
 
 // x / s rounded to odd, sign carried (s > 0, inv = 1 / s to a few units of the last place, the residual not denormal)
@@ -319,7 +321,7 @@ __global__ __launch_bounds__(256) void k_rows_write(RowsArgs a) {
   if (!in || p.row < 0 || (a.owner && a.owner[p.row] != (int)(a.i0 + p.i))) return;
   // an infinite or NaN value makes the whole group NaN: it is not hidden, and nothing finite is made of it
   const float top = __uint_as_float(top_bits);
-  const float s = top_bits < 0x7f800000u ? top / Code<FMT>::top : __builtin_nanf("");
+  const float s = top_bits < 0x7f800000u ? fminf(top / Code<FMT>::top, Code<FMT>::most) : __builtin_nanf("");
   const bool tiny = top < 0x1p-60f && s > 0.f;
   const float inv = s > 0.f ? __builtin_amdgcn_rcpf(s) : 0.f;
   unsigned char* cd = codes_at<Code<FMT>::bits>(a, p);

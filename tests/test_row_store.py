@@ -390,3 +390,22 @@ def test_groups_of_the_smallest_numbers(fmt, dtype):
     if fmt != "e4m3":
         assert (st.codes.cpu()[torch.from_numpy(s[..., 0] == 0)] == 0).all()
         assert not torch.signbit(out[out == 0]).any()
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "e4m3", "int4"])
+def test_groups_of_the_largest_numbers_read_back_finite(fmt):
+    """Up to fp32's largest number, of either sign (what a mask of the type's lowest value is): no finite group reads back as an
+    infinity, and every value is as near as elsewhere."""
+    top = torch.full((40,), torch.finfo(torch.float32).max).view(torch.int32) - torch.arange(40, dtype=torch.int32)
+    v = torch.zeros(40, 1, 8)
+    v[:, 0, 0] = top.view(torch.float32)
+    v[:, 0, 1], v[:, 0, 2], v[:, 0, 3] = -v[:, 0, 0], v[:, 0, 0] / 2, -v[:, 0, 0] / 3
+    v[::2, 0, 0] = 0.0                                        # the negative one by itself
+    st = QuantizedRows(40, 1, 8, fmt).write(v.cuda())
+    q, s, want = _expect(v, fmt, 8, torch.float32)
+    out = st.read().cpu()
+    assert torch.isfinite(out).all() and _same(st.scales.cpu(), s) and _same(_decode_codes(st.codes, fmt), q) and _same(out, want)
+    # half a code step: of the scale for integers, 2^-4 of the value for e4m3; and the product's rounding
+    step = torch.from_numpy(s).double() / 2 if fmt != "e4m3" else v.double().abs() * 2.0 ** -4
+    assert ((out.double() - v.double()).abs() <= step + v.double().abs() * 2.0 ** -23).all()
