@@ -407,8 +407,11 @@ static int run_rows(const char* who, const psl_rows_args* q, bool write, hipStre
   if (q->value_row_stride < 0 || q->value_head_stride < 0 || q->value_row_stride > big || q->value_head_stride > big || q->codes_row_stride > big || q->scales_row_stride > big ||
       q->codes_row_stride < hd * bits / 8 || q->scales_row_stride < hd / q->group)
     PSL_BAD("%s: bad stride", who);
-  if (!write && ((q->heads > 1 && q->value_head_stride < q->dim) || (q->n > 1 && q->value_row_stride < (q->heads - 1) * q->value_head_stride + q->dim)))
-    PSL_BAD("%s: rows of the output overlap", who);
+  // heads inside their row and rows one behind the other, or rows inside their head and heads one behind the other
+  const long long vr = q->value_row_stride, vh = q->value_head_stride;
+  const bool by_row = (q->heads == 1 || vh >= q->dim) && (q->n == 1 || vr >= (q->heads - 1) * vh + q->dim);
+  const bool by_head = (q->n == 1 || vr >= q->dim) && (q->heads == 1 || vh >= (q->n - 1) * vr + q->dim);
+  if (!write && !by_row && !by_head) PSL_BAD("%s: rows of the output overlap", who);
   const uintptr_t pv = (uintptr_t)q->values, pc = (uintptr_t)q->codes, ps = (uintptr_t)q->scales;
   if (pv % es || ps % 4 || (q->rows && (uintptr_t)q->rows % (q->rows_bits / 8))) PSL_BAD("%s: misaligned pointer", who);
   // VEC: the widest piece that divides a group and that every address keeps aligned (16-byte loads of values, code words of

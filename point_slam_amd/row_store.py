@@ -145,7 +145,8 @@ class QuantizedRows:
     def read(self, rows: Optional[torch.Tensor] = None, first: int = 0, count: Optional[int] = None,
              dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The values [n, heads, dim] of rows `rows`, or of [first, first + count) (to the end by default).  Ids outside the
-        store give zeros; the same id may come any number of times."""
+        store give zeros; the same id may come any number of times.  `out` may be strided (rows inside wider records, or
+        [heads, n, dim] memory seen as [n, heads, dim]) as long as no two of its values share memory."""
         if rows is None:
             n = self.capacity - first if count is None else int(count)
             self._range(first, n)

@@ -409,3 +409,29 @@ def test_groups_of_the_largest_numbers_read_back_finite(fmt):
     # half a code step: of the scale for integers, 2^-4 of the value for e4m3; and the product's rounding
     step = torch.from_numpy(s).double() / 2 if fmt != "e4m3" else v.double().abs() * 2.0 ** -4
     assert ((out.double() - v.double()).abs() <= step + v.double().abs() * 2.0 ** -23).all()
+
+
+@gpu
+@pytest.mark.parametrize("fmt", ["int8", "int4"])
+def test_a_read_into_heads_that_follow_one_another(fmt):
+    """[heads, n, dim] memory seen as [n, heads, dim]: a row of one head lies between the heads of another, and none overlap."""
+    v = _values(37, 3, 32, "f32")
+    st = QuantizedRows(37, 3, 32, fmt).write(v.cuda())
+    _, _, want = _expect(v, fmt, 32, torch.float32)
+    for pad in (0, 8):
+        out = torch.full((3, 37, 32 + pad), 7.0, device="cuda")
+        st.read(out=out[:, :, :32].transpose(0, 1))
+        assert _same(out[:, :, :32].transpose(0, 1).cpu(), want) and (out[:, :, 32:] == 7.0).all()
+        rows = torch.tensor([5, -1, 36, 5], device="cuda")
+        few = torch.full((3, 4, 32 + pad), 7.0, device="cuda")
+        st.read(rows=rows, out=few[:, :, :32].transpose(0, 1))
+        expect = want[[5, 0, 36, 5]]
+        expect[1] = 0
+        assert _same(few[:, :, :32].transpose(0, 1).cpu(), expect)
+
+
+def test_outputs_whose_rows_overlap_are_refused_in_either_order():
+    L = _lib.lib()
+    for kw in (dict(value_row_stride=32, value_head_stride=127), dict(value_row_stride=31, value_head_stride=128), dict(value_row_stride=0, value_head_stride=128),
+               dict(value_row_stride=40, value_head_stride=40), dict(value_row_stride=64, value_head_stride=0), dict(value_row_stride=33, value_head_stride=32)):
+        assert L.psl_rows_read(C.byref(_args(**kw)), None) == -1 and b"overlap" in L.psl_last_error(), kw
