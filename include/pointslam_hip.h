@@ -396,7 +396,10 @@ int psl_rows_read(const psl_rows_args* a, void* stream);
  * prob (may be NULL) is its weight over that sum.  T <= 0 or top_p <= 0: the first entry of the order.  A score of +inf
  * takes all.  A row with no entry to draw gives index -1, prob 0.  Weights and sums are fp64 and of one fixed order.
  * Per-row parameters are device arrays [n_rows]; a NULL one means the value for all rows beside it.  ABI v8.
- * ws: psl_draw_ws_bytes bytes, 256-byte aligned, in use until the work on `stream` has finished. */
+ * ws: 256-byte aligned, in use until the work on `stream` has finished.  psl_draw_ws_bytes is enough for any draws from rows of that
+ * size; psl_draw_call_ws_bytes (ABI v9) is what a call with these sizes and limits needs: 256 bytes where up to 16 384 entries
+ * of a row are handled in one launch, which keeps them in LDS (up to 1 024 draws of a row, 4 096 with limits).  Of `a` it looks at the
+ * sizes, the limits for all rows, and whether per-row ones are there. */
 typedef struct psl_draw_args {
   int32_t n_rows, n_cols, n_draws;      /* n_rows <= 65535; draws per row */
   int32_t dtype;                        /* psl_dtype of scores */
@@ -419,6 +422,7 @@ typedef struct psl_draw_args {
   int64_t ws_bytes;
 } psl_draw_args;
 int64_t psl_draw_ws_bytes(int32_t n_rows, int32_t n_cols);
+int64_t psl_draw_call_ws_bytes(const psl_draw_args* a);
 int psl_draw_indices(const psl_draw_args* a, void* stream);
 
 /* ---- multi-GPU exchange ("periodic RCCL all-gather over xGMI of newly-added

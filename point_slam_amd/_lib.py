@@ -17,11 +17,12 @@ class PslError(RuntimeError):
     pass
 
 
-ABI_VERSION = 8     # include/pointslam_hip.h: psl_abi_version(); v2: psl_render_args.z_vals; v3: exposure blocks,
+ABI_VERSION = 9     # include/pointslam_hip.h: psl_abi_version(); v2: psl_render_args.z_vals; v3: exposure blocks,
 #                     full-image pixel indices in psl_track_args, step0_params in psl_map_args; v4: psl_dedupe_count / psl_dedupe_blocks,
 #                     psl_comm_* / psl_allgather_new_points (RCCL inside the library), psl_map_args refinement fields;
 #                     v5: psl_allgather_decide (rank-invariant capacity decision), psl_selftest_math; v6: psl_comm_reserve, psl_pose_const_speed, psl_selftest_traffic;
-#                     v8: psl_rows_write / psl_rows_read (feature rows in 8 or 4 bits), psl_draw_ws_bytes / psl_draw_indices (draws from scores)
+#                     v8: psl_rows_write / psl_rows_read (feature rows in 8 or 4 bits), psl_draw_ws_bytes / psl_draw_indices (draws from scores);
+#                     v9: psl_draw_call_ws_bytes
 EXPOSURE_DIM, EXPOSURE_MLP_FLOATS = 8, 2700
 
 
@@ -171,6 +172,7 @@ _SIGS = {
     "psl_rows_write": (C.c_int, [C.POINTER(psl_rows_args), C.c_void_p]),
     "psl_rows_read": (C.c_int, [C.POINTER(psl_rows_args), C.c_void_p]),
     "psl_draw_ws_bytes": (C.c_int64, [C.c_int32, C.c_int32]),
+    "psl_draw_call_ws_bytes": (C.c_int64, [C.POINTER(psl_draw_args)]),
     "psl_draw_indices": (C.c_int, [C.POINTER(psl_draw_args), C.c_void_p]),
     "psl_sync": (C.c_int, [C.c_void_p, C.c_void_p]),
     "psl_profile_enable": (C.c_int, [C.c_void_p, C.c_int]),

@@ -1316,8 +1316,9 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   if (parts > most) parts = most;
   l.part_len = (int)(((cols + parts - 1) / parts + 2047) / 2048 * 2048);
   l.n_parts = (int)((cols + l.part_len - 1) / l.part_len);
-  // Lists hold a quarter of a row: more entries in one bin mean that many equal scores, and then the row itself is read.
-  l.list_cap = (int)(cols / 4 > 4096 ? cols / 4 : 4096);
+  // Lists hold a quarter of a row (all of it up to 4 096 entries): more entries in one bin mean that many equal scores, and then the
+  // row itself is read.
+  l.list_cap = (int)(cols / 4 > 4096 ? cols / 4 : cols < 4096 ? cols : 4096);
   l.part_max = take(sizeof(unsigned) * n_rows * l.n_parts);
   l.part_min = take(sizeof(unsigned) * n_rows * l.n_parts);
   // maxima for last_bin: up to kTops of a row (kMaxParts * 256 / 64), of four lanes or more
@@ -1333,11 +1334,17 @@ static DrawLayout draw_layout(long long n_rows, long long n_cols) {
   l.total = o;
   return l;
 }
-template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
-  // Short rows in one launch (1 x 2 048, top-k and top-p: 15 us, in seven 27; 256 x 16 384: 26 and 39).  A row's draws are then
-  // one workgroup's: without limits, where three launches would do, up to 1 024 of them (1 x 16 384: 18 and 21 us; for 2 048 24 and
-  // 21), with limits up to 4 096 (1 x 16 384, both: 30 and 35 us; for 16 384 46 and 42).
-  if (a.n_cols <= kRowCols && a.n_draws <= (a.cuts ? 4096 : 1024)) {
+// whether any row may have a limit, as far as the host knows
+static bool may_cut(const psl_draw_args* q) {
+  return q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
+}
+// Short rows in one launch (1 x 2 048, top-k and top-p: 13.3 us, in seven 27; 256 x 16 384: 26 and 39).  A row's draws are then
+// one workgroup's: without limits, where three launches would do, up to 1 024 of them (1 x 16 384: 18 and 21 us; for 2 048 24 and
+// 21), with limits up to 4 096 (1 x 16 384, both: 30 and 35 us; for 16 384 46 and 42).
+static bool in_one_launch(const psl_draw_args* q) { return q->n_cols <= kRowCols && q->n_draws <= (may_cut(q) ? 4096 : 1024); }
+constexpr int64_t kNoWorkspace = 256;      // what a call asks for that uses none: `ws` is a pointer all the same
+template <int DT> static void launch_draw(const DrawArgs& a, bool one_launch, hipStream_t s) {
+  if (one_launch) {
     hipLaunchKernelGGL(k_draw_row<DT>, dim3(a.n_rows), dim3(1024), 0, s, a);
     return;
   }
@@ -1355,13 +1362,18 @@ template <int DT> static void launch_draw(const DrawArgs& a, hipStream_t s) {
 }  // namespace psl
 using namespace psl;
 
+#define PSL_BAD(...) do { set_error(__VA_ARGS__); return PSL_ERR_ARG; } while (0)
 extern "C" int64_t psl_draw_ws_bytes(int32_t n_rows, int32_t n_cols) {
-  if (n_rows < 0 || n_cols < 0 || n_rows > 65535 || n_cols > 0x7f000000) { set_error("psl_draw_ws_bytes: %d rows of %d", n_rows, n_cols); return PSL_ERR_ARG; }
+  if (n_rows < 0 || n_cols < 0 || n_rows > 65535 || n_cols > 0x7f000000) PSL_BAD("psl_draw_ws_bytes: %d rows of %d", n_rows, n_cols);
   return (int64_t)draw_layout(n_rows, n_cols).total;
+}
+extern "C" int64_t psl_draw_call_ws_bytes(const psl_draw_args* q) {
+  if (!q) PSL_BAD("psl_draw_call_ws_bytes: null argument");
+  const int64_t all = psl_draw_ws_bytes(q->n_rows, q->n_cols);
+  return all > kNoWorkspace && in_one_launch(q) ? kNoWorkspace : all;
 }
 
 extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
-#define PSL_BAD(...) do { set_error(__VA_ARGS__); return PSL_ERR_ARG; } while (0)
   if (!q) PSL_BAD("psl_draw_indices: null argument");
   if (q->dtype < PSL_F32 || q->dtype > PSL_F16) PSL_BAD("psl_draw_indices: unknown dtype %d", q->dtype);
   if (q->n_rows < 0 || q->n_rows > 65535 || q->n_cols < 0 || q->n_cols > 0x7f000000 || q->n_draws < 0)
@@ -1379,23 +1391,28 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   if ((!q->temperature && q->temperature_all != q->temperature_all) || (!q->top_p && q->top_p_all != q->top_p_all) ||
       (!q->min_p && q->min_p_all != q->min_p_all))
     PSL_BAD("psl_draw_indices: NaN parameter");
+  const bool one_launch = in_one_launch(q);
   const DrawLayout l = draw_layout(q->n_rows, q->n_cols);
-  if (q->ws_bytes < (int64_t)l.total) PSL_BAD("psl_draw_indices: workspace of %lld bytes, %lld needed", (long long)q->ws_bytes, (long long)l.total);
-  DrawArgs a;
+  const int64_t need = one_launch ? kNoWorkspace : (int64_t)l.total;
+  if (q->ws_bytes < need) PSL_BAD("psl_draw_indices: workspace of %lld bytes, %lld needed", (long long)q->ws_bytes, (long long)need);
+  DrawArgs a{};
   a.n_rows = q->n_rows; a.n_cols = q->n_cols; a.n_draws = q->n_draws;
   a.scores = q->scores; a.stride = q->score_stride; a.mask = q->mask; a.mask_stride = q->mask_stride;
   a.temperature = q->temperature; a.top_k = q->top_k; a.top_p = q->top_p; a.min_p = q->min_p;
   a.t_all = q->temperature_all; a.p_all = q->top_p_all; a.m_all = q->min_p_all; a.k_all = q->top_k_all;
   a.u = q->u; a.u_stride = q->u_stride; a.idx = q->idx; a.prob = q->prob;
-  char* w = (char*)q->ws;
-  a.state = (DrawState*)(w + l.state); a.cut = (DrawCut*)(w + l.cut); a.chunk_sum = (double*)(w + l.chunk_sum); a.group = (DrawGroup*)(w + l.group);
-  a.group_incl = (double*)(w + l.group_incl);
-  a.n_chunks = l.n_chunks; a.chunk = l.chunk;
-  a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.n_parts = l.n_parts; a.part_len = l.part_len;
-  a.tops = (unsigned*)(w + l.tops); a.top_lanes = l.top_lanes; a.n_tops = l.n_tops;
-  a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
-  a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b); a.list_cap = l.list_cap;
-  a.cuts = q->temperature || q->top_k || q->top_p || !(q->temperature_all > 0.0) || q->top_k_all > 0 || q->top_p_all < 1.0;
+  // (the row kernel keeps everything in LDS: its pointers into the workspace stay null)
+  if (!one_launch) {
+    char* w = (char*)q->ws;
+    a.state = (DrawState*)(w + l.state); a.cut = (DrawCut*)(w + l.cut); a.chunk_sum = (double*)(w + l.chunk_sum); a.group = (DrawGroup*)(w + l.group);
+    a.group_incl = (double*)(w + l.group_incl);
+    a.part_max = (unsigned*)(w + l.part_max); a.part_min = (unsigned*)(w + l.part_min); a.tops = (unsigned*)(w + l.tops);
+    a.bin_cnt = (unsigned*)(w + l.bin_cnt); a.bin_mass = (u64*)(w + l.bin_mass); a.bin_excl = (double*)(w + l.bin_excl);
+    a.list_a = (u64*)(w + l.list_a); a.list_b = (u64*)(w + l.list_b);
+  }
+  a.n_chunks = l.n_chunks; a.chunk = l.chunk; a.n_parts = l.n_parts; a.part_len = l.part_len; a.top_lanes = l.top_lanes; a.n_tops = l.n_tops;
+  a.list_cap = l.list_cap;
+  a.cuts = may_cut(q);
   // A row's workgroup draws from its list: 64 x 131 072 with top-k and top-p, one draw of each: 42 us, by sums and k_draw_pick 59; for
   // 16 384 draws 52 and 84; of a single row 43 and 43, and more draws want more workgroups.
   a.listed_draws = a.cuts && a.n_draws <= 16384;
@@ -1411,9 +1428,9 @@ extern "C" int psl_draw_indices(const psl_draw_args* q, void* stream) {
   while ((long long)a.n_chunks * (per_chunk / a.place_groups) > (a.n_draws / 2 > a.n_cols / kGroup ? kPlaces : a.n_chunks))
     a.place_groups = per_chunk % (2 * a.place_groups) == 0 ? 2 * a.place_groups : per_chunk;
   hipStream_t s = (hipStream_t)stream;
-  if (q->dtype == PSL_F32) launch_draw<PSL_F32>(a, s);
-  else if (q->dtype == PSL_BF16) launch_draw<PSL_BF16>(a, s);
-  else launch_draw<PSL_F16>(a, s);
+  if (q->dtype == PSL_F32) launch_draw<PSL_F32>(a, one_launch, s);
+  else if (q->dtype == PSL_BF16) launch_draw<PSL_BF16>(a, one_launch, s);
+  else launch_draw<PSL_F16>(a, one_launch, s);
   PSL_LAUNCH_CHECK();
   return PSL_OK;
 #undef PSL_BAD

@@ -113,7 +113,7 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     idx = torch.empty(R, n, dtype=torch.int32, device=dev)
     prob = torch.empty(R, n, dtype=torch.float32, device=dev) if with_prob else None
     if R and n:
-        a.ws_bytes = _lib.check(_lib.lib().psl_draw_ws_bytes(R, V), "psl_draw_ws_bytes")
+        a.ws_bytes = _lib.check(_lib.lib().psl_draw_call_ws_bytes(C.byref(a)), "psl_draw_call_ws_bytes")
         ws = torch.empty(a.ws_bytes, dtype=torch.uint8, device=dev)
         a.idx, a.prob, a.ws = idx.data_ptr(), prob.data_ptr() if with_prob else None, ws.data_ptr()
         _lib.call_on(dev, "psl_draw_indices", a)

@@ -485,3 +485,49 @@ def test_u_on_a_border_with_nothing_to_draw_behind_it(how):
     u = torch.full((R, 3), 0.5)
     idx = frame_ops.draw_indices(s.cuda(), u.cuda(), mask=ok.cuda() if how == "masked" else None).cpu()
     assert bool(((idx == 1599) | (idx == 2497)).all()), idx[(idx != 1599) & (idx != 2497)].unique()
+
+
+def test_a_call_asks_for_the_workspace_it_uses():
+    L = _lib.lib()
+
+    def need(R, V, n, **kw):
+        return L.psl_draw_call_ws_bytes(C.byref(_args(n_rows=R, n_cols=V, n_draws=n, **kw)))
+    some = C.c_float(0.0)
+    for R, V, n, kw in ((1, 2048, 1, {}), (4096, 2048, 1, dict(top_k_all=50)), (65535, 2048, 1, {}), (3, 16384, 1024, {}), (3, 16384, 4096, dict(top_p_all=0.9)),
+                        (3, 0, 7, {}), (2, 500, 4096, dict(temperature=C.addressof(some))), (2, 500, 4096, dict(temperature_all=0.0))):
+        assert need(R, V, n, **kw) == 256, (R, V, n, kw)
+    for R, V, n, kw in ((3, 16384, 1025, {}), (3, 16384, 4097, dict(top_p_all=0.9)), (3, 16385, 1, {}), (3, 2048, 1025, dict(min_p_all=0.1)), (2, 816000, 5, dict(top_k_all=9))):
+        assert need(R, V, n, **kw) == L.psl_draw_ws_bytes(R, V), (R, V, n, kw)
+    assert L.psl_draw_ws_bytes(4096, 2048) < 4096 * 64 * 1024
+    assert need(-1, 5, 1) == -1 and need(5, -1, 1) == -1 and need(65536, 5, 1) == -1 and L.psl_draw_call_ws_bytes(None) == -1
+    for kw in (dict(ws_bytes=255), dict(n_draws=2000, ws_bytes=L.psl_draw_ws_bytes(1, 16) - 1)):
+        assert L.psl_draw_indices(C.byref(_args(**kw)), None) == -1 and b"workspace" in L.psl_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("R,V,n,k", [(7, 2048, 5, 50), (7, 16384, 1024, 0), (2, 700, 4096, 300), (2, 700, 4097, 300), (3, 3000, 1025, 0), (3, 16385, 2, 900),
+                                     (3, 16385, 20000, 9000), (2, 50021, 3, 0)])
+def test_nothing_behind_the_workspace_is_written(R, V, n, k):
+    s, u = _scores(R, V, "f32").cuda(), torch.rand(R, n).cuda()
+    want = frame_ops.draw_indices(s, u, top_k=k)
+    idx = torch.empty(R, n, dtype=torch.int32, device="cuda")
+    a = _lib.psl_draw_args(n_rows=R, n_cols=V, n_draws=n, scores=s.data_ptr(), score_stride=V, u=u.data_ptr(), u_stride=n, idx=idx.data_ptr(),
+                           temperature_all=1.0, top_p_all=1.0, top_k_all=k)
+    a.ws_bytes = _lib.lib().psl_draw_call_ws_bytes(C.byref(a))
+    ws = torch.full((a.ws_bytes + 4096,), 0xa5, dtype=torch.uint8, device="cuda")
+    a.ws = ws.data_ptr()
+    _lib.call_on(s.device, "psl_draw_indices", a)
+    assert torch.equal(idx, want) and (ws[a.ws_bytes:] == 0xa5).all()
+
+
+@gpu
+def test_many_short_rows_take_no_workspace_to_speak_of():
+    s, u = _scores(4096, 2048, "bf16").cuda(), torch.rand(4096, 1, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    idx = frame_ops.draw_indices(s, u, top_k=40, top_p=0.9)
+    assert torch.cuda.max_memory_allocated() - before <= 1 << 20
+    for r in (0, 1, 2047, 4095):
+        want, _ = DO.draws(s[r].double().cpu().numpy(), u[r].cpu().numpy(), top_k=40, top_p=0.9)
+        assert int(idx[r, 0]) == want[0]
