@@ -20,7 +20,7 @@ the per-frame exposure latents (:399-401,530-548; Tracker.py:305-311).  BA is no
 from __future__ import annotations
 
 import ctypes as C
-from typing import List, Optional
+from typing import List, Mapping, Optional
 
 import torch
 
@@ -82,6 +82,18 @@ def camera_tensor_from_c2w(c2w: torch.Tensor) -> torch.Tensor:
     return torch.from_numpy(np.concatenate([q, m[:3, 3]])).float()
 
 
+def score_cut(section: dict) -> Optional[dict]:
+    """tracking / mapping section of a configuration -> the parameters of its `score_sampling`, or None where pixels are drawn
+    uniformly (no such key, None, False).  {} is score sampling with every default."""
+    cut = section.get("score_sampling")
+    if not cut and not isinstance(cut, Mapping):
+        return None
+    known = ("temperature", "top_k", "top_p", "min_p", "floor")
+    if not isinstance(cut, Mapping) or any(k not in known for k in cut):
+        raise ValueError(f"score_sampling: a dict of {', '.join(known)}, got {cut!r}")
+    return cut
+
+
 class HipSLAM:
     def __init__(self, cfg, cam: dict, device="cuda:0", max_points=2_500_000, engine="native", decoders=None):
         self.cfg, self.cam, self.device, self.engine = cfg, cam, torch.device(device), engine
@@ -91,7 +103,8 @@ class HipSLAM:
                                       "native engine, or HipRenderer inside the reference's own Tracker/Mapper")
         cfgd = dict(cfg)
         cfgd["mapping"] = dict(cfg["mapping"], device=str(device))
-        if engine != "native" and (cfg["tracking"].get("score_sampling") or cfg["mapping"].get("score_sampling")):
+        by_score = [score_cut(cfg[k]) is not None for k in ("tracking", "mapping")]
+        if engine != "native" and any(by_score):
             raise NotImplementedError("score_sampling draws full-image pixels for the native engine")
         self.npc = HipNeuralPointCloud(cfgd, max_points=max_points, device=str(device))
         import types
@@ -260,11 +273,11 @@ class HipSLAM:
         L = _lib.lib()
         tr, cam = self.cfg["tracking"], self.cam
         eh, ew = tr["ignore_edge_H"], tr["ignore_edge_W"]
-        by_score = tr.get("score_sampling")
-        full = bool(tr.get("sample_with_color_grad", False) or by_score)
+        by_score = score_cut(tr)
+        full = bool(tr.get("sample_with_color_grad", False)) or by_score is not None
         if draws is not None:
             idx, fb = draws
-        elif by_score:
+        elif by_score is not None:
             idx = self.score_draws([frame], n_iters * n_pix, by_score, eh, ew).reshape(n_iters, n_pix)
             fb = torch.zeros(n_iters, 2, 32, device=self.device).normal_(mean=0, std=0.01)
         elif full:
@@ -501,10 +514,11 @@ class HipSLAM:
         mp, cam, dev = self.cfg["mapping"], self.cam, self.device
         W = len(window)
         n = W * ppf
+        by_score = score_cut(mp)
         if draws is not None:
             idx, fb = draws
-        elif mp.get("score_sampling"):
-            idx = self.score_draws(window, n_iters * ppf, mp["score_sampling"]).reshape(W, n_iters, ppf)
+        elif by_score is not None:
+            idx = self.score_draws(window, n_iters * ppf, by_score).reshape(W, n_iters, ppf)
             idx = idx.transpose(0, 1).reshape(n_iters, n).contiguous()
             fb = torch.zeros(n_iters, 2, 32, device=dev).normal_(mean=0, std=0.01)
         else:

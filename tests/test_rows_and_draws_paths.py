@@ -373,3 +373,44 @@ def test_a_mapped_frame_end_to_end():
     # a rendered depth is a weighted mean of samples at 0.98 .. 1.02 of the sensor depth, whatever the features are
     assert (full[0] - q8[0]).abs().max() <= 0.041 * gd.max() and torch.isfinite(q8[2]).all()
     assert not torch.equal(full[2], q8[2])
+
+
+def _small_slam(tracking=None, mapping=None, **kw):
+    from point_slam_amd.slam import HipSLAM
+    cfg = base_cfg()
+    if tracking is not None:
+        cfg["tracking"]["score_sampling"] = tracking
+    if mapping is not None:
+        cfg["mapping"]["score_sampling"] = mapping
+    return HipSLAM(cfg, dict(H=120, W=160, fx=100.0, fy=100.0, cx=80.0, cy=60.0), **kw)
+
+
+def test_score_sampling_with_nothing_but_defaults_is_score_sampling():
+    """{} names no parameter and takes every default; only an absent key, None and False mean uniform draws."""
+    from point_slam_amd.slam import score_cut
+    assert score_cut({}) is None and score_cut({"score_sampling": None}) is None and score_cut({"score_sampling": False}) is None
+    assert score_cut({"score_sampling": {}}) == {} and score_cut({"score_sampling": {"top_p": 0.9}}) == {"top_p": 0.9}
+    for bad in (True, 0.7, "top_p", [("top_p", 0.9)], {"topp": 0.9}, {"mask": None}, {"with_prob": True}):
+        with pytest.raises(ValueError, match="score_sampling"):
+            score_cut({"score_sampling": bad})
+    for where in ("tracking", "mapping"):
+        with pytest.raises(NotImplementedError):
+            _small_slam(**{where: {}}, engine="dropin")
+        with pytest.raises(ValueError, match="score_sampling"):
+            _small_slam(**{where: True})
+
+
+@gpu
+def test_the_loops_draw_by_score_with_nothing_but_defaults(monkeypatch):
+    cfg = base_cfg()
+    cfg["tracking"].update(score_sampling={}, iters=2, pixels=100)
+    cfg["mapping"].update(score_sampling={}, iters=3, pixels=200, pixels_adding=200)
+    from point_slam_amd.slam import HipSLAM, camera_tensor_from_c2w
+    cam, s, frames = _slam(cfg)
+    calls = []
+    draws = HipSLAM.score_draws
+    monkeypatch.setattr(HipSLAM, "score_draws", lambda self, *a, **kw: calls.append(a[2]) or draws(self, *a, **kw))
+    s.map(frames[0], frames[0].c2w, n_iters=3, fixed_iters=True)
+    assert calls == [{}]
+    s.track(frames[1], camera_tensor_from_c2w(frames[1].c2w))
+    assert calls == [{}, {}] and torch.isfinite(s.last_losses).all()
