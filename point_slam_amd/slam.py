@@ -243,10 +243,18 @@ class HipSLAM:
         with weights (colour-gradient magnitude + floor) ** (1 / temperature) over the pixels with sensor depth inside the
         border, the tail cut by top_k / top_p / min_p (frame_ops.draw_indices; `cut` = tracking.score_sampling or
         mapping.score_sampling, e.g. {"temperature": 0.7, "top_p": 0.9}).  A soft form of sample_with_color_grad, which takes
-        pixels of the hard top-k alike.  floor (default 1e-3) is what a flat pixel weighs."""
+        pixels of the hard top-k alike.  floor (default 1e-3) is what a flat pixel weighs; with 0 flat pixels
+        are drawn where nothing else is left.  A frame with no sensor depth inside the border draws the first pixel there, whose
+        missing depth every loop filters."""
         from . import frame_ops
         par = dict(cut)
         floor = float(par.pop("floor", 1e-3))
+        if not 0.0 <= floor < float("inf"):
+            raise ValueError(f"score_sampling: floor {floor}: a number, 0 or above")
+        floor = max(floor, torch.finfo(torch.float64).tiny)      # (a score, not -inf: a frame without any gradient has pixels too)
+        H_, W_ = self.cam["H"], self.cam["W"]
+        if not (0 <= 2 * edge_h < H_ and 0 <= 2 * edge_w < W_):
+            raise ValueError(f"a border of {edge_h} x {edge_w} leaves nothing of {H_} x {W_} pixels")
         scores, mask = [], []
         for f in frames:
             if f.grad_scores is None or f.grad_scores[0] != floor:
@@ -260,7 +268,7 @@ class HipSLAM:
             mask.append(m.reshape(-1))
         u = torch.rand(len(frames), n_draws, device=self.device)
         idx = frame_ops.draw_indices(torch.stack(scores), u, mask=torch.stack(mask), **par)
-        return idx.clamp_(min=0)          # a frame without any sensor depth: pixel 0, whose missing depth every loop filters
+        return idx.masked_fill_(idx < 0, edge_h * W_ + edge_w)
 
     def _exposure_block(self, feats, lr_mlp, lr_feat=0.001):
         """psl_exposure_args over the shared MLP blob and `feats` ([8] or [F,8]); returns (struct, keep-alive)."""

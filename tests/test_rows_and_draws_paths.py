@@ -414,3 +414,42 @@ def test_the_loops_draw_by_score_with_nothing_but_defaults(monkeypatch):
     assert calls == [{}]
     s.track(frames[1], camera_tensor_from_c2w(frames[1].c2w))
     assert calls == [{}, {}] and torch.isfinite(s.last_losses).all()
+
+
+@gpu
+def test_a_frame_with_depth_in_its_border_only_draws_a_pixel_the_loops_filter():
+    cam, s, frames = _slam(base_cfg())
+    f = frames[0]
+    f.depth[10:-10, 15:-15] = 0.0
+    assert float(f.depth[0, 0]) > 0                          # a pixel of the border, which the loops would take
+    idx = s.score_draws([f], 50, {"temperature": 0.7}, edge_h=10, edge_w=15)
+    assert (f.depth.reshape(-1)[idx.long()] == 0).all()
+    v, u = idx // cam["W"], idx % cam["W"]
+    assert (v >= 10).all() and (v < cam["H"] - 10).all() and (u >= 15).all() and (u < cam["W"] - 15).all()
+
+
+@gpu
+def test_the_floor_of_flat_pixels():
+    cam, s, frames = _slam(base_cfg())
+    for floor in (-1e-3, float("nan"), float("inf")):
+        with pytest.raises(ValueError, match="floor"):
+            s.score_draws(frames[:1], 5, {"floor": floor})
+    f = frames[0]
+    f.color[:, :160] = 0.5                                   # flat but for the half that is not
+    flat = (s.grad_mag(f) == 0).reshape(-1)
+    assert int(flat.sum()) > 1000
+    idx = s.score_draws([f], 5000, {"floor": 0.0}).long()
+    assert not flat[idx].any() and (f.depth.reshape(-1)[idx] > 0).all()
+    assert flat[s.score_draws([f], 5000, {"floor": 10.0}).long()].any()
+    frames[1].color.fill_(0.5)                               # no gradient anywhere: every pixel with depth alike
+    for floor in (0.0, 1e-3):
+        idx = s.score_draws(frames[1:2], 2000, {"floor": floor, "top_p": 0.9}).long()
+        assert (frames[1].depth.reshape(-1)[idx] > 0).all() and idx.unique().numel() > 1000
+
+
+@gpu
+def test_a_border_that_leaves_no_pixel_is_refused():
+    cam, s, frames = _slam(base_cfg())
+    for eh, ew in ((cam["H"] // 2, 0), (0, cam["W"] // 2), (cam["H"], cam["W"]), (-1, 0)):
+        with pytest.raises(ValueError, match="border"):
+            s.score_draws(frames[:1], 5, {}, edge_h=eh, edge_w=ew)
