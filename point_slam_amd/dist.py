@@ -213,7 +213,7 @@ def merge_new_points(npc, n_base: int, group=None, dedupe: bool = True, transpor
     rows in the records (module docstring)."""
     tr = transport or _TorchTransport(group)
     rw = _RowWire(wire)
-    c_feat, c_rad = (3, 67) if wire is None else (4, 3)           # codes start on a 16-byte boundary
+    c_feat, c_rad = (3, 67) if wire is None else (4, 3)           # codes start on 8 bytes (rows of 88: int8, e4m3)
     n_now = npc.pts_num()
     n_new = n_now - n_base
     dev = npc.get_geo_feats().device

@@ -531,3 +531,34 @@ def test_many_short_rows_take_no_workspace_to_speak_of():
     for r in (0, 1, 2047, 4095):
         want, _ = DO.draws(s[r].double().cpu().numpy(), u[r].cpu().numpy(), top_k=40, top_p=0.9)
         assert int(idx[r, 0]) == want[0]
+
+
+@gpu
+def test_as_many_rows_as_a_call_takes():
+    R = 65535
+    for V, kw in ((2100, dict(top_k=50, top_p=0.9)), (16385, dict()), (16385, dict(top_k=90, top_p=0.9))):
+        s = _scores(1, V, "bf16", seed=V).cuda()
+        u = torch.rand(R, 1, device="cuda")
+        idx, prob = frame_ops.draw_indices(s.expand(R, V), u, with_prob=True, **kw)
+        one, p1 = frame_ops.draw_indices(s, u.t().contiguous()[:, :1000], with_prob=True, **kw)
+        want, p = DO.draws(s[0].double().cpu().numpy(), u[:, 0].cpu().numpy(), **kw)
+        assert np.array_equal(idx[:, 0].cpu().numpy(), want) and torch.equal(idx[:1000, 0], one[0]) and torch.equal(prob[:1000, 0], p1[0])
+        assert np.all(np.abs(prob[:, 0].cpu().double().numpy() - p) <= 1.001 * 2.0 ** -24 * p)
+
+
+@gpu
+def test_calls_on_several_streams_at_once():
+    jobs = [(_scores(3, V, "f32", seed=V).cuda(), torch.rand(3, n).cuda(), kw) for V, n, kw in
+            ((200000, 20000, dict(top_p=0.95)), (40000, 5, dict(top_k=300, top_p=0.9)), (3000, 100, dict(top_k=50)), (120000, 3000, dict(min_p=1e-3)))]
+    want = [frame_ops.draw_indices(s, u, with_prob=True, **kw) for s, u, kw in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(5):
+        for k, (s, u, kw) in enumerate(jobs):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(frame_ops.draw_indices(s, u, with_prob=True, **kw))
+    torch.cuda.synchronize()
+    for k, w in enumerate(want):
+        for g in got[k]:
+            assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1]), k

@@ -453,3 +453,70 @@ def test_a_border_that_leaves_no_pixel_is_refused():
     for eh, ew in ((cam["H"] // 2, 0), (0, cam["W"] // 2), (cam["H"], cam["W"]), (-1, 0)):
         with pytest.raises(ValueError, match="border"):
             s.score_draws(frames[:1], 5, {}, edge_h=eh, edge_w=ew)
+
+
+def _owner_worker(rank, world, port, q, fmt):
+    import torch.distributed as dist
+    os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    from point_slam_amd import dist as PD
+    from tests.test_dist_gloo import FakeCloud
+    PD._RowWire = _HostWire
+    g = torch.Generator().manual_seed(100)
+    cloud = FakeCloud(torch.rand(10, 3, generator=g) + 5.0, torch.randn(10, 32, generator=g), torch.randn(10, 32, generator=g))
+    before = torch.stack([cloud.geo, cloud.col], 1).clone()
+    theta = torch.arange(6.0)
+    sync = PD.FrameParallelSync(cloud, theta, n_color=4, wire=fmt, merge="owner")
+    gr = torch.Generator().manual_seed(rank + 1)
+    rows = [0, 1] if rank == 0 else [1, 2]
+    sync.note_rows(cloud, torch.tensor(rows))
+    for r in rows:
+        cloud.geo[r] += torch.randn(32, generator=gr) * 0.1; cloud.col[r] += torch.randn(32, generator=gr) * 0.1
+    moved = torch.stack([cloud.geo[:10], cloud.col[:10]], 1) - before
+    theta += rank + 1
+    counts = sync.exchange(cloud, theta)                     # no new points: the records of that half are empty
+    q.put(tuple(x.numpy() if torch.is_tensor(x) else x for x in (rank, counts, torch.stack([cloud.geo, cloud.col], 1), moved, before, theta)))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_owner_writes_with_quantised_records_world2(fmt):
+    """Of a row of the seed map that both ranks trained the lowest rank's change counts, as sent; the decoder stays fp32."""
+    s = socket.socket(); s.bind(("127.0.0.1", 0)); port = s.getsockname()[1]; s.close()
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    procs = [ctx.Process(target=_owner_worker, args=(r, 2, port, q, fmt)) for r in range(2)]
+    for p in procs:
+        p.start()
+    res = sorted([q.get(timeout=120) for _ in range(2)], key=lambda x: x[0])
+    for p in procs:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    (_, c0, f0, d0, before, t0), (_, c1, f1, d1, _, t1) = [[torch.from_numpy(x) if isinstance(x, np.ndarray) else x for x in r] for r in res]
+    assert c0 == c1 == [0, 0] and torch.equal(f0, f1) and torch.equal(t0[:4], t1[:4]) and torch.equal(t0[:4], torch.arange(4.0) + 1.5)
+    want = before.clone()
+    q0, q1 = _stands_for(d0, fmt), _stands_for(d1, fmt)
+    want[0] += q0[0]; want[1] += q0[1]; want[2] += q1[2]
+    assert torch.equal(f0, want)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_records_of_halves_match_the_oracle(fmt, dtype):
+    """bf16 and fp16 values into records, several groups to a head, the codes where a row of records begins on a multiple of 4 bytes only."""
+    from point_slam_amd import row_store
+    v = (torch.randn(301, 3, 64) * 0.1).to(dtype)
+    for group in (64, 16):
+        cw, sw = row_store.record_floats(3, 64, fmt, group)
+        q, s = RO.quantize(v.float().numpy(), fmt, group)
+        for code_col, scale_col, width in ((0, cw, cw + sw), (sw + 1, 1, cw + sw + 4), (2, cw + 5, cw + sw + 5)):
+            rec = torch.full((301, width), 7.0, device="cuda")
+            row_store.write_records(rec, v.cuda(), fmt, code_col, scale_col, group)
+            back = row_store.read_records(rec, 3, 64, fmt, code_col, scale_col, group).cpu()
+            assert torch.equal(back, torch.from_numpy(RO.values(q, s)))
+            host = rec.cpu()
+            assert torch.equal(host[:, scale_col:scale_col + sw], torch.from_numpy(s).reshape(301, sw))
+            keep = torch.ones(width, dtype=torch.bool); keep[code_col:code_col + cw] = False; keep[scale_col:scale_col + sw] = False
+            assert (host[:, keep] == 7.0).all()
