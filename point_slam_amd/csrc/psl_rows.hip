@@ -9,8 +9,9 @@
 //   once more, to four bits, is the rounding of the exact quotient.
 //
 // Bound: memory.  A thread owns VEC consecutive values; the lanes of a group find its maximum by moves between lanes, so a value
-// is read once and lives in registers until its code is stored.  2.5 M rows of 2 x 32 fp32 to 8 bits and back: 140 and 142 us
-// each by itself, 164 and 150 in turn -- the 820 MB that each reads and writes at 5.8 and 5.2 TB/s, where a copy of 256 MiB reaches 5.4.
+// is read once and lives in registers until its code is stored.  2.5 M rows of 2 x 32 fp32 to 8 bits and back: 295 us
+// for the pair, 5.6 TB/s of the 820 MB that each reads and writes (kernel trace: 165 and 144 in turn; 140 and 142 each by itself),
+// where a copy of 1 GiB reaches 5.07 and one of 256 MiB 5.31 (codes and scales fit the 256 MB cache between the two calls).
 #include "psl_common.h"
 
 namespace psl {
@@ -331,7 +332,7 @@ __global__ __launch_bounds__(256) void k_rows_write(RowsArgs a) {
     if (c < a.chunks) {
       float q[VEC];
       quotients<FMT, VEC>(x[it], s, inv, q);
-      if (tiny) { asm volatile(""); quotients_tiny<FMT, VEC>(x[it], s, q); }      // (the asm keeps this a branch: it is never taken)
+      if (tiny) { asm volatile(""); quotients_tiny<FMT, VEC>(x[it], s, q); }      // (the asm keeps this a branch, for groups below 2^-60 alone)
       encode<FMT, VEC>(q, cd + (c * (unsigned)VEC * Code<FMT>::bits >> 3));
     }
   }

@@ -66,7 +66,8 @@ def draw_indices(scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, mask
     the lower index; temperature or a limit may be a number or a tensor [R].  `mask` (bool or uint8, [R, V] or [V]): entries
     that may be drawn -- what the others hold, NaN included, does not matter.  A vector of scores and a vector u make one row.
     Returns indices int32 [R, n] (-1 where a row has nothing to draw) and, with_prob, their probabilities fp32 [R, n] under
-    the cut distribution (what an importance weight divides by)."""
+    the cut distribution (what an importance weight divides by).  Probabilities are numbers, not part of an autograd graph: no
+    gradient reaches scores through them, whether scores require one or not."""
     one = scores.dim() == 1
     if one:
         scores, u = scores.unsqueeze(0), u.unsqueeze(0)

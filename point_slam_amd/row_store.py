@@ -4,13 +4,13 @@
 A row is `heads` x `dim` values -- the geometry and the colour feature of a neural point are two heads of 32 -- and every
 `group` of values shares one fp32 scale:
 
-    scale = max|x| / Q     Q = 127 ("int8"), 7 ("int4"), 448 ("e4m3")        code = nearest(x / scale), ties to even
+    scale = max|x| / Q     Q = 127 ("int8"), 7 ("int4"), 448 ("e4m3")        code = nearest(x / scale), ties to even; 0 for scale 0
     value = code * scale   in fp32, then converted to the type that is read
 
 so a value is off by at most half a code step (scale / 2 for the integer formats, 2^-4 of the value for e4m3's normal
 range).  A group with an infinite or NaN value reads back as NaN throughout.  dist.FrameParallelSync(wire=...) sends new
 points and trained rows in this form, checkpoint.checkpoint_dict(feature_format=...) saves them in it.
-There is no torch fallback.
+There is no torch fallback, and no gradient passes through a store.
 """
 from __future__ import annotations
 
