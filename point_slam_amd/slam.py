@@ -251,14 +251,14 @@ class HipSLAM:
         floor = float(par.pop("floor", 1e-3))
         if not 0.0 <= floor < float("inf"):
             raise ValueError(f"score_sampling: floor {floor}: a number, 0 or above")
-        floor = max(floor, torch.finfo(torch.float64).tiny)      # (a score, not -inf: a frame without any gradient has pixels too)
-        H_, W_ = self.cam["H"], self.cam["W"]
-        if not (0 <= 2 * edge_h < H_ and 0 <= 2 * edge_w < W_):
-            raise ValueError(f"a border of {edge_h} x {edge_w} leaves nothing of {H_} x {W_} pixels")
+        cam = self.cam
+        if not (0 <= 2 * edge_h < cam["H"] and 0 <= 2 * edge_w < cam["W"]):
+            raise ValueError(f"a border of {edge_h} x {edge_w} leaves nothing of {cam['H']} x {cam['W']} pixels")
         scores, mask = [], []
         for f in frames:
             if f.grad_scores is None or f.grad_scores[0] != floor:
-                f.grad_scores = (floor, torch.log(self.grad_mag(f) + floor).float().reshape(-1))
+                # -1e30, not -inf: weighs nothing beside any other score, but a frame without any gradient has pixels too
+                f.grad_scores = (floor, torch.log(self.grad_mag(f) + floor).float().reshape(-1).clamp_(min=-1e30))
             scores.append(f.grad_scores[1])
             m = f.depth > 0
             if edge_h or edge_w:
@@ -268,7 +268,7 @@ class HipSLAM:
             mask.append(m.reshape(-1))
         u = torch.rand(len(frames), n_draws, device=self.device)
         idx = frame_ops.draw_indices(torch.stack(scores), u, mask=torch.stack(mask), **par)
-        return idx.masked_fill_(idx < 0, edge_h * W_ + edge_w)
+        return idx.masked_fill_(idx < 0, edge_h * cam["W"] + edge_w)
 
     def _exposure_block(self, feats, lr_mlp, lr_feat=0.001):
         """psl_exposure_args over the shared MLP blob and `feats` ([8] or [F,8]); returns (struct, keep-alive)."""

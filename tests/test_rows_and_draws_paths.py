@@ -520,3 +520,18 @@ def test_records_of_halves_match_the_oracle(fmt, dtype):
             assert torch.equal(host[:, scale_col:scale_col + sw], torch.from_numpy(s).reshape(301, sw))
             keep = torch.ones(width, dtype=torch.bool); keep[code_col:code_col + cw] = False; keep[scale_col:scale_col + sw] = False
             assert (host[:, keep] == 7.0).all()
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [0.5, 1.0, 4.0])
+def test_a_floor_of_zero_keeps_flat_pixels_out_whatever_u_is(temperature, monkeypatch):
+    """u = 0 takes the first pixel that weighs anything at all: the flat ones in front of it must not."""
+    cam, s, frames = _slam(base_cfg())
+    f = frames[0]
+    f.color[:, :160] = 0.5
+    flat = (s.grad_mag(f) == 0).reshape(-1)
+    live = (f.depth.reshape(-1) > 0)
+    assert bool((flat & live)[:100].any()) and int((flat & live).nonzero()[0]) < int((~flat & live).nonzero()[0])
+    monkeypatch.setattr(torch, "rand", lambda *size, **kw: torch.zeros(*size, **kw))
+    idx = s.score_draws([f], 70, {"floor": 0.0, "temperature": temperature})
+    assert (idx == int((~flat & live).nonzero()[0])).all()
