@@ -1097,9 +1097,9 @@ template <int DT> __global__ __launch_bounds__(kPickThreads, 8) void k_draw_pick
 #pragma unroll
     for (int j = 0; j < 16; ++j) { sum += __builtin_amdgcn_exp2f((x[j] - top) * per_octave); x[j] = sum; }
     const float share = (float)in_block * __builtin_amdgcn_rcpf((float)mass) * sum, room = sum * 0x1p-18f;
-    // A share that is a number of at least 0 is passed by a kept entry: the sum before it is below share - room, the one it
-    // ends above share + room.  It is none, and fp64 decides, where the block's mass has no fp32 reciprocal (entries 88 temperatures below
-    // the largest; 0 / 0 for u = 0), and below 0 where the block was stepped to from one without kept entries.
+    // A share that is a number of at least 0 is passed by a kept entry: the sum in front of it is below share - room, the sum with
+    // it above share + room.  fp64 decides where the share is no number (the block's mass has no fp32 reciprocal, its entries lie 88
+    // temperatures below the largest, and u = 0 makes it 0 / 0) or below 0 (the block was stepped to from one without kept entries).
     // (the sums never fall: as many borders as lie in front of the target's)
     int at = 0, far = 0;
 #pragma unroll

@@ -1,9 +1,9 @@
 // Feature rows held in 8 or 4 bits: quantised as they are written, expanded as they are read.
 //
 // A row is heads x dim values, cut into groups of G; a group shares one fp32 scale s = max|x| / Q (Q = 127 int8, 7 int4,
-// 448 e4m3; rounded to nearest, down where Q s would not be finite) and every code is the NEAREST representable value to x / s, ties to even.  fp32's x / s cannot decide that by
-// itself: it rounds quotients beside the middle between two codes onto it (with bf16 inputs x = a / 2 that happens in
-// every few rows).  What decides is the residual x - n s, which one fma gives exactly:
+// 448 e4m3; rounded to nearest, down where Q s would not be finite) and every code is the NEAREST representable value to x / s,
+// ties to even.  fp32's x / s cannot decide that by itself: it rounds quotients beside the middle between two codes onto it (with
+// bf16 inputs x = a / 2 that happens in every few rows).  What decides is the residual x - n s, which one fma gives exactly:
 //   integers: n = rint(x / s), and x - n s against s / 2 says whether n is the nearest (it nearly always is);
 //   e4m3: the quotient rounded to ODD -- truncated, its last bit set when the residual is not zero.  Rounding that 24-bit value
 //   once more, to four bits, is the rounding of the exact quotient.
